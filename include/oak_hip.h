@@ -410,6 +410,128 @@ int oak_kmeans_plusplus(oak_ctx* ctx, const double* X, int64_t N, int32_t D, int
                         int64_t first_index, const double* uniforms, int32_t n_trials, double* centres_out,
                         int64_t* indices_out);
 
+/* ---- mixtures of models: routing, dispatch, combination ------------------------------------------ */
+/* The operators of this section and the next come in two forms.  oak_X(ctx, args): the arrays are on the host, contiguous and
+   float64 like everywhere else; the call copies them, runs on the context's stream and returns when the outputs are there.
+   oak_X_device(device, stream, args): the arrays are in the memory of `device`, of any of the types below, rows `ld` elements apart
+   (their columns are consecutive; rows may start anywhere); the call enqueues its kernels on `stream` (a hipStream_t, NULL is
+   the default stream) and returns.  It allocates nothing, keeps nothing, waits for nothing and may be captured into a graph.  The arrays must belong to
+   the HIP runtime this library is linked against (oak_device_pointer_check).
+   Sums, weights, losses and softmax statistics are float64 for float64 arrays and float32 otherwise: "wide" below. */
+#define OAK_F64   0
+#define OAK_F32   1
+#define OAK_BF16  2
+#define OAK_F16   3
+
+#define OAK_MAX_EXPERTS      1024   /* oak_route */
+#define OAK_MAX_PLAN_EXPERTS 4096   /* oak_plan, oak_dispatch, oak_combine: k-means labels are experts too */
+#define OAK_MAX_TOP_K        64
+
+#define OAK_SCORE_SOFTMAX 0
+#define OAK_SCORE_SIGMOID 1
+#define OAK_GROUP_MAX     0         /* a group's score: its highest key ...                      */
+#define OAK_GROUP_TOP2    1         /* ... or the sum of its two highest (the one, if it has one) */
+
+/* OAK_OK if p is memory of `device` known to this library's HIP runtime (a process can hold two copies of that runtime). */
+int oak_device_pointer_check(int32_t device, const void* p);
+
+/* Each row's experts.  p = softmax over the row's open scores, or sigmoid; a score is open unless its mask is 0 or it is -inf.
+   key = p + bias where there is a bias (it moves the choice, not the weights), else the score itself.  With n_groups > 1 only the
+   top_groups groups of consecutive experts with the highest group scores stay open.  The top_k highest keys are chosen, highest
+   first, ties by lower index; slots left over get expert -1 and weight 0.  weight = scale p, or scale p / sum of the chosen p.
+   A row with a NaN or +inf among its open scores gets experts -1 and weights NaN.
+   oak_route_grad: dscores from dweights for the experts chosen, recomputing p; the choice itself is not differentiated, slots whose expert is
+   not in [0, n_experts) count for nothing and a row without experts has gradient 0. */
+typedef struct oak_route_args {
+    int64_t n_rows, ld_scores, ld_mask, ld_dscores;   /* ld_mask 0: one mask for all rows */
+    int32_t n_experts, top_k, n_groups, top_groups, dtype, score, group_score, renormalise, bias_f64;
+    double scale;
+    const void* scores;        /* [n_rows, n_experts] dtype                          */
+    const void* bias;          /* [n_experts] float32 or (bias_f64) float64; or NULL  */
+    const uint8_t* mask;       /* [n_rows, n_experts] or [n_experts]; or NULL         */
+    int32_t* experts;          /* [n_rows, top_k] out; in for oak_route_grad          */
+    void* weights;             /* [n_rows, top_k] wide, out                           */
+    const void* dweights;      /* oak_route_grad: [n_rows, top_k] wide                */
+    void* dscores;             /* oak_route_grad: [n_rows, n_experts] dtype, out      */
+} oak_route_args;
+int oak_route(oak_ctx* ctx, const oak_route_args* args);
+int oak_route_device(int32_t device, void* stream, const oak_route_args* args);
+int oak_route_grad(oak_ctx* ctx, const oak_route_args* args);
+int oak_route_grad_device(int32_t device, void* stream, const oak_route_args* args);
+
+/* The order of slots by expert.  Slot n top_k + j is row n's j-th expert.  counts[e] slots belong to expert e and are the places
+   offsets[e] .. offsets[e + 1) - 1 of the order, in slot order.  positions[slot] is the slot's place (-1: its expert is not in
+   [0, n_experts)), rows[place] the row it holds (-1 from offsets[n_experts] on).
+   The device form needs workspace_ints >= oak_plan_workspace(...) int32 of scratch of its own (0 for small plans). */
+typedef struct oak_plan_args {
+    int64_t n_rows, workspace_ints;
+    int32_t top_k, n_experts;
+    const int32_t* experts;    /* [n_rows, top_k]      */
+    int32_t* rows;             /* [n_rows top_k] out   */
+    int32_t* positions;        /* [n_rows, top_k] out  */
+    int32_t* counts;           /* [n_experts] out      */
+    int32_t* offsets;          /* [n_experts + 1] out  */
+    int32_t* workspace;
+} oak_plan_args;
+int64_t oak_plan_workspace(int64_t n_rows, int32_t top_k, int32_t n_experts);
+int oak_plan(oak_ctx* ctx, const oak_plan_args* args);
+int oak_plan_device(int32_t device, void* stream, const oak_plan_args* args);
+
+/* Row arrays have n_rows rows (ld_rows apart), slot arrays n_rows top_k rows (ld_slots apart) in the plan's order; places behind
+   the last used one (offsets[n_experts]) are written as zeros where a slot array is an output.
+   oak_dispatch:      dst slots[place] = src rows[row of the place]
+   oak_combine:       dst rows[n] = sum_j weights[n, j] src slots[positions[n, j]], slots without a place count as zeros;
+                      weights NULL: all 1 (the gradient of oak_dispatch)
+   oak_combine_grad:  src slots and dout rows (ld_grad apart) -> dslots [n_rows top_k, n_cols] contiguous, dweights [n_rows, top_k] */
+typedef struct oak_mix_args {
+    int64_t n_rows, ld_rows, ld_slots, ld_grad;
+    int32_t top_k, n_experts, n_cols, dtype;
+    const int32_t* positions;
+    const int32_t* offsets;
+    const void* weights;       /* [n_rows, top_k] wide */
+    const void* src;
+    void* dst;
+    const void* dout;
+    void* dslots;
+    void* dweights;            /* wide */
+} oak_mix_args;
+int oak_dispatch(oak_ctx* ctx, const oak_mix_args* args);
+int oak_dispatch_device(int32_t device, void* stream, const oak_mix_args* args);
+int oak_combine(oak_ctx* ctx, const oak_mix_args* args);
+int oak_combine_device(int32_t device, void* stream, const oak_mix_args* args);
+int oak_combine_grad(oak_ctx* ctx, const oak_mix_args* args);
+int oak_combine_grad_device(int32_t device, void* stream, const oak_mix_args* args);
+
+/* ---- distillation ------------------------------------------------------------------------------- */
+/* Divergence of a student's class distribution q = softmax(logits / temperature) from a teacher of which only the top_k highest logits
+   are kept, and its gradient.  Entries with index -1 or value -inf are padding; entries of one class are merged (their
+   probabilities add).  Without top_lse the teacher is softmax(top / temperature) over its entries.  With top_lse[n] = log sum over ALL the
+   teacher's classes of exp(logit / temperature), p_k = exp(top_k / temperature - top_lse) and the mass left over, p_rest = max(0, 1 - sum p), is
+   one more outcome, held against the student's mass outside the entries (none if the entries are all the classes).
+     forward  L[n] = row_weight temperature^2 [ sum_k p_k log(p_k / q_k) + p_rest log(p_rest / q_rest) ]
+     reverse  L[n] = row_weight temperature^2 [ sum_k q_k log(q_k / p_k) + q_rest log(q_rest / p_rest) ]   (needs top_lse; p_rest at
+              least the resolution of top_lse, 2^-24 or for float64 2^-53)
+   dlogits (may be NULL) is the gradient of sum_n L[n].  A row of weight 0 is not read: its loss and gradient are 0.  A teacher that kept nothing
+   has loss and gradient 0.  A row with an index outside [-1, n_classes) gets loss and gradient NaN. */
+#define OAK_KL_FORWARD 0
+#define OAK_KL_REVERSE 1
+#define OAK_MAX_TEACHER 1024
+#define OAK_MAX_CLASSES (1 << 20)
+typedef struct oak_distill_args {
+    int64_t n_rows, ld_logits, ld_top, ld_index, ld_dlogits;
+    int32_t n_classes, top_k, dtype, top_dtype, lse_dtype, weight_dtype, index_64, direction;
+    double temperature;
+    const void* logits;        /* [n_rows, n_classes] dtype                */
+    const void* top;           /* [n_rows, top_k] top_dtype                */
+    const void* index;         /* [n_rows, top_k] int32 or (index_64) int64 */
+    const void* top_lse;       /* [n_rows] lse_dtype, or NULL               */
+    const void* row_weight;    /* [n_rows] weight_dtype, or NULL: all 1     */
+    void* loss;                /* [n_rows] wide, out                        */
+    void* dlogits;             /* [n_rows, n_classes] dtype, out, or NULL   */
+} oak_distill_args;
+int oak_distill(oak_ctx* ctx, const oak_distill_args* args);
+int oak_distill_device(int32_t device, void* stream, const oak_distill_args* args);
+
 /* Measurement hooks (oak_bench_*: resident Gram pass, the tail's Cholesky and the many-row triangular solve on their own) are not part
    of the drop-in surface: include/oak_hip_bench.h. */
 

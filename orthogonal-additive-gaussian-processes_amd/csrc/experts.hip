@@ -1,0 +1,882 @@
+// Mixtures of models: rows routed to their experts, laid out by expert, and the experts' answers summed with the router's weights.
+//
+//   route      x[n, e] -> the k experts of each row and their weights            (route_kernel), and the gradient (route_grad_kernel)
+//   plan       experts[n, k] -> a stable order of the slots by expert             (plan_small_kernel | plan_count / _scan / _place)
+//   dispatch   X[n] copied to the places of its slots                              (dispatch_kernel)
+//   combine    y[n] = sum_j w[n, j] F[place(n, j)], and its gradients              (combine_kernel, combine_grad_kernel)
+//
+// A hard assignment of rows (k-means labels) is the case k = 1 without a router.
+#include "lowp.h"
+
+namespace oak {
+
+// ---------------------------------------------------------------------------------------------------------------------
+// route
+// ---------------------------------------------------------------------------------------------------------------------
+// A row belongs to a team of L lanes; lane l of the team holds the experts [l VPL, (l + 1) VPL) in registers, so that the row is read
+// once, in pieces of VPL consecutive scores.  The k best are taken one after the other: the largest key of the team, then the
+// lowest expert that has it (ties go to the lowest index), then that one is struck out.
+//
+// Keys: the scores themselves where nothing is added to them -- softmax and sigmoid keep their order, and no rounding can tie what
+// differs.  With a bias (or group scores that add two probabilities) the keys are probabilities in 64 bits: scores next to each other
+// differ by less than the rounding of 32 bits often enough to matter (a few rows in ten thousand).
+template <typename T, int VPL> __device__ __forceinline__ void load_scores(const T* p, int base, int E, typename Num<T>::acc (&x)[VPL]) {
+    using acc = typename Num<T>::acc;
+    typedef T block __attribute__((ext_vector_type(VPL)));
+    typedef block block_at __attribute__((aligned(sizeof(T))));
+    if (base + VPL <= E) {
+        const block b = *reinterpret_cast<const block_at*>(p + base);
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) x[s] = (acc)b[s];
+    } else {
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) x[s] = base + s < E ? (acc)p[base + s] : (acc)0;
+    }
+}
+
+struct RouteDev {
+    int64_t n, ld, ld_mask, ld_out;
+    int E, k, groups, top_groups, group_size;
+    int sigmoid, top2, renorm, bias_f64;
+    double scale;
+    const void* scores; const void* bias; const unsigned char* mask;
+    int* experts; void* weights;
+    const void* dweights; void* dscores;
+};
+
+// log of the sigmoid, finite for every finite x
+__device__ __forceinline__ double log_sigmoid(double x) { return (x < 0.0 ? x : 0.0) - log1p(exp(-fabs(x))); }
+
+// Bits of the team's scores that are open (in range, not masked, not -inf); *bad: an open one is NaN or +inf
+template <int L, int VPL, typename A>
+__device__ __forceinline__ unsigned open_scores(const RouteDev& a, bool live, int64_t row, int base, const A (&x)[VPL], bool* bad) {
+    unsigned open = 0, wrong = 0;
+    if (live) {
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) {
+            bool o = base + s < a.E;
+            if (o && a.mask != nullptr) o = a.mask[row * a.ld_mask + base + s] != 0;
+            o = o && !(x[s] == -INFINITY);
+            open |= o ? 1u << s : 0u;
+            wrong |= o && !(x[s] < INFINITY) ? 1u : 0u;
+        }
+    }
+    *bad = lanes_reduce<L>((int)wrong, OpMax()) != 0;
+    return open;
+}
+
+template <typename T, int L, int VPL, typename KEY>
+__global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
+    using acc = typename Num<T>::acc;
+    constexpr int TEAMS = 64 / L;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, team = lane / L, l = lane & (L - 1);
+    const int64_t row = ((int64_t)blockIdx.x * 4 + wave) * TEAMS + team;
+    const bool live = row < a.n;
+    const int base = l * VPL;
+    const size_t sel_bytes = (size_t)4 * TEAMS * a.k * sizeof(int);
+    int* sel = reinterpret_cast<int*>(lds) + (wave * TEAMS + team) * a.k;
+    const T* xrow = static_cast<const T*>(a.scores) + (live ? row : 0) * a.ld;
+
+    acc x[VPL];
+    if (live) load_scores<T, VPL>(xrow, base, a.E, x);
+    else {
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) x[s] = 0;
+    }
+    bool bad;
+    const unsigned open = open_scores<L, VPL>(a, live, row, base, x, &bad);
+
+    // softmax over the open scores
+    acc xmax = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < VPL; ++s) xmax = open >> s & 1 ? (x[s] > xmax ? x[s] : xmax) : xmax;
+    xmax = lanes_reduce<L>(xmax, OpMax());
+
+    // float keys are made for plain ones only (route_launch)
+    const bool plain_keys = sizeof(KEY) == 4 || (a.bias == nullptr && !(a.groups > 1 && a.top2));
+    KEY v[VPL];
+    if (plain_keys) {
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) v[s] = open >> s & 1 ? (KEY)x[s] : (KEY)-INFINITY;
+    } else {
+        double p[VPL], inv = 1.0;
+        if (a.sigmoid) {
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) p[s] = 1.0 / (1.0 + exp(-(double)x[s]));
+        } else {
+            double z = 0.0;
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) { p[s] = open >> s & 1 ? exp((double)x[s] - (double)xmax) : 0.0; z += p[s]; }
+            z = lanes_reduce<L>(z, OpSum());
+            inv = z;
+        }
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) {
+            double key = p[s] / inv;
+            if (a.bias != nullptr && base + s < a.E)
+                key += a.bias_f64 ? static_cast<const double*>(a.bias)[base + s] : (double)static_cast<const float*>(a.bias)[base + s];
+            v[s] = open >> s & 1 ? (KEY)key : (KEY)-INFINITY;
+        }
+    }
+
+    if (a.groups > 1) {
+        // the team's keys through LDS: lane l scores the groups l, l + L, ...
+        KEY* keys = reinterpret_cast<KEY*>(lds + ((sel_bytes + 15) & ~(size_t)15)) + (size_t)(wave * TEAMS + team) * (a.E + a.groups);
+        KEY* gs = keys + a.E;
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) if (base + s < a.E) keys[base + s] = v[s];
+        wave_sync();
+        for (int g = l; g < a.groups; g += L) {
+            KEY m1 = -INFINITY, m2 = -INFINITY;
+            for (int i = 0; i < a.group_size; ++i) {
+                const KEY t = keys[g * a.group_size + i];
+                if (t > m1) { m2 = m1; m1 = t; } else if (t > m2) m2 = t;
+            }
+            gs[g] = a.top2 && m2 > -INFINITY ? m1 + m2 : m1;
+        }
+        wave_sync();
+        unsigned long long kept = 0;
+        for (int g = l; g < a.groups; g += L) {
+            const KEY mine = gs[g];
+            int ahead = 0;
+            for (int h = 0; h < a.groups; ++h) { const KEY o = gs[h]; ahead += o > mine || (o == mine && h < g) ? 1 : 0; }
+            if (ahead < a.top_groups) kept |= 1ull << g;
+        }
+#pragma unroll
+        for (int m = 1; m < L; m <<= 1) kept |= __shfl_xor(kept, m, 64);
+        int g = base / a.group_size, r = base - g * a.group_size;
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) {
+            if (g < a.groups && !(kept >> g & 1)) v[s] = -INFINITY;
+            if (++r == a.group_size) { r = 0; ++g; }
+        }
+    }
+
+    for (int j = 0; j < a.k; ++j) {
+        KEY m = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) m = v[s] > m ? v[s] : m;
+        m = lanes_reduce<L>(m, OpMax());
+        int at = a.E;
+#pragma unroll
+        for (int s = VPL - 1; s >= 0; --s) at = v[s] == m ? base + s : at;
+        at = lanes_reduce<L>(at, OpMin());
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) v[s] = base + s == at ? (KEY)-INFINITY : v[s];
+        if (l == 0) sel[j] = m > -INFINITY && !bad ? at : -1;
+    }
+    wave_sync();
+
+    // weights of the chosen, in acc (the sums of a sigmoid's renormalisation in 64 bits: all of them may be far below 1)
+    acc z = 0;
+    if (!a.sigmoid && !a.renorm) {
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) z += open >> s & 1 ? exp(x[s] - xmax) : (acc)0;
+        z = lanes_reduce<L>(z, OpSum());
+    }
+    double top = -INFINITY, sum = 0.0;
+    if (a.renorm) {
+        for (int j = l; j < a.k; j += L) if (sel[j] >= 0) {
+            const double xe = (double)(acc)xrow[sel[j]], t = a.sigmoid ? log_sigmoid(xe) : xe;
+            top = t > top ? t : top;
+        }
+        top = lanes_reduce<L>(top, OpMax());
+        for (int j = l; j < a.k; j += L) if (sel[j] >= 0) {
+            const double xe = (double)(acc)xrow[sel[j]], t = a.sigmoid ? log_sigmoid(xe) : xe;
+            sum += exp(t - top);
+        }
+        sum = lanes_reduce<L>(sum, OpSum());
+    }
+    if (!live) return;
+    for (int j = l; j < a.k; j += L) {
+        const int e = sel[j];
+        a.experts[row * a.k + j] = e;
+        acc w = 0;
+        if (bad) w = NAN;
+        else if (e >= 0) {
+            const acc xe = (acc)xrow[e];
+            if (a.renorm) w = (acc)(a.scale * (exp((a.sigmoid ? log_sigmoid((double)xe) : (double)xe) - top) / sum));
+            else if (a.sigmoid) w = (acc)(a.scale / (1.0 + exp(-(double)xe)));
+            else w = (acc)a.scale * (exp(xe - xmax) / z);
+        }
+        static_cast<acc*>(a.weights)[row * a.k + j] = w;
+    }
+}
+
+// d(scores).  With p = softmax or sigmoid, g_j = scale dw_j of the chosen and r their renormalised weights (without the scale):
+//   softmax, plain   p_i (g_i [chosen] - sum_j p_j g_j)          sigmoid, plain   p_i (1 - p_i) g_i
+//   softmax, renorm  r_i (g_i - sum_j r_j g_j)                    sigmoid, renorm  r_i (g_i - sum_j r_j g_j)(1 - p_i)
+// Only the first is dense; the chosen ones' terms go through an LDS row so that every row leaves in one coalesced piece.
+// A row without experts has gradient zero.
+template <typename T, int L, int VPL>
+__global__ void __launch_bounds__(256) route_grad_kernel(RouteDev a) {
+    using acc = typename Num<T>::acc;
+    constexpr int TEAMS = 64 / L;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, team = lane / L, l = lane & (L - 1);
+    const int64_t row = ((int64_t)blockIdx.x * 4 + wave) * TEAMS + team;
+    const bool live = row < a.n;
+    const int base = l * VPL;
+    acc* buf = reinterpret_cast<acc*>(lds) + (size_t)(wave * TEAMS + team) * a.E;
+    const T* xrow = static_cast<const T*>(a.scores) + (live ? row : 0) * a.ld;
+    const int* sel = a.experts + (live ? row : 0) * a.k;
+    const acc* dw = static_cast<const acc*>(a.dweights) + (live ? row : 0) * a.k;
+    const bool dense = !a.sigmoid && !a.renorm;
+
+    acc x[VPL], xmax = -INFINITY, z = 0;
+    unsigned open = 0;
+    if (dense) {
+        if (live) load_scores<T, VPL>(xrow, base, a.E, x);
+        else {
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) x[s] = 0;
+        }
+        bool bad;
+        open = open_scores<L, VPL>(a, live, row, base, x, &bad);
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) xmax = open >> s & 1 ? (x[s] > xmax ? x[s] : xmax) : xmax;
+        xmax = lanes_reduce<L>(xmax, OpMax());
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) { x[s] = open >> s & 1 ? exp(x[s] - xmax) : (acc)0; z += x[s]; }
+        z = lanes_reduce<L>(z, OpSum());
+    }
+#pragma unroll
+    for (int s = 0; s < VPL; ++s) if (base + s < a.E) buf[base + s] = 0;
+    wave_sync();
+
+    double top = -INFINITY, sum = 0.0, dot = 0.0;
+    int some = 0;
+    if (live) {
+        for (int j = l; j < a.k; j += L) {
+            const int e = sel[j];
+            if (e < 0 || e >= a.E) continue;
+            some = 1;
+            const double xe = (double)(acc)xrow[e], t = a.sigmoid ? log_sigmoid(xe) : xe;
+            top = t > top ? t : top;
+        }
+    }
+    top = lanes_reduce<L>(top, OpMax());
+    some = lanes_reduce<L>(some, OpMax());
+    if (live && (a.renorm || dense)) {
+        for (int j = l; j < a.k; j += L) {
+            const int e = sel[j];
+            if (e < 0 || e >= a.E) continue;
+            const double xe = (double)(acc)xrow[e], g = a.scale * (double)dw[j];
+            const double r = dense ? exp(xe - (double)xmax) / (double)z : exp((a.sigmoid ? log_sigmoid(xe) : xe) - top);
+            sum += r; dot += r * g;
+        }
+    }
+    sum = lanes_reduce<L>(sum, OpSum());
+    dot = lanes_reduce<L>(dot, OpSum());
+    if (live) {
+        for (int j = l; j < a.k; j += L) {
+            const int e = sel[j];
+            if (e < 0 || e >= a.E) continue;
+            const double xe = (double)(acc)xrow[e], g = a.scale * (double)dw[j];
+            double d;
+            if (dense) d = g;
+            else if (a.renorm) {
+                d = exp((a.sigmoid ? log_sigmoid(xe) : xe) - top) / sum * (g - dot / sum);
+                if (a.sigmoid) d *= 1.0 / (1.0 + exp(xe));
+            } else d = g / (1.0 + exp(-xe)) / (1.0 + exp(xe));
+            atomicAdd(&buf[e], (acc)d);
+        }
+    }
+    wave_sync();
+    if (!live) return;
+    T* out = static_cast<T*>(a.dscores) + row * a.ld_out;
+#pragma unroll
+    for (int s = 0; s < VPL; ++s) {
+        if (base + s >= a.E) break;
+        acc d = buf[base + s];
+        if (dense) d = some ? x[s] / z * (d - (acc)dot) : (acc)0;
+        out[base + s] = (T)d;
+    }
+}
+
+// lanes per row and scores per lane: the fewest lanes that hold a row with at most 16 scores each, so that the steps across lanes,
+// which a row of a team pays k times, are few
+template <typename F> static int with_team(int E, F&& fn) {
+    if (E <= 16) return fn(std::integral_constant<int, 4>(), std::integral_constant<int, 4>());
+    if (E <= 32) return fn(std::integral_constant<int, 4>(), std::integral_constant<int, 8>());
+    if (E <= 64) return fn(std::integral_constant<int, 4>(), std::integral_constant<int, 16>());
+    if (E <= 128) return fn(std::integral_constant<int, 8>(), std::integral_constant<int, 16>());
+    if (E <= 256) return fn(std::integral_constant<int, 16>(), std::integral_constant<int, 16>());
+    if (E <= 512) return fn(std::integral_constant<int, 32>(), std::integral_constant<int, 16>());
+    return fn(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
+}
+
+static int route_check(const oak_route_args* a) {
+    OAK_REQUIRE(a != nullptr, "route: arguments are NULL");
+    OAK_REQUIRE(a->n_rows >= 0, "route: n_rows = %lld", (long long)a->n_rows);
+    OAK_REQUIRE(a->n_experts >= 1 && a->n_experts <= OAK_MAX_EXPERTS, "route: n_experts = %d is not in 1 .. %d", a->n_experts, OAK_MAX_EXPERTS);
+    OAK_REQUIRE(a->n_groups >= 1 && a->n_groups <= 64 && a->n_experts % a->n_groups == 0,
+                "route: n_groups = %d must divide the %d experts and be at most 64", a->n_groups, a->n_experts);
+    OAK_REQUIRE(a->top_groups >= 1 && a->top_groups <= a->n_groups, "route: top_groups = %d of %d groups", a->top_groups, a->n_groups);
+    OAK_REQUIRE(a->top_k >= 1 && a->top_k <= OAK_MAX_TOP_K && a->top_k <= a->top_groups * (a->n_experts / a->n_groups),
+                "route: top_k = %d, at most %d and at most the experts of the groups kept (%d)", a->top_k, OAK_MAX_TOP_K,
+                a->top_groups * (a->n_experts / a->n_groups));
+    OAK_REQUIRE(a->dtype >= OAK_F64 && a->dtype <= OAK_F16, "route: unknown element type %d", a->dtype);
+    OAK_REQUIRE(a->score == OAK_SCORE_SOFTMAX || a->score == OAK_SCORE_SIGMOID, "route: unknown score %d", a->score);
+    OAK_REQUIRE(a->group_score == OAK_GROUP_MAX || a->group_score == OAK_GROUP_TOP2, "route: unknown group score %d", a->group_score);
+    OAK_REQUIRE(a->scale - a->scale == 0.0, "route: scale is not finite");
+    OAK_REQUIRE(a->n_rows <= 1 || a->ld_scores >= 0, "route: negative row stride");
+    OAK_REQUIRE(a->n_rows == 0 || (a->scores && a->experts), "route: scores or experts are NULL");
+    OAK_REQUIRE(a->n_rows * (int64_t)a->top_k < ((int64_t)1 << 31), "route: %lld rows x %d experts pass 2^31 slots", (long long)a->n_rows, a->top_k);
+    return OAK_OK;
+}
+
+static RouteDev route_dev(const oak_route_args* a) {
+    RouteDev d{};
+    d.n = a->n_rows; d.ld = a->ld_scores; d.ld_mask = a->ld_mask; d.ld_out = a->ld_dscores;
+    d.E = a->n_experts; d.k = a->top_k; d.groups = a->n_groups; d.top_groups = a->top_groups; d.group_size = a->n_experts / a->n_groups;
+    d.sigmoid = a->score == OAK_SCORE_SIGMOID; d.top2 = a->group_score == OAK_GROUP_TOP2; d.renorm = a->renormalise != 0; d.bias_f64 = a->bias_f64;
+    d.scale = a->scale; d.scores = a->scores; d.bias = a->bias; d.mask = a->mask; d.experts = a->experts; d.weights = a->weights;
+    d.dweights = a->dweights; d.dscores = a->dscores;
+    return d;
+}
+
+static int route_launch(hipStream_t stream, const oak_route_args* a) {
+    if (a->n_rows == 0) return OAK_OK;
+    const RouteDev d = route_dev(a);
+    const bool plain_keys = d.bias == nullptr && !(d.groups > 1 && d.top2);
+    return with_dtype(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        return with_team(d.E, [&](auto lc, auto vc) {
+            constexpr int L = decltype(lc)::value, VPL = decltype(vc)::value, TEAMS = 64 / L;
+            const dim3 grid((unsigned)((d.n + 4 * TEAMS - 1) / (4 * TEAMS)));
+            const size_t sel = ((size_t)4 * TEAMS * d.k * sizeof(int) + 15) & ~(size_t)15;
+            auto go = [&](auto key) {
+                using KEY = decltype(key);
+                const size_t lds = sel + (d.groups > 1 ? (size_t)4 * TEAMS * (d.E + d.groups) * sizeof(KEY) : 0);
+                auto kernel = route_kernel<T, L, VPL, KEY>;
+                if (lds > 64 * 1024) OAK_CHECK(ensure_dynamic_lds((const void*)kernel, 160 * 1024));
+                return launch(kernel, grid, dim3(256), lds, stream, d);
+            };
+            if constexpr (sizeof(T) < 8) { if (plain_keys) return go((float)0); }
+            return go((double)0);
+        });
+    });
+}
+
+static int route_grad_launch(hipStream_t stream, const oak_route_args* a) {
+    if (a->n_rows == 0) return OAK_OK;
+    const RouteDev d = route_dev(a);
+    return with_dtype(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        return with_team(d.E, [&](auto lc, auto vc) {
+            constexpr int L = decltype(lc)::value, VPL = decltype(vc)::value, TEAMS = 64 / L;
+            const dim3 grid((unsigned)((d.n + 4 * TEAMS - 1) / (4 * TEAMS)));
+            const size_t lds = (size_t)4 * TEAMS * d.E * sizeof(typename Num<T>::acc);
+            return launch(route_grad_kernel<T, L, VPL>, grid, dim3(256), lds, stream, d);
+        });
+    });
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// plan: stable counting sort of the n k slots by expert
+// ---------------------------------------------------------------------------------------------------------------------
+// Every wave owns one consecutive piece of the slots, so that the order inside an expert is the slots' own without any atomic
+// whose order could show: pieces are counted, the counts are summed in piece order, and each wave then places its slots 64 at a
+// time -- a slot's rank among the 64 is the number of lower lanes with the same expert (one ballot per bit of the expert's number).
+struct PlanDev {
+    int64_t slots, piece;
+    int k, E, npieces, bits;
+    const int* experts; int* rows; int* positions; int* counts; int* offsets;
+    int* ws;                    // [E][npieces]
+};
+
+__device__ __forceinline__ int slot_expert(const PlanDev& a, int64_t s, int64_t end) {
+    const int e = s < end ? a.experts[s] : -1;
+    return (unsigned)e < (unsigned)a.E ? e : -1;      // whatever is not an expert's number belongs to no expert
+}
+
+// places the slots [s0, s1) of one wave; next[e] (LDS, this wave's own): where the expert's next slot goes
+__device__ __forceinline__ void plan_place_piece(const PlanDev& a, int* next, int64_t s0, int64_t s1) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t t = s0; t < s1; t += 64) {
+        const int64_t s = t + lane;
+        const int e = slot_expert(a, s, s1);
+        unsigned long long same = __ballot(e >= 0);
+        for (int b = 0; b < a.bits; ++b) {
+            const unsigned long long ones = __ballot(e >> b & 1);
+            same &= (e >> b & 1) ? ones : ~ones;
+        }
+        int pos = -1;
+        if (e >= 0) {
+            const int rank = __popcll(same & (((unsigned long long)1 << lane) - 1));
+            pos = next[e] + rank;
+        }
+        wave_sync();
+        if (e >= 0 && (same >> lane) == 1ull) next[e] = pos + 1;      // the last of them
+        wave_sync();
+        if (s < s1) a.positions[s] = pos;
+        if (pos >= 0) a.rows[pos] = (int)(s / a.k);
+    }
+}
+
+// few slots: one workgroup of 16 waves does it all (one launch instead of three)
+__global__ void __launch_bounds__(1024) plan_small_kernel(PlanDev a) {
+    extern __shared__ int plan_lds[];                 // [16][E]
+    int* cnt = plan_lds;
+    __shared__ int wsum[17];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    for (int i = tid; i < 16 * a.E; i += 1024) cnt[i] = 0;
+    __syncthreads();
+    const int64_t s0 = wave * a.piece < a.slots ? wave * a.piece : a.slots, s1 = s0 + a.piece < a.slots ? s0 + a.piece : a.slots;
+    for (int64_t s = s0 + lane; s < s1; s += 64) {
+        const int e = slot_expert(a, s, s1);
+        if (e >= 0) atomicAdd(&cnt[wave * a.E + e], 1);
+    }
+    __syncthreads();
+    int total = 0;                                    // E <= 1024: one expert per thread
+    if (tid < a.E) for (int w = 0; w < 16; ++w) total += cnt[w * a.E + tid];
+    int incl = total;
+    for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
+    if (lane == 63) wsum[wave] = incl;
+    __syncthreads();
+    int off = incl - total, all = 0;
+    for (int w = 0; w < 16; ++w) { if (w < wave) off += wsum[w]; all += wsum[w]; }
+    if (tid < a.E) {
+        a.counts[tid] = total; a.offsets[tid] = off;
+        for (int w = 0; w < 16; ++w) { const int c = cnt[w * a.E + tid]; cnt[w * a.E + tid] = off; off += c; }
+    }
+    if (tid == 0) a.offsets[a.E] = all;
+    __syncthreads();
+    plan_place_piece(a, cnt + wave * a.E, s0, s1);
+    for (int64_t s = all + tid; s < a.slots; s += 1024) a.rows[s] = -1;
+}
+
+__global__ void __launch_bounds__(256) plan_count_kernel(PlanDev a) {
+    extern __shared__ int plan_lds[];                 // [4][E]
+    int* cnt = plan_lds;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t piece = (int64_t)blockIdx.x * 4 + wave;
+    int* mine = cnt + wave * a.E;
+    for (int e = lane; e < a.E; e += 64) mine[e] = 0;
+    wave_sync();
+    const int64_t s0 = piece * a.piece, s1 = s0 + a.piece < a.slots ? s0 + a.piece : a.slots;
+    for (int64_t s = s0 + lane; s < s1; s += 64) {
+        const int e = slot_expert(a, s, s1);
+        if (e >= 0) atomicAdd(&mine[e], 1);
+    }
+    wave_sync();
+    if (piece < a.npieces) for (int e = lane; e < a.E; e += 64) a.ws[(int64_t)e * a.npieces + piece] = mine[e];
+}
+
+// one wave per expert: counts of its pieces -> what lies before each piece
+__global__ void __launch_bounds__(256) plan_scan_kernel(PlanDev a) {
+    const int e = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (e >= a.E) return;
+    int* col = a.ws + (int64_t)e * a.npieces;
+    int before = 0;
+    for (int p0 = 0; p0 < a.npieces; p0 += 64) {
+        const int p = p0 + lane;
+        const int c = p < a.npieces ? col[p] : 0;
+        int incl = c;
+        for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
+        if (p < a.npieces) col[p] = before + incl - c;
+        before += __shfl(incl, 63, 64);
+    }
+    if (lane == 0) a.counts[e] = before;
+}
+
+__global__ void __launch_bounds__(256) plan_place_kernel(PlanDev a) {
+    extern __shared__ int plan_lds[];                 // [4][E] next places, [E + 1] offsets
+    int* lds = plan_lds;
+    __shared__ int wsum[4];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    int* off = lds + 4 * a.E;
+    // offsets of the experts from their counts: every workgroup sums them itself
+    const int per = (a.E + 255) / 256, e0 = tid * per, e1 = e0 + per < a.E ? e0 + per : a.E;
+    int mine = 0;
+    for (int e = e0; e < e1; ++e) mine += a.counts[e];
+    int incl = mine;
+    for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
+    if (lane == 63) wsum[wave] = incl;
+    __syncthreads();
+    int at = incl - mine;
+    for (int w = 0; w < wave; ++w) at += wsum[w];
+    for (int e = e0; e < e1; ++e) { off[e] = at; at += a.counts[e]; }
+    if (tid == 0) off[a.E] = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+    __syncthreads();
+    if (blockIdx.x == 0) for (int e = tid; e <= a.E; e += 256) a.offsets[e] = off[e];
+    const int all = off[a.E];
+    const int64_t piece = (int64_t)blockIdx.x * 4 + wave;
+    if (piece < a.npieces) {
+        int* next = lds + wave * a.E;
+        for (int e = lane; e < a.E; e += 64) next[e] = off[e] + a.ws[(int64_t)e * a.npieces + piece];
+        wave_sync();
+        const int64_t s0 = piece * a.piece, s1 = s0 + a.piece < a.slots ? s0 + a.piece : a.slots;
+        plan_place_piece(a, next, s0, s1);
+        for (int64_t s = s0 + lane; s < s1; s += 64) if (s >= all) a.rows[s] = -1;
+    }
+}
+
+constexpr int64_t PLAN_SMALL_SLOTS = 16384;
+constexpr int PLAN_MAX_PIECES = 2048;
+
+static void plan_pieces(int64_t slots, int E, int64_t* piece, int* npieces, bool* small) {
+    *small = slots <= PLAN_SMALL_SLOTS && E <= 1024;
+    const int want = *small ? 16 : PLAN_MAX_PIECES;
+    int64_t p = (slots + want - 1) / want;
+    const int64_t least = *small ? 64 : 256;
+    p = p < least ? least : (p + 63) / 64 * 64;
+    *piece = p;
+    *npieces = (int)((slots + p - 1) / p);
+}
+
+static int plan_check(const oak_plan_args* a) {
+    OAK_REQUIRE(a != nullptr, "plan: arguments are NULL");
+    OAK_REQUIRE(a->n_rows >= 0 && a->top_k >= 1 && a->top_k <= OAK_MAX_TOP_K, "plan: %lld rows of %d experts", (long long)a->n_rows, a->top_k);
+    OAK_REQUIRE(a->n_experts >= 1 && a->n_experts <= OAK_MAX_PLAN_EXPERTS, "plan: n_experts = %d is not in 1 .. %d", a->n_experts, OAK_MAX_PLAN_EXPERTS);
+    OAK_REQUIRE(a->n_rows * (int64_t)a->top_k < ((int64_t)1 << 31), "plan: %lld rows x %d experts pass 2^31 slots", (long long)a->n_rows, a->top_k);
+    OAK_REQUIRE(a->counts && a->offsets && (a->n_rows == 0 || (a->experts && a->rows && a->positions)), "plan: an array is NULL");
+    return OAK_OK;
+}
+
+static int plan_launch(hipStream_t stream, const oak_plan_args* a) {
+    PlanDev d{};
+    bool small;
+    d.slots = a->n_rows * a->top_k; d.k = a->top_k; d.E = a->n_experts;
+    plan_pieces(d.slots, d.E, &d.piece, &d.npieces, &small);
+    d.experts = a->experts; d.rows = a->rows; d.positions = a->positions; d.counts = a->counts; d.offsets = a->offsets; d.ws = a->workspace;
+    while ((1 << d.bits) < d.E) ++d.bits;
+    if (small) {
+        const size_t lds = (size_t)16 * d.E * sizeof(int);
+        if (lds > 32 * 1024) OAK_CHECK(ensure_dynamic_lds((const void*)plan_small_kernel, 16 * 1024 * sizeof(int)));
+        return launch(plan_small_kernel, dim3(1), dim3(1024), lds, stream, d);
+    }
+    const unsigned wgs = (unsigned)((d.npieces + 3) / 4);
+    const size_t lds = (size_t)(5 * d.E + 1) * sizeof(int);
+    if (lds > 32 * 1024) {
+        OAK_CHECK(ensure_dynamic_lds((const void*)plan_count_kernel, 128 * 1024));
+        OAK_CHECK(ensure_dynamic_lds((const void*)plan_place_kernel, 128 * 1024));
+    }
+    OAK_CHECK(launch(plan_count_kernel, dim3(wgs), dim3(256), (size_t)4 * d.E * sizeof(int), stream, d));
+    OAK_CHECK(launch(plan_scan_kernel, dim3((unsigned)((d.E + 3) / 4)), dim3(256), 0, stream, d));
+    return launch(plan_place_kernel, dim3(wgs), dim3(256), lds, stream, d);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// dispatch, combine and their gradients
+// ---------------------------------------------------------------------------------------------------------------------
+// All of them walk rows: a row is read or written once where the slots' order would touch it k times.  TPR threads share a row; a
+// unit is 16 bytes, the row's last elements that do not fill one are units of their own.
+struct MixDev {
+    int64_t n, slots, ld_rows, ld_slots, ld_grad;
+    int64_t units;              // 16-byte units of a row, then its last elements
+    int C, k, nvec, E, tpr_log2;
+    const int* positions; const int* offsets; const void* weights;
+    const void* src; void* dst; const void* dout; void* dslots; void* dweights;
+};
+
+template <typename T> __device__ __forceinline__ void zero_unit(const MixDev& a, T* row, int64_t u) {
+    if (u < a.nvec) { typename Vec<T>::raw z = {}; Vec<T>::store(row + u * Vec<T>::N, z); }
+    else row[a.nvec * (int64_t)Vec<T>::N + (u - a.nvec)] = (T)0;
+}
+
+// a place outside [0, slots) is no place
+__device__ __forceinline__ int64_t place_of(const MixDev& a, int64_t n, int j) {
+    const int p = a.positions[n * a.k + j];
+    return p >= 0 && p < a.slots ? p : -1;
+}
+
+template <typename T> __global__ void __launch_bounds__(256) dispatch_kernel(MixDev a) {
+    const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x, n = g >> a.tpr_log2;
+    const int tpr = 1 << a.tpr_log2, t = (int)(g & (tpr - 1));
+    if (n >= a.n) return;
+    const T* src = static_cast<const T*>(a.src) + n * a.ld_rows;
+    T* dst = static_cast<T*>(a.dst);
+    const int used = a.offsets[a.E];
+    for (int64_t u = t; u < a.units; u += tpr) {
+        if (u < a.nvec) {
+            const auto v = Vec<T>::load(src + u * Vec<T>::N);
+            for (int j = 0; j < a.k; ++j) { const int64_t p = place_of(a, n, j); if (p >= 0) Vec<T>::store(dst + p * a.ld_slots + u * Vec<T>::N, v); }
+        } else {
+            const int64_t c = a.nvec * (int64_t)Vec<T>::N + (u - a.nvec);
+            const T v = src[c];
+            for (int j = 0; j < a.k; ++j) { const int64_t p = place_of(a, n, j); if (p >= 0) dst[p * a.ld_slots + c] = v; }
+        }
+        for (int j = 0; j < a.k; ++j) if (n * a.k + j >= used) zero_unit<T>(a, dst + (n * a.k + j) * a.ld_slots, u);
+    }
+}
+
+template <typename T> __global__ void __launch_bounds__(256) combine_kernel(MixDev a) {
+    using acc = typename Num<T>::acc;
+    const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x, n = g >> a.tpr_log2;
+    const int tpr = 1 << a.tpr_log2, t = (int)(g & (tpr - 1));
+    if (n >= a.n) return;
+    const T* src = static_cast<const T*>(a.src);
+    T* dst = static_cast<T*>(a.dst) + n * a.ld_rows;
+    const acc* w = static_cast<const acc*>(a.weights);
+    for (int64_t u = t; u < a.units; u += tpr) {
+        if (u < a.nvec) {
+            acc y[Vec<T>::N] = {};
+            for (int j = 0; j < a.k; ++j) {
+                const int64_t p = place_of(a, n, j);
+                const acc wj = w ? w[n * a.k + j] : (acc)1;
+                if (p < 0) {                           // no expert: weight times nothing (a NaN weight still shows)
+                    if (w) for (int i = 0; i < Vec<T>::N; ++i) y[i] += wj * (acc)0;
+                    continue;
+                }
+                const auto f = Vec<T>::load(src + p * a.ld_slots + u * Vec<T>::N);
+#pragma unroll
+                for (int i = 0; i < Vec<T>::N; ++i) y[i] += wj * (acc)f[i];
+            }
+            typename Vec<T>::raw o;
+#pragma unroll
+            for (int i = 0; i < Vec<T>::N; ++i) o[i] = (T)y[i];
+            Vec<T>::store(dst + u * Vec<T>::N, o);
+        } else {
+            const int64_t c = a.nvec * (int64_t)Vec<T>::N + (u - a.nvec);
+            acc y = 0;
+            for (int j = 0; j < a.k; ++j) {
+                const int64_t p = place_of(a, n, j);
+                const acc wj = w ? w[n * a.k + j] : (acc)1;
+                if (p >= 0) y += wj * (acc)src[p * a.ld_slots + c];
+                else if (w) y += wj * (acc)0;
+            }
+            dst[c] = (T)y;
+        }
+    }
+}
+
+// dF[place] = w dy, dw = <dy, F[place]>: slot by slot, the row of dy stays in the nearest cache.  TPR <= 64: the dot product is
+// finished inside a wave.
+template <typename T> __global__ void __launch_bounds__(256) combine_grad_kernel(MixDev a) {
+    using acc = typename Num<T>::acc;
+    const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x, n = g >> a.tpr_log2;
+    const int tpr = 1 << a.tpr_log2, t = (int)(g & (tpr - 1));
+    const bool live = n < a.n;                         // whole waves stay for the shuffles
+    const T* F = static_cast<const T*>(a.src);
+    const T* dy = static_cast<const T*>(a.dout) + (live ? n : 0) * a.ld_grad;
+    T* dF = static_cast<T*>(a.dslots);
+    const acc* w = static_cast<const acc*>(a.weights);
+    const int used = a.offsets[a.E];
+    for (int j = 0; j < a.k; ++j) {
+        const int64_t p = live ? place_of(a, n, j) : -1;
+        acc d = 0;
+        if (p >= 0) {
+            const acc wj = w[n * a.k + j];
+            for (int64_t u = t; u < a.units; u += tpr) {
+                if (u < a.nvec) {
+                    const auto f = Vec<T>::load(F + p * a.ld_slots + u * Vec<T>::N), v = Vec<T>::load(dy + u * Vec<T>::N);
+                    typename Vec<T>::raw o;
+#pragma unroll
+                    for (int i = 0; i < Vec<T>::N; ++i) { d += (acc)f[i] * (acc)v[i]; o[i] = (T)(wj * (acc)v[i]); }
+                    Vec<T>::store(dF + p * (int64_t)a.C + u * Vec<T>::N, o);
+                } else {
+                    const int64_t c = a.nvec * (int64_t)Vec<T>::N + (u - a.nvec);
+                    const acc v = (acc)dy[c];
+                    d += (acc)F[p * a.ld_slots + c] * v;
+                    dF[p * (int64_t)a.C + c] = (T)(wj * v);
+                }
+            }
+        }
+        for (int m = 1; m < tpr; m <<= 1) d += __shfl_xor(d, m, 64);
+        if (live && t == 0) static_cast<acc*>(a.dweights)[n * a.k + j] = d;
+        if (live && n * a.k + j >= used) for (int64_t u = t; u < a.units; u += tpr) zero_unit<T>(a, dF + (n * a.k + j) * (int64_t)a.C, u);
+    }
+}
+
+static int mix_check(const char* what, const oak_mix_args* a) {
+    OAK_REQUIRE(a != nullptr, "%s: arguments are NULL", what);
+    OAK_REQUIRE(a->n_rows >= 0 && a->top_k >= 1 && a->top_k <= OAK_MAX_TOP_K, "%s: %lld rows of %d experts", what, (long long)a->n_rows, a->top_k);
+    OAK_REQUIRE(a->n_experts >= 1 && a->n_experts <= OAK_MAX_PLAN_EXPERTS, "%s: n_experts = %d", what, a->n_experts);
+    OAK_REQUIRE(a->n_cols >= 1 && a->n_cols <= (1 << 30), "%s: n_cols = %d", what, a->n_cols);
+    OAK_REQUIRE(a->dtype >= OAK_F64 && a->dtype <= OAK_F16, "%s: unknown element type %d", what, a->dtype);
+    OAK_REQUIRE(a->n_rows * (int64_t)a->top_k < ((int64_t)1 << 31), "%s: %lld rows x %d experts pass 2^31 slots", what, (long long)a->n_rows, a->top_k);
+    OAK_REQUIRE(a->ld_rows >= 0 && a->ld_slots >= 0 && a->ld_grad >= 0, "%s: negative row stride", what);
+    OAK_REQUIRE(a->n_rows == 0 || (a->positions && a->offsets), "%s: positions or offsets are NULL", what);
+    return OAK_OK;
+}
+
+static int mix_launch(hipStream_t stream, const oak_mix_args* a, int what /* 0 dispatch, 1 combine, 2 combine_grad */) {
+    if (a->n_rows == 0) return OAK_OK;
+    MixDev d{};
+    const int vec = 16 / (int)dtype_size(a->dtype);
+    d.n = a->n_rows; d.k = a->top_k; d.slots = d.n * d.k; d.ld_rows = a->ld_rows; d.ld_slots = a->ld_slots; d.ld_grad = a->ld_grad; d.C = a->n_cols;
+    d.E = a->n_experts; d.nvec = d.C / vec; d.units = d.nvec + d.C % vec;
+    d.positions = a->positions; d.offsets = a->offsets; d.weights = a->weights; d.src = a->src; d.dst = a->dst; d.dout = a->dout;
+    d.dslots = a->dslots; d.dweights = a->dweights;
+    const int most = what == 2 ? 6 : 8;
+    while (d.tpr_log2 < most && ((int64_t)1 << d.tpr_log2) < d.units) ++d.tpr_log2;
+    const int64_t wgs = ((d.n << d.tpr_log2) + 255) / 256;
+    OAK_REQUIRE(wgs < ((int64_t)1 << 31), "mixture: %lld rows are too many for one launch", (long long)d.n);
+    return with_dtype(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        auto kernel = what == 0 ? dispatch_kernel<T> : what == 1 ? combine_kernel<T> : combine_grad_kernel<T>;
+        return launch(kernel, dim3((unsigned)wgs), dim3(256), 0, stream, d);
+    });
+}
+
+}  // namespace oak
+
+using namespace oak;
+
+extern "C" {
+
+int oak_route_device(int32_t device, void* stream, const oak_route_args* a) {
+    return c_entry([&] {
+        OAK_CHECK(route_check(a));
+        OAK_REQUIRE(a->n_rows == 0 || a->weights, "route: weights are NULL");
+        DeviceGuard g;
+        OAK_CHECK(g.enter(device));
+        return route_launch((hipStream_t)stream, a);
+    });
+}
+
+int oak_route_grad_device(int32_t device, void* stream, const oak_route_args* a) {
+    return c_entry([&] {
+        OAK_CHECK(route_check(a));
+        OAK_REQUIRE(a->n_rows == 0 || (a->dweights && a->dscores), "route_grad: dweights or dscores are NULL");
+        OAK_REQUIRE(a->n_rows <= 1 || a->ld_dscores >= a->n_experts, "route_grad: rows of dscores overlap");
+        DeviceGuard g;
+        OAK_CHECK(g.enter(device));
+        return route_grad_launch((hipStream_t)stream, a);
+    });
+}
+
+static int route_host(oak_ctx* ctx, const oak_route_args* args, bool grad) {
+    if (!ctx) { set_error("ctx is NULL"); return OAK_E_ARG; }
+    OAK_CHECK(route_check(args));
+    OAK_REQUIRE(args->dtype == OAK_F64 && (!args->bias || args->bias_f64), "route: host arrays are float64");
+    OAK_REQUIRE(args->ld_scores == args->n_experts && (!args->mask || args->ld_mask == args->n_experts || args->ld_mask == 0),
+                "route: host arrays are contiguous");
+    OAK_REQUIRE(args->n_rows == 0 || (grad ? args->dweights && args->dscores && args->ld_dscores == args->n_experts : args->weights != nullptr),
+                "route: an array is NULL");
+    OAK_HIP_CHECK(hipSetDevice(ctx->device));
+    if (args->n_rows == 0) return OAK_OK;
+    PhaseTimer t(ctx, grad ? "route_grad" : "route");
+    oak_route_args a = *args;
+    HostStage st(ctx);
+    const size_t cells = (size_t)a.n_rows * a.n_experts, slots = (size_t)a.n_rows * a.top_k;
+    OAK_CHECK(st.in("ex_scores", a.scores, cells * 8));
+    OAK_CHECK(st.in("ex_bias", a.bias, (size_t)a.n_experts * 8));
+    OAK_CHECK(st.in("ex_mask", a.mask, a.ld_mask ? cells : (size_t)a.n_experts));
+    if (grad) {
+        OAK_CHECK(st.in("ex_experts", a.experts, slots * 4));
+        OAK_CHECK(st.in("ex_dweights", a.dweights, slots * 8));
+        OAK_CHECK(st.out("ex_dscores", a.dscores, cells * 8));
+        OAK_CHECK(route_grad_launch(ctx->stream, &a));
+    } else {
+        OAK_CHECK(st.out("ex_experts", a.experts, slots * 4));
+        OAK_CHECK(st.out("ex_weights", a.weights, slots * 8));
+        OAK_CHECK(route_launch(ctx->stream, &a));
+    }
+    t.stop();
+    return st.finish();
+}
+
+int oak_route(oak_ctx* ctx, const oak_route_args* a) { return c_entry([&] { return route_host(ctx, a, false); }); }
+int oak_route_grad(oak_ctx* ctx, const oak_route_args* a) { return c_entry([&] { return route_host(ctx, a, true); }); }
+
+int64_t oak_plan_workspace(int64_t n_rows, int32_t top_k, int32_t n_experts) {
+    if (n_rows <= 0 || top_k <= 0 || n_experts <= 0) return 0;
+    int64_t piece; int np; bool small;
+    plan_pieces(n_rows * top_k, n_experts, &piece, &np, &small);
+    return small ? 0 : (int64_t)np * n_experts;
+}
+
+int oak_plan_device(int32_t device, void* stream, const oak_plan_args* a) {
+    return c_entry([&] {
+        OAK_CHECK(plan_check(a));
+        const int64_t ints = oak_plan_workspace(a->n_rows, a->top_k, a->n_experts);
+        OAK_REQUIRE(ints == 0 || (a->workspace && a->workspace_ints >= ints), "plan: the workspace holds %lld of the %lld integers asked for by oak_plan_workspace",
+                    (long long)a->workspace_ints, (long long)ints);
+        DeviceGuard g;
+        OAK_CHECK(g.enter(device));
+        return plan_launch((hipStream_t)stream, a);
+    });
+}
+
+int oak_plan(oak_ctx* ctx, const oak_plan_args* args) {
+    return c_entry([&] {
+        if (!ctx) { set_error("ctx is NULL"); return OAK_E_ARG; }
+        OAK_CHECK(plan_check(args));
+        OAK_HIP_CHECK(hipSetDevice(ctx->device));
+        PhaseTimer t(ctx, "plan");
+        oak_plan_args a = *args;
+        HostStage st(ctx);
+        const size_t slots = (size_t)a.n_rows * a.top_k;
+        OAK_CHECK(st.in("ex_experts", a.experts, slots * 4));
+        OAK_CHECK(st.out("ex_rows", a.rows, slots * 4));
+        OAK_CHECK(st.out("ex_positions", a.positions, slots * 4));
+        OAK_CHECK(st.out("ex_counts", a.counts, (size_t)a.n_experts * 4));
+        OAK_CHECK(st.out("ex_offsets", a.offsets, (size_t)(a.n_experts + 1) * 4));
+        a.workspace_ints = oak_plan_workspace(a.n_rows, a.top_k, a.n_experts);
+        void* ws = nullptr;
+        OAK_CHECK(get_buf(ctx, "ex_plan_ws", (size_t)a.workspace_ints * 4, &ws));
+        a.workspace = (int32_t*)ws;
+        OAK_CHECK(plan_launch(ctx->stream, &a));
+        t.stop();
+        return st.finish();
+    });
+}
+
+static int mix_arrays(const char* name, const oak_mix_args* a, int what) {
+    OAK_CHECK(mix_check(name, a));
+    if (a->n_rows == 0) return OAK_OK;
+    OAK_REQUIRE(a->src != nullptr, "%s: the input is NULL", name);
+    if (what == 2) {
+        OAK_REQUIRE(a->weights && a->dout && a->dslots && a->dweights, "%s: an array is NULL", name);
+    } else {
+        OAK_REQUIRE(a->dst != nullptr, "%s: the output is NULL", name);
+        const int64_t ld_out = what == 0 ? a->ld_slots : a->ld_rows;
+        OAK_REQUIRE(a->n_rows * (what == 0 ? a->top_k : 1) <= 1 || ld_out >= a->n_cols, "%s: rows of the output overlap", name);
+    }
+    return OAK_OK;
+}
+
+static int mix_device(const char* name, int32_t device, void* stream, const oak_mix_args* a, int what) {
+    return c_entry([&] {
+        OAK_CHECK(mix_arrays(name, a, what));
+        DeviceGuard g;
+        OAK_CHECK(g.enter(device));
+        return mix_launch((hipStream_t)stream, a, what);
+    });
+}
+
+static int mix_host(const char* name, oak_ctx* ctx, const oak_mix_args* args, int what) {
+    return c_entry([&] {
+        if (!ctx) { set_error("ctx is NULL"); return OAK_E_ARG; }
+        OAK_CHECK(mix_arrays(name, args, what));
+        OAK_REQUIRE(args->dtype == OAK_F64 && args->ld_rows == args->n_cols && args->ld_slots == args->n_cols && args->ld_grad == args->n_cols,
+                    "%s: host arrays are contiguous float64", name);
+        OAK_HIP_CHECK(hipSetDevice(ctx->device));
+        if (args->n_rows == 0) return (int)OAK_OK;
+        PhaseTimer t(ctx, name);
+        oak_mix_args a = *args;
+        HostStage st(ctx);
+        const size_t slots = (size_t)a.n_rows * a.top_k, rb = (size_t)a.n_rows * a.n_cols * 8, sb = slots * a.n_cols * 8;
+        OAK_CHECK(st.in("ex_positions", a.positions, slots * 4));
+        OAK_CHECK(st.in("ex_offsets", a.offsets, (size_t)(a.n_experts + 1) * 4));
+        OAK_CHECK(st.in("ex_weights", a.weights, slots * 8));
+        if (what == 0) {
+            OAK_CHECK(st.in("mix_rows", a.src, rb));
+            OAK_CHECK(st.out("mix_slots", a.dst, sb));
+        } else {
+            OAK_CHECK(st.in("mix_slots", a.src, sb));
+            if (what == 1) OAK_CHECK(st.out("mix_rows", a.dst, rb));
+            else {
+                OAK_CHECK(st.in("mix_rows", a.dout, rb));
+                OAK_CHECK(st.out("mix_dslots", a.dslots, sb));
+                OAK_CHECK(st.out("mix_dweights", a.dweights, slots * 8));
+            }
+        }
+        OAK_CHECK(mix_launch(ctx->stream, &a, what));
+        t.stop();
+        return st.finish();
+    });
+}
+
+int oak_dispatch(oak_ctx* ctx, const oak_mix_args* a) { return mix_host("dispatch", ctx, a, 0); }
+int oak_combine(oak_ctx* ctx, const oak_mix_args* a) { return mix_host("combine", ctx, a, 1); }
+int oak_combine_grad(oak_ctx* ctx, const oak_mix_args* a) { return mix_host("combine_grad", ctx, a, 2); }
+int oak_dispatch_device(int32_t device, void* stream, const oak_mix_args* a) { return mix_device("dispatch", device, stream, a, 0); }
+int oak_combine_device(int32_t device, void* stream, const oak_mix_args* a) { return mix_device("combine", device, stream, a, 1); }
+int oak_combine_grad_device(int32_t device, void* stream, const oak_mix_args* a) { return mix_device("combine_grad", device, stream, a, 2); }
+
+}  // extern "C"

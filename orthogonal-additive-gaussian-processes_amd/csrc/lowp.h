@@ -1,0 +1,127 @@
+// Element types, unaligned vector access and cross-lane reductions shared by the operators that take device arrays of several
+// types (experts.hip, distill.hip).
+#pragma once
+#include <exception>
+#include <tuple>
+#include "oak_internal.h"
+
+namespace oak {
+
+// Sums, softmax statistics and weights of T are held in Num<T>::acc: 32 bits for the 16- and 32-bit types, 64 for double.
+template <typename T> struct Num { using acc = float; };
+template <> struct Num<double> { using acc = double; };
+
+// 16 bytes of T.  The alignment is the element's: rows may start anywhere (odd leading dimensions, sliced arrays) and gfx950's global
+// loads and stores of 4 dwords need no more than that.
+template <typename T> struct Vec {
+    static constexpr int N = 16 / (int)sizeof(T);
+    typedef T raw __attribute__((ext_vector_type(16 / sizeof(T))));
+    typedef raw at __attribute__((aligned(sizeof(T))));
+    static __device__ __forceinline__ raw load(const T* p) { return *reinterpret_cast<const at*>(p); }
+    static __device__ __forceinline__ void store(T* p, raw v) { *reinterpret_cast<at*>(p) = v; }
+    // results that no later kernel of the call reads: kept out of the caches' way
+    static __device__ __forceinline__ void store_stream(T* p, raw v) { __builtin_nontemporal_store(v, reinterpret_cast<at*>(p)); }
+};
+
+inline size_t dtype_size(int dtype) { return dtype == OAK_F64 ? 8 : dtype == OAK_F32 ? 4 : 2; }
+inline size_t dtype_acc_size(int dtype) { return dtype == OAK_F64 ? 8 : 4; }
+
+// calls fn.template operator()<T>() for the element type of a run-time code
+template <typename F> inline int with_dtype(int dtype, F&& fn) {
+    switch (dtype) {
+        case OAK_F64: return fn((double)0);
+        case OAK_F32: return fn((float)0);
+        case OAK_BF16: return fn((__bf16)0.0f);
+        case OAK_F16: return fn((_Float16)0.0f);
+        default: set_error("unknown element type %d", dtype); return OAK_E_ARG;
+    }
+}
+
+// one value of an array whose type is only known at run time
+__device__ __forceinline__ double load_any(const void* p, int dtype, int64_t i) {
+    switch (dtype) {
+        case OAK_F64: return static_cast<const double*>(p)[i];
+        case OAK_F32: return (double)static_cast<const float*>(p)[i];
+        case OAK_BF16: return (double)(float)static_cast<const __bf16*>(p)[i];
+        default: return (double)(float)static_cast<const _Float16*>(p)[i];
+    }
+}
+
+// ---- reductions over L consecutive lanes (L a power of two up to 64); every lane gets the result --------------------------
+struct OpMax { template <typename A> __device__ __forceinline__ A operator()(A a, A b) const { return a > b ? a : b; } };
+struct OpMin { template <typename A> __device__ __forceinline__ A operator()(A a, A b) const { return a < b ? a : b; } };
+struct OpSum { template <typename A> __device__ __forceinline__ A operator()(A a, A b) const { return a + b; } };
+
+template <int L, typename Op, typename A> __device__ __forceinline__ A lanes_reduce(A v, Op op) {
+#pragma unroll
+    for (int m = 1; m < L; m <<= 1) v = op(v, __shfl_xor(v, m, 64));
+    return v;
+}
+
+// order of LDS accesses between the lanes of one wave (no other wave is waited for)
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The launch's own status: hipGetLastError() would also report an error some other library of the process left behind.
+template <typename... P, typename... A>
+inline int launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t stream, A&&... args) {
+    std::tuple<P...> held{static_cast<P>(args)...};
+    void* ptrs[sizeof...(P)];
+    int i = 0;
+    std::apply([&](auto&... a) { ((ptrs[i++] = (void*)&a), ...); }, held);
+    OAK_HIP_CHECK(hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, ptrs, lds, stream));
+    return OAK_OK;
+}
+
+// no C++ exception leaves a C entry point
+template <typename F> inline int c_entry(F&& fn) {
+    try { return fn(); }
+    catch (const std::exception& e) { set_error("%s", e.what()); return OAK_E_HIP; }
+    catch (...) { set_error("unknown C++ exception"); return OAK_E_HIP; }
+}
+
+// the device entry points run on whatever device and stream their caller names and leave the thread's current device as it was
+struct DeviceGuard {
+    int before = -1; bool switched = false;
+    int enter(int device) {
+        OAK_HIP_CHECK(hipGetDevice(&before));
+        if (before != device) { OAK_HIP_CHECK(hipSetDevice(device)); switched = true; }
+        return OAK_OK;
+    }
+    ~DeviceGuard() { if (switched) (void)hipSetDevice(before); }
+};
+
+// host arrays of a call -> named scratch of the context and back.  Inputs are copied on the context's stream before the kernels,
+// outputs behind them; finish() waits for that stream.
+struct HostStage {
+    oak_ctx* ctx;
+    struct Out { void* host; void* dev; size_t bytes; };
+    std::vector<Out> outs;
+    explicit HostStage(oak_ctx* c) : ctx(c) {}
+    template <typename P> int in(const char* name, P& p, size_t bytes) {
+        if (p == nullptr || bytes == 0) return OAK_OK;
+        void* d = nullptr;
+        OAK_CHECK(get_buf(ctx, name, bytes, &d));
+        OAK_HIP_CHECK(hipMemcpyAsync(d, p, bytes, hipMemcpyHostToDevice, ctx->stream));
+        p = static_cast<P>(d);
+        return OAK_OK;
+    }
+    template <typename P> int out(const char* name, P& p, size_t bytes) {
+        if (p == nullptr || bytes == 0) return OAK_OK;
+        void* d = nullptr;
+        OAK_CHECK(get_buf(ctx, name, bytes, &d));
+        outs.push_back({p, d, bytes});
+        p = static_cast<P>(d);
+        return OAK_OK;
+    }
+    int finish() {
+        for (const Out& o : outs) OAK_HIP_CHECK(hipMemcpyAsync(o.host, o.dev, o.bytes, hipMemcpyDeviceToHost, ctx->stream));
+        OAK_HIP_CHECK(hipStreamSynchronize(ctx->stream));
+        return OAK_OK;
+    }
+};
+
+}  // namespace oak

@@ -51,6 +51,32 @@ class KernelDescStruct(C.Structure):
     ]
 
 
+class RouteArgs(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("n_rows", "ld_scores", "ld_mask", "ld_dscores")]
+                + [(n, C.c_int32) for n in ("n_experts", "top_k", "n_groups", "top_groups", "dtype", "score", "group_score", "renormalise",
+                                            "bias_f64")]
+                + [("scale", C.c_double)]
+                + [(n, C.c_void_p) for n in ("scores", "bias", "mask", "experts", "weights", "dweights", "dscores")])
+
+
+class PlanArgs(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("n_rows", "workspace_ints")] + [(n, C.c_int32) for n in ("top_k", "n_experts")]
+                + [(n, C.c_void_p) for n in ("experts", "rows", "positions", "counts", "offsets", "workspace")])
+
+
+class MixArgs(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("n_rows", "ld_rows", "ld_slots", "ld_grad")]
+                + [(n, C.c_int32) for n in ("top_k", "n_experts", "n_cols", "dtype")]
+                + [(n, C.c_void_p) for n in ("positions", "offsets", "weights", "src", "dst", "dout", "dslots", "dweights")])
+
+
+class DistillArgs(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("n_rows", "ld_logits", "ld_top", "ld_index", "ld_dlogits")]
+                + [(n, C.c_int32) for n in ("n_classes", "top_k", "dtype", "top_dtype", "lse_dtype", "weight_dtype", "index_64", "direction")]
+                + [("temperature", C.c_double)]
+                + [(n, C.c_void_p) for n in ("logits", "top", "index", "top_lse", "row_weight", "loss", "dlogits")])
+
+
 _D = C.POINTER(C.c_double)
 _I = C.POINTER(C.c_int32)
 _CTX = C.c_void_p
@@ -139,6 +165,14 @@ SIGNATURES = {
     "oak_kmeans": (C.c_int, [_CTX, _D, C.c_int64, C.c_int32, C.c_int32, C.c_int32, _D, C.c_int32, C.c_double, _D, _I,
                              _D, _I]),
 }
+
+# oak_X(ctx, args) on host arrays, oak_X_device(device, stream, args) on device arrays
+for _name, _args in (("route", RouteArgs), ("route_grad", RouteArgs), ("plan", PlanArgs), ("dispatch", MixArgs), ("combine", MixArgs),
+                     ("combine_grad", MixArgs), ("distill", DistillArgs)):
+    SIGNATURES[f"oak_{_name}"] = (C.c_int, [_CTX, C.POINTER(_args)])
+    SIGNATURES[f"oak_{_name}_device"] = (C.c_int, [C.c_int32, C.c_void_p, C.POINTER(_args)])
+SIGNATURES["oak_plan_workspace"] = (C.c_int64, [C.c_int64, C.c_int32, C.c_int32])
+SIGNATURES["oak_device_pointer_check"] = (C.c_int, [C.c_int32, C.c_void_p])
 
 _lib = None
 
@@ -889,6 +923,11 @@ class HipContext:
                                              idx.ctypes.data_as(C.POINTER(C.c_int64))))
         return centres, idx
 
+    # -- operators on host or device arrays (oak.experts, oak.distillation) -----------------------
+    def call(self, name: str, args):
+        """One operator of the ``oak_X(ctx, args)`` form on contiguous float64 host arrays."""
+        _check(getattr(self._lib, f"oak_{name}")(self._h, C.byref(args)))
+
     # -- benchmarking -------------------------------------------------------------------------
     def bench_gram_resident(self, desc: KernelDesc) -> float:
         b = C.c_double()
@@ -934,6 +973,22 @@ def default_context() -> HipContext:
         dev = int(os.environ.get("OAK_HIP_DEVICE", os.environ.get("LOCAL_RANK", "0")))
         _default_ctx = HipContext(dev)
     return _default_ctx
+
+
+def call_device(name: str, device: int, stream: int, args):
+    """One operator of the ``oak_X_device(device, stream, args)`` form; enqueued, not waited for."""
+    status = getattr(_lib or load_library(), f"oak_{name}_device")(device, stream, C.byref(args))
+    if status != OAK_OK:
+        _check(status)
+
+
+def plan_workspace(n_rows: int, top_k: int, n_experts: int) -> int:
+    return load_library().oak_plan_workspace(n_rows, top_k, n_experts)
+
+
+def check_device_pointer(device: int, pointer: int):
+    """Raises unless ``pointer`` is memory of ``device`` known to the HIP runtime the library runs on."""
+    _check(load_library().oak_device_pointer_check(device, pointer))
 
 
 def debug_state() -> str:

@@ -1,0 +1,309 @@
+"""Mixtures of models: rows routed to experts, laid out by expert, and the experts' answers summed.
+
+An additive model that is too stiff for a whole data set is replaced by several, each fitted and asked on its own rows: a router
+gives every row a score for every expert (a gating model's outputs, distances to k-means centres, ...), :func:`route` picks each row's experts and
+their weights, :func:`plan` and :func:`dispatch` lay the rows out so that every expert finds its own in one block, and
+:func:`combine` sums the answers.  The ``*_grad`` functions are the closed-form adjoints, so that a router and its experts can be
+trained against any loss on the mixture's output (:mod:`oak.distillation` has one).
+
+All functions take NumPy arrays (float64, results are NumPy arrays) or torch tensors on a HIP device (float64, float32, bfloat16, float16;
+results are tensors on the same device, computed on its current stream without waiting for them).  Sums, weights and
+their gradients are float64 for float64 arrays and float32 otherwise.
+
+>>> experts, weights = route(scores, top_k=2)                 # [N, 2], [N, 2]
+>>> p = plan(experts, n_experts=scores.shape[1])
+>>> rows = dispatch(X, p)                                      # expert e's rows: rows[p.offsets[e]:p.offsets[e + 1]]
+>>> y = combine(answers, weights, p)                           # answers in the same layout
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import numpy as np
+
+from . import _arrays as A
+from . import _capi
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORES = {"max": 0, "top2": 1}
+
+
+def _code(table, value, what):
+    try:
+        return table[value]
+    except (KeyError, TypeError):
+        raise ValueError(f"{what} must be one of {', '.join(map(repr, table))}, not {value!r}") from None
+
+
+def _route_args(scores, top_k, score, n_groups, top_groups, group_score, renormalise, scale, code, ld):
+    n, e = scores.shape
+    a = _capi.RouteArgs(n_rows=n, ld_scores=ld, n_experts=e, top_k=int(top_k), n_groups=int(n_groups),
+                        top_groups=int(n_groups if top_groups is None else top_groups), dtype=code, score=_code(_SCORES, score, "score"),
+                        group_score=_code(_GROUP_SCORES, group_score, "group_score"), renormalise=1 if renormalise else 0, scale=float(scale))
+    a.scores = A.ptr(scores)
+    return a
+
+
+def _device_mask(d, mask, n, e, a):
+    """Boolean (or uint8) [n, e] or [e] -> the tensor to keep alive."""
+    if mask is None:
+        return None
+    mask = d.tensor(mask, "mask")
+    if mask.dtype not in (d.torch.bool, d.torch.uint8):
+        raise ValueError(f"mask is of type {mask.dtype}; bool is expected")
+    if tuple(mask.shape) == (e,):
+        mask, a.ld_mask = mask.contiguous(), 0
+    else:
+        mask = d.matrix(mask, "mask", (n, e))
+        a.ld_mask = mask.stride(0)
+    a.mask = A.ptr(mask)
+    return mask
+
+
+def _host_mask(mask, n, e, a):
+    if mask is None:
+        return None
+    mask = np.ascontiguousarray(mask, dtype=bool).view(np.uint8)
+    if mask.shape not in ((e,), (n, e)):
+        raise ValueError(f"mask has shape {mask.shape}, expected {(n, e)} or {(e,)}")
+    a.ld_mask = 0 if mask.ndim == 1 else e
+    a.mask = A.ptr(mask)
+    return mask
+
+
+def route(scores, top_k: int, *, score: str = "softmax", bias=None, n_groups: int = 1, top_groups: int | None = None,
+          group_score: str = "max", renormalise: bool = True, scale: float = 1.0, mask=None):
+    """Each row's ``top_k`` experts and their weights: (experts [N, k] int32, weights [N, k]).
+
+    ``scores`` [N, E] become probabilities p by ``score`` = "softmax" (over the row's open experts) or "sigmoid".  An expert is
+    open to a row unless ``mask`` [N, E] or [E] is False there or its score is -inf.  The choice goes by p + ``bias`` [E] (a balance
+    correction, finite: it moves the choice, not the weights), highest first, ties to the lower index.  With ``n_groups`` > 1 the experts form groups
+    of consecutive ones, of which the ``top_groups`` best stay open; ``group_score`` = "max" ranks them by their best expert,
+    "top2" by the sum of their two best.  weights = ``scale`` * p, divided by the chosen experts' sum if ``renormalise``.
+
+    Slots that no open expert is left for hold expert -1 and weight 0.  A row with a NaN or +inf among its open scores holds
+    experts -1 and weights NaN.  At most 1024 experts, ``top_k`` at most 64.
+    """
+    if A.on_device(scores):
+        d = A.Device(scores)
+        scores = d.matrix(scores, "scores")
+        n, e = scores.shape
+        code = A.code_of(scores, "scores")
+        a = _route_args(scores, top_k, score, n_groups, top_groups, group_score, renormalise, scale, code, scores.stride(0))
+        mask = _device_mask(d, mask, n, e, a)
+        if bias is not None:
+            bias = d.dense(bias, "bias", (e,))
+            if bias.dtype not in (d.torch.float32, d.torch.float64):
+                bias = bias.to(d.torch.float32)
+            a.bias_f64, a.bias = int(bias.dtype == d.torch.float64), A.ptr(bias)
+        experts, weights = d.empty((n, max(a.top_k, 0)), d.torch.int32), d.empty((n, max(a.top_k, 0)), d.wide(code))
+        a.experts, a.weights = A.ptr(experts), A.ptr(weights)
+        _capi.call_device("route", d.index, d.stream, a)
+        return experts, weights
+    scores = A.host(scores, "scores")
+    n, e = scores.shape
+    a = _route_args(scores, top_k, score, n_groups, top_groups, group_score, renormalise, scale, A.F64, e)
+    mask = _host_mask(mask, n, e, a)
+    if bias is not None:
+        bias = A.host(bias, "bias", (e,))
+        if not np.isfinite(bias).all():
+            raise ValueError("bias is not finite")
+        a.bias_f64, a.bias = 1, A.ptr(bias)
+    experts, weights = np.empty((n, max(a.top_k, 0)), dtype=np.int32), np.empty((n, max(a.top_k, 0)))
+    a.experts, a.weights = A.ptr(experts), A.ptr(weights)
+    _capi.default_context().call("route", a)
+    return experts, weights
+
+
+def route_grad(scores, experts, dweights, *, score: str = "softmax", renormalise: bool = True, scale: float = 1.0, mask=None):
+    """Gradient with respect to ``scores`` from the gradient ``dweights`` [N, k] with respect to :func:`route`'s weights.
+
+    ``experts`` are the ones :func:`route` chose (different ones in every row; -1: none), the other arguments those of its
+    call; the choice itself is not differentiated.  A row without experts has gradient 0.
+    """
+    if A.on_device(scores):
+        d = A.Device(scores)
+        scores = d.matrix(scores, "scores")
+        n, e = scores.shape
+        code = A.code_of(scores, "scores")
+        k = _columns(experts, n, "experts")
+        experts = _device_experts(d, experts, (n, k), e)
+        dweights = d.dense(dweights, "dweights", (n, k), d.wide(code))
+        a = _route_args(scores, k, score, 1, 1, "max", renormalise, scale, code, scores.stride(0))
+        mask = _device_mask(d, mask, n, e, a)
+        out = d.empty((n, e), scores.dtype)
+        a.experts, a.dweights, a.dscores, a.ld_dscores = A.ptr(experts), A.ptr(dweights), A.ptr(out), e
+        _capi.call_device("route_grad", d.index, d.stream, a)
+        return out
+    scores = A.host(scores, "scores")
+    n, e = scores.shape
+    k = _columns(experts, n, "experts")
+    experts = A.host_index(experts, "experts", -1, e)
+    dweights = A.host(dweights, "dweights", (n, k))
+    a = _route_args(scores, k, score, 1, 1, "max", renormalise, scale, A.F64, e)
+    mask = _host_mask(mask, n, e, a)
+    out = np.empty((n, e))
+    a.experts, a.dweights, a.dscores, a.ld_dscores = A.ptr(experts), A.ptr(dweights), A.ptr(out), e
+    _capi.default_context().call("route_grad", a)
+    return out
+
+
+def _columns(experts, n, what):
+    shape = tuple(experts.shape) if hasattr(experts, "shape") else np.shape(experts)
+    if len(shape) != 2 or shape[0] != n:
+        raise ValueError(f"{what} has shape {shape}, expected {n} rows")
+    return shape[1]
+
+
+def _device_experts(d, experts, shape, n_experts):
+    experts = d.tensor(experts, "experts")
+    if experts.dtype == d.torch.int32:
+        return d.dense(experts, "experts", shape)
+    if experts.dtype.is_floating_point or experts.dtype.is_complex or experts.dtype == d.torch.bool:
+        raise ValueError(f"experts must be integers, not {experts.dtype}")
+    return d.dense(experts.clamp(-1, n_experts), "experts", shape, d.torch.int32) if experts.dtype == d.torch.int64 else d.dense(
+        experts, "experts", shape, d.torch.int32)
+
+
+class Plan(NamedTuple):
+    """Where every slot (row n's j-th expert) sits in the layout by expert.
+
+    ``rows`` [N k]: the row at each place, -1 behind the last used one; ``positions``: the place of each slot, -1 for slots without an
+    expert, in the shape of the experts; ``counts`` [E] and ``offsets`` [E + 1]: expert e has the places offsets[e] .. offsets[e + 1).
+    All int32, of the kind (array or tensor) of the experts.
+    """
+    rows: object
+    positions: object
+    counts: object
+    offsets: object
+    n_rows: int
+    top_k: int
+    n_experts: int
+
+
+def plan(experts, n_experts: int) -> Plan:
+    """The layout by expert of ``experts`` [N, k], or of labels [N] (one expert a row, as k-means gives them).
+
+    Slots keep their order within an expert, so the layout depends on nothing but its input.  A slot whose expert is -1 has no place.  On a device any
+    other value outside 0 .. n_experts - 1 has none either; in a NumPy array it is refused.  At most 4096 experts.
+    """
+    n_experts = int(n_experts)
+    shape = tuple(experts.shape) if hasattr(experts, "shape") else np.shape(experts)
+    if len(shape) not in (1, 2):
+        raise ValueError(f"experts has shape {shape}, expected [N, k] or [N]")
+    n, k = shape[0], shape[1] if len(shape) == 2 else 1
+    a = _capi.PlanArgs(n_rows=n, top_k=k, n_experts=n_experts)
+    if A.on_device(experts):
+        d = A.Device(experts)
+        experts = _device_experts(d, experts, shape, n_experts)
+        i32 = d.torch.int32
+        out = [d.empty((n * k,), i32), d.empty(shape, i32), d.empty((max(n_experts, 0),), i32), d.empty((max(n_experts, 0) + 1,), i32)]
+        a.workspace_ints = _capi.plan_workspace(n, k, n_experts)
+        workspace = d.empty((a.workspace_ints,), i32) if a.workspace_ints else None
+        a.workspace = A.ptr(workspace)
+    else:
+        experts = A.host_index(experts, "experts", -1, n_experts)
+        out = [np.empty(s, dtype=np.int32) for s in ((n * k,), shape, (max(n_experts, 0),), (max(n_experts, 0) + 1,))]
+    a.experts = A.ptr(experts)
+    a.rows, a.positions, a.counts, a.offsets = map(A.ptr, out)
+    if A.on_device(experts):
+        _capi.call_device("plan", d.index, d.stream, a)
+    else:
+        _capi.default_context().call("plan", a)
+    return Plan(*out, n, k, n_experts)
+
+
+def _mix(name, plan, first, what, slots_in, weights=None, dout=None):
+    """Common body of dispatch (rows -> slots), combine (slots -> rows) and combine_grad."""
+    if not isinstance(plan, Plan):
+        raise ValueError("plan must come from oak.experts.plan")
+    device = A.on_device(first)
+    if device != A.on_device(plan.positions):
+        raise ValueError(f"{what} and the plan must both be device arrays or both be host arrays")
+    n, k = plan.n_rows, plan.top_k
+    shape = tuple(first.shape) if hasattr(first, "shape") else np.shape(first)
+    rows_in = n * k if slots_in else n
+    if len(shape) not in (1, 2) or shape[0] != rows_in:
+        raise ValueError(f"{what} has shape {shape}, the plan expects {rows_in} rows")
+    flat, c = len(shape) == 1, 1 if len(shape) == 1 else shape[1]
+    a = _capi.MixArgs(n_rows=n, top_k=k, n_experts=plan.n_experts, n_cols=c, ld_rows=c, ld_slots=c, ld_grad=c)
+
+    def two(x):
+        return x[:, None] if flat and x.ndim == 1 else x
+
+    if device:
+        d = A.Device(first)
+        src = d.matrix(two(first), what)
+        a.dtype = A.code_of(src, what)
+        d.tensor(plan.positions, "the plan")
+        wide = d.wide(a.dtype)
+        if weights is not None:
+            weights = d.dense(weights, "weights", (n, k), wide)
+        if dout is not None:
+            dout = d.matrix(two(dout), "dout", (n, c))
+            if dout.dtype != src.dtype:
+                dout = dout.to(src.dtype)
+            a.ld_grad = dout.stride(0)
+        empty = lambda m: d.empty((m, c), src.dtype)                                   # noqa: E731
+        empty_w = lambda: d.empty((n, k), wide)                                        # noqa: E731
+        stride = src.stride(0)
+    else:
+        src = A.host(two(np.asarray(first)), what)
+        if weights is not None:
+            weights = A.host(weights, "weights", (n, k))
+        if dout is not None:
+            dout = A.host(two(np.asarray(dout)), "dout", (n, c))
+        a.dtype = A.F64
+        empty = lambda m: np.empty((m, c))                                             # noqa: E731
+        empty_w = lambda: np.empty((n, k))                                             # noqa: E731
+        stride = c
+    if slots_in:
+        a.ld_slots = stride
+    else:
+        a.ld_rows = stride
+    a.src, a.weights, a.dout = A.ptr(src), A.ptr(weights), A.ptr(dout)
+    a.positions, a.offsets = A.ptr(plan.positions), A.ptr(plan.offsets)
+    if name == "combine_grad":
+        out, dweights = empty(n * k), empty_w()
+        a.dslots, a.dweights = A.ptr(out), A.ptr(dweights)
+    else:
+        out, dweights = empty(n if slots_in else n * k), None
+        a.dst = A.ptr(out)
+    if c == 0:
+        if dweights is not None:
+            dweights[...] = 0
+    elif device:
+        _capi.call_device(name, d.index, d.stream, a)
+    else:
+        _capi.default_context().call(name, a)
+    out = out[:, 0] if flat else out
+    return out if dweights is None else (out, dweights)
+
+
+def dispatch(X, plan: Plan):
+    """Rows ``X`` [N, C] (or [N]) laid out by expert: [N k, C], zeros behind the last used place."""
+    return _mix("dispatch", plan, X, "X", False)
+
+
+def dispatch_grad(dlaid, plan: Plan):
+    """Gradient with respect to ``X`` of :func:`dispatch`: each row's sum over its places of ``dlaid`` [N k, C]."""
+    return _mix("combine", plan, dlaid, "dlaid", True)
+
+
+def combine(answers, weights, plan: Plan):
+    """Sum over each row's experts of weight times answer, [N, C]; ``answers`` [N k, C] (or [N k]) in the plan's layout.
+
+    Slots without a place count as zeros.  What stands behind the last used place is not read.
+    """
+    return _mix("combine", plan, answers, "answers", True, weights=_required(weights, "weights"))
+
+
+def combine_grad(answers, weights, plan: Plan, dout):
+    """Gradients of :func:`combine` from ``dout`` [N, C]: (danswers [N k, C], zeros behind the last used place; dweights [N, k])."""
+    return _mix("combine_grad", plan, answers, "answers", True, weights=_required(weights, "weights"), dout=_required(dout, "dout"))
+
+
+def _required(a, what):
+    if a is None:
+        raise ValueError(f"{what} is missing")
+    return a

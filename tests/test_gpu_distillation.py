@@ -1,0 +1,219 @@
+"""Distillation from a teacher's top logits on the device against the float64 oracle (oracle/experts_oracle.py).
+
+Tolerances, u = 2^-24 (2^-53 for float64).  log z carries d = (far / tau + V / 64 + 16) u: the argument's rounding is u of the
+distance ``far`` of the logits, the exponential's two, and a sum of V terms by at least 64 threads takes at most V / 64 + 12 roundings.  A
+divergence adds d (and a few u of its terms, ``size`` of the oracle) to its value; a gradient entry carries 2 d of both of its parts and
+one rounding to its type, half a step.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oak import distillation as od
+from oracle import experts_oracle as eo
+
+pytestmark = pytest.mark.gpu
+DT = {"f64": torch.float64, "f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def back(t):
+    return t.double().cpu().numpy() if t.is_floating_point() else t.cpu().numpy()
+
+
+def problem(n, v, k, dtype, tail, tau=1.0, seed=0, pad=0, index_64=True, spread=2.0):
+    rng = np.random.default_rng(seed + v)
+    teacher = rng.standard_normal((n, v)) * spread
+    s = torch.as_tensor(0.8 * teacher + rng.standard_normal((n, v)), device="cuda").to(DT[dtype])
+    store = torch.full((n, v + pad), float("nan"), dtype=DT[dtype], device="cuda")
+    off = 1 if pad else 0
+    store[:, off:off + v] = s
+    s = store[:, off:off + v]
+    wide = torch.float64 if dtype == "f64" else torch.float32
+    order = np.argsort(-teacher, 1)[:, :k].copy()
+    top = torch.as_tensor(np.take_along_axis(teacher, order, 1), device="cuda").to(wide)
+    m = teacher.max(1, keepdims=True) / tau
+    lse = torch.as_tensor((m + np.log(np.exp(teacher / tau - m).sum(1, keepdims=True)))[:, 0], device="cuda").to(wide) if tail else None
+    return s, top, torch.as_tensor(order, dtype=torch.int64 if index_64 else torch.int32, device="cuda"), lse
+
+
+def compare(s, top, idx, lse, tau, direction, weight, dtype):
+    kw = dict(top_lse=lse, temperature=tau, direction=direction, row_weight=weight)
+    loss, grad = od.distill_grad(s, top, idx, **kw)
+    only = od.distill(s, top, idx, **kw)
+    assert torch.equal(torch.nan_to_num(only, nan=7.0), torch.nan_to_num(loss, nan=7.0))
+    assert grad.dtype == s.dtype and loss.dtype == (torch.float64 if dtype == "f64" else torch.float32)
+    x = back(s)
+    n, v = x.shape
+    resolution = 2.0 ** -53 if dtype == "f64" else 2.0 ** -24
+    ref, gref, size = eo.distill(x, back(top), back(idx), None if lse is None else back(lse), tau, direction,
+                                 None if weight is None else back(weight), resolution)
+    u = 2.0 ** -53 if dtype == "f64" else 2.0 ** -24
+    finite = np.where(np.isfinite(x), x, np.nan)
+    far = np.array([np.ptp(r[np.isfinite(r)]) if np.isfinite(r).any() else 0.0 for r in finite])
+    far = np.minimum(far, 110.0 * tau)                                   # further down an exponential is 0 in 32 bits
+    d = (far / tau + v / 64 + 16) * u
+    assert np.array_equal(np.isnan(back(loss)), np.isnan(ref)) and np.array_equal(np.isinf(back(loss)), np.isinf(ref))
+    ok = np.isfinite(ref)
+    err, tol = np.abs(back(loss) - np.where(ok, ref, 0)), (2 * d + 4 * u) * (size + np.abs(np.where(ok, ref, 0)))
+    # exact zeros of the oracle's size (rows of weight 0, empty teachers) are zeros here
+    assert (err[ok] <= tol[ok]).all(), (err[ok].max(), tol[ok][err[ok].argmax()])
+    q = np.exp(x / tau - (x / tau).max(1, keepdims=True))
+    q = q / q.sum(1, keepdims=True)
+    w = np.ones(n) if weight is None else back(weight)
+    half = torch.finfo(DT[dtype]).eps / 2
+    gok = np.isfinite(gref)
+    part = np.where(gok, np.abs(gref), 0) + tau * np.abs(w)[:, None] * np.nan_to_num(q)
+    gtol = 2 * d[:, None] * (part + np.nan_to_num(q) * (size / tau)[:, None]) + half * np.abs(np.where(gok, gref, 0)) + 1e-37
+    if dtype == "f16":
+        gtol = gtol + 2.0 ** -25                                         # half a step of the smallest float16 numbers
+    gerr = np.abs(back(grad) - np.where(gok, gref, 0))
+    assert (gerr[gok] <= gtol[gok]).all(), (gerr - gtol)[gok].max()
+    return loss, grad, ref, gref
+
+
+CASES = [
+    # n, V, k, dtype, tail, tau, direction, pad, index_64
+    (1, 1, 1, "f32", False, 1.0, "forward", 0, True),
+    (4, 2, 1, "bf16", True, 1.0, "reverse", 0, False),
+    (7, 10, 10, "f32", True, 1.0, "forward", 0, True),                  # the entries are all the classes: no rest
+    (7, 10, 10, "f32", True, 1.0, "reverse", 0, True),
+    (70, 100, 5, "f64", True, 2.0, "reverse", 3, True),
+    (33, 1000, 10, "f32", False, 2.0, "forward", 0, False),
+    (20, 1024, 256, "bf16", True, 1.0, "forward", 0, True),
+    (6, 1024, 300, "f16", True, 0.7, "forward", 1, True),
+    (9, 1025, 3, "bf16", True, 4.0, "forward", 1, True),
+    (5, 4099, 64, "f16", False, 1.0, "forward", 0, True),
+    (3, 8191, 1024, "f32", True, 1.5, "reverse", 11, False),
+    (4, 16384, 20, "bf16", True, 1.0, "forward", 0, True),
+    (2, 50021, 33, "f32", True, 1.5, "reverse", 3, True),
+    (3, 49157, 20, "f16", True, 1.0, "forward", 0, True),
+    (2, 131072, 128, "bf16", True, 1.0, "forward", 0, True),
+    (2, 140001, 7, "bf16", False, 1.0, "forward", 0, True),
+    (2, 30000, 17, "f64", True, 1.0, "forward", 1, True),
+    (1, 1 << 20, 1024, "bf16", True, 1.0, "forward", 0, True),
+]
+
+
+@pytest.mark.parametrize("n,v,k,dtype,tail,tau,direction,pad,index_64", CASES)
+def test_distill(n, v, k, dtype, tail, tau, direction, pad, index_64):
+    s, top, idx, lse = problem(n, v, k, dtype, tail, tau, 0, pad, index_64)
+    w = torch.rand(n, device="cuda", dtype=top.dtype) + 0.5
+    compare(s, top, idx, lse, tau, direction, w, dtype)
+
+
+@pytest.mark.parametrize("v", [50, 3000, 40000])
+@pytest.mark.parametrize("direction", ["forward", "reverse"])
+def test_ragged_teachers_masked_rows_and_wrong_indices(v, direction):
+    s, top, idx, lse = problem(12, v, 9, "bf16", True, seed=3)
+    s, top, idx = s.clone(), top.clone(), idx.clone()
+    idx[0, 4:] = -1                                                      # padding by index,
+    top[1, 2:] = -float("inf")                                           # by value,
+    idx[2] = -1                                                          # a teacher that kept nothing
+    s[3] = float("nan")                                                  # a row that is left out may hold anything
+    idx[3, 0] = v + 5
+    idx[4, 3] = v                                                        # no class
+    idx[5, 0] = -2
+    s[6, :v // 2] = -float("inf")                                        # classes the student rules out ...
+    top[6, 0], idx[6, 0] = 1.0, 0                                        # ... one of which the teacher holds
+    s[7, 3] = float("nan")
+    s[8] = torch.finfo(torch.bfloat16).min                               # all at the type's lowest value: uniform
+    w = torch.ones(12, device="cuda")
+    w[3] = 0
+    loss, grad, _, _ = compare(s, top, idx, lse, 1.0, direction, w, "bf16")
+    loss, grad = back(loss), back(grad)
+    assert loss[2] == 0 and loss[3] == 0 and (grad[2] == 0).all() and (grad[3] == 0).all()
+    assert np.isnan(loss[[4, 5, 7]]).all() and np.isnan(grad[4]).all() and np.isnan(grad[5]).all()
+    if direction == "forward":
+        assert np.isposinf(loss[6])
+    assert np.isfinite(loss[[0, 1, 8, 9, 10, 11]]).all()
+
+
+@pytest.mark.parametrize("v", [40, 5000])
+@pytest.mark.parametrize("direction", ["forward", "reverse"])
+def test_entries_of_one_class_are_merged(v, direction):
+    s, top, idx, lse = problem(6, v, 12, "f32", True, seed=8)
+    idx = idx.clone()
+    idx[0, 5] = idx[0, 2]
+    idx[1, :] = idx[1, 0]
+    idx[2, 11] = idx[2, 0]
+    lse = torch.logsumexp(top, 1) + 0.3
+    compare(s, top, idx, lse, 1.0, direction, None, "f32")
+    if direction == "forward":
+        compare(s, top, idx, None, 1.0, direction, None, "f32")
+
+
+@pytest.mark.parametrize("v", [64, 4096])
+def test_a_student_that_is_sure_of_itself_keeps_its_rest(v):
+    """The rest's mass far below the rounding of the top's: its logarithm has to come from the rest itself."""
+    s = torch.zeros(2, v, device="cuda", dtype=torch.float64)
+    s[0, 5], s[1, 5] = 60.0, 300.0
+    for dtype in ("f32", "f64", "bf16"):
+        top = torch.full((2, 1), 3.0, device="cuda", dtype=torch.float64 if dtype == "f64" else torch.float32)
+        idx = torch.full((2, 1), 5, device="cuda")
+        lse = torch.full((2,), 3.5, device="cuda", dtype=top.dtype)
+        compare(s.to(DT[dtype]), top, idx, lse, 1.0, "forward", None, dtype)
+
+
+def test_types_of_the_teacher():
+    s, top, idx, lse = problem(20, 300, 8, "bf16", True)
+    for t in (torch.bfloat16, torch.float16, torch.float64):
+        compare(s, top.to(t), idx.to(torch.int32), lse.double(), 1.0, "forward", torch.ones(20, device="cuda", dtype=t), "bf16")
+    s32, top, idx, lse = problem(20, 300, 8, "f64", True)
+    compare(s32, top.float(), idx, lse.float(), 1.0, "forward", None, "f64")
+
+
+def test_strides():
+    s, top, idx, lse = problem(16, 200, 6, "f32", True)
+    wide = torch.zeros(16, 20, device="cuda")
+    wide[:, 3:9] = top
+    compare(s.t().contiguous().t(), wide[:, 3:9], idx.t().contiguous().t(), lse, 1.0, "forward", None, "f32")
+    one = s[:1].expand(5, 200)                                           # one row for all
+    loss = od.distill(one, top[:1].expand(5, 6), idx[:1].expand(5, 6), top_lse=lse[:1].expand(5))
+    assert torch.equal(loss, od.distill(s[:1], top[:1], idx[:1], top_lse=lse[:1]).expand(5))
+    loss, grad = od.distill_grad(s[:0], top[:0], idx[:0])
+    assert loss.shape == (0,) and grad.shape == (0, 200)
+
+
+def test_numpy_arrays_and_differences():
+    rng = np.random.default_rng(1)
+    n, v, k = 9, 30, 5
+    teacher, s = rng.standard_normal((n, v)) * 2, rng.standard_normal((n, v))
+    idx = np.argsort(-teacher, 1)[:, :k].copy()
+    top, lse = np.take_along_axis(teacher, idx, 1), np.log(np.exp(teacher / 1.3).sum(1))
+    idx[2, 3:] = -1
+    w = rng.random(n) + 0.2
+    for direction, given in (("forward", None), ("forward", lse), ("reverse", lse)):
+        kw = dict(top_lse=given, temperature=1.3, direction=direction, row_weight=w)
+        loss, grad = od.distill_grad(s, top, idx, **kw)
+        ref, gref, _ = eo.distill(s, top, idx, given, 1.3, direction, w)
+        np.testing.assert_allclose(loss, ref, rtol=1e-12, atol=1e-13)
+        np.testing.assert_allclose(grad, gref, rtol=1e-11, atol=1e-13)
+        np.testing.assert_array_equal(od.distill(s, top, idx, **kw), loss)
+        np.testing.assert_allclose(grad.sum(1), 0, atol=1e-12)           # a shift of all logits changes nothing
+        for i, j in ((0, idx[0, 0]), (2, 7), (5, idx[5, 4]), (8, 29)):
+            up, down = s.copy(), s.copy()
+            up[i, j] += 1e-5
+            down[i, j] -= 1e-5
+            fd = (od.distill(up, top, idx, **kw).sum() - od.distill(down, top, idx, **kw).sum()) / 2e-5
+            assert abs(fd - grad[i, j]) <= 1e-8
+
+
+def test_streams_and_captured_graphs():
+    s, top, idx, lse = problem(40, 9000, 16, "bf16", True)
+    s = s.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = od.distill_grad(s, top, idx, top_lse=lse)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(od.distill_grad(s, top, idx, top_lse=lse), other):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = od.distill_grad(s, top, idx, top_lse=lse)
+    for seed in range(4):
+        s.copy_(torch.randn(s.shape, generator=torch.Generator().manual_seed(seed)).to("cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(od.distill_grad(s, top, idx, top_lse=lse), held):
+            assert torch.equal(a, b)

@@ -1,0 +1,349 @@
+"""Routing, layout by expert and combination on the device against the float64 oracle (oracle/experts_oracle.py).
+
+Tolerances, u = 2^-24 (2^-53 for float64): the chosen experts and the plan are integers and must be equal.  Weights that are formed in
+64 bits carry one rounding; the plain softmax carries its exponentials (argument rounding |x - max| u, function 2 u), a sum of at most 16
+terms a lane and 6 steps across lanes, a division and a product: (|x - max| + 32) u.  A result of a 16-bit type adds half a step, eps / 2.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oak import experts as ox
+from oracle import experts_oracle as eo
+
+pytestmark = pytest.mark.gpu
+DT = {"f64": torch.float64, "f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def unit(dtype):
+    return 2.0 ** -53 if dtype == "f64" else 2.0 ** -24
+
+
+def half_step(dtype, ref):
+    """Half a step of the type around ref; float16 numbers below 2^-14 are 2^-24 apart."""
+    return torch.finfo(DT[dtype]).eps / 2 * np.abs(ref) + (2.0 ** -25 if dtype == "f16" else 0.0)
+
+
+def tensor(a, dtype=None, pad=0):
+    """On the device; ``pad`` puts the rows into a wider array one element off its start."""
+    t = torch.as_tensor(np.ascontiguousarray(a)).to("cuda")
+    t = t if dtype is None else t.to(DT[dtype])
+    if pad:
+        store = torch.full((t.shape[0], t.shape[1] + pad), float("nan") if t.is_floating_point() else 0, dtype=t.dtype, device="cuda")
+        store[:, 1:1 + t.shape[1]] = t
+        t = store[:, 1:1 + t.shape[1]]
+    return t
+
+
+def back(t):
+    return t.double().cpu().numpy() if t.is_floating_point() else t.cpu().numpy()
+
+
+def scores_of(rng, n, e, dtype, pad=0, spread=1.5):
+    t = tensor(rng.standard_normal((n, e)) * spread, dtype, pad)
+    return t, back(t)
+
+
+ROUTE = [
+    # n, E, k, dtype, options
+    (1, 1, 1, "f32", {}),
+    (5, 2, 2, "bf16", {"score": "sigmoid"}),
+    (257, 7, 3, "f32", {"renormalise": False}),
+    (33, 16, 16, "f16", {}),
+    (100, 17, 4, "bf16", {"bias": True}),
+    (301, 24, 2, "f32", {"renormalise": False, "pad": 5}),
+    (64, 33, 5, "f64", {"mask": 0.5}),
+    (130, 64, 6, "bf16", {"pad": 3}),
+    (70, 65, 8, "f32", {"score": "sigmoid", "bias": True, "scale": 2.5}),
+    (50, 128, 1, "bf16", {"renormalise": False, "mask": 0.1}),
+    (43, 160, 6, "bf16", {"renormalise": False, "mask": 0.9}),
+    (90, 256, 8, "bf16", {"score": "sigmoid", "bias": True, "n_groups": 8, "top_groups": 4, "group_score": "top2", "scale": 2.5}),
+    (31, 300, 16, "f16", {"bias": True, "n_groups": 10, "top_groups": 3}),
+    (20, 513, 64, "f32", {"score": "sigmoid", "renormalise": False}),
+    (9, 1024, 33, "f64", {"bias": True, "mask": 0.7, "n_groups": 64, "top_groups": 9, "group_score": "top2"}),
+    (200, 60, 4, "bf16", {"n_groups": 6, "top_groups": 2, "mask": 0.15}),
+    (65, 64, 3, "f32", {"n_groups": 64, "top_groups": 3, "group_score": "top2"}),
+    (65, 64, 3, "f32", {"n_groups": 1, "mask": "shared"}),
+]
+
+
+def route_case(n, e, k, dtype, opt, seed=0):
+    rng = np.random.default_rng(seed + 1000 * e + n)
+    opt = dict(opt)
+    x, xr = scores_of(rng, n, e, dtype, opt.pop("pad", 0))
+    kw = dict(opt)
+    host = dict(opt)
+    if opt.get("bias"):
+        b = torch.as_tensor(rng.standard_normal(e) * 0.05, dtype=torch.float32, device="cuda")
+        kw["bias"], host["bias"] = b, back(b)
+    if "mask" in opt:
+        m = rng.random(e) < 0.5 if opt["mask"] == "shared" else rng.random((n, e)) < opt["mask"]
+        if opt["mask"] != "shared" and n > 2:
+            m[n // 2] = False                                            # a row that is left nothing
+        kw["mask"], host["mask"] = torch.as_tensor(m, device="cuda"), m
+    return x, xr, kw, host
+
+
+def check_weights(w, ref, xr, experts, dtype, kw):
+    formed_wide = kw.get("renormalise", True) or kw.get("score") == "sigmoid"
+    far = np.ptp(np.where(np.isfinite(xr), xr, 0.0)) if xr.size else 0.0
+    tol = (2 if formed_wide and dtype != "f64" else far + 32) * unit(dtype)
+    np.testing.assert_allclose(w, ref, rtol=tol, atol=1e-37)
+
+
+@pytest.mark.parametrize("n,e,k,dtype,opt", ROUTE)
+def test_route(n, e, k, dtype, opt):
+    x, xr, kw, host = route_case(n, e, k, dtype, opt)
+    ex, w = ox.route(x, k, **kw)
+    er, wr = eo.route(xr, k, **host)
+    assert ex.dtype == torch.int32 and w.dtype == (torch.float64 if dtype == "f64" else torch.float32)
+    np.testing.assert_array_equal(back(ex), er)
+    check_weights(back(w), wr, xr, er, dtype, kw)
+
+
+@pytest.mark.parametrize("n,e,k,dtype,opt", ROUTE)
+def test_route_grad(n, e, k, dtype, opt):
+    x, xr, kw, host = route_case(n, e, k, dtype, opt)
+    ex, _ = ox.route(x, k, **kw)
+    for name in ("bias", "n_groups", "top_groups", "group_score"):
+        kw.pop(name, None), host.pop(name, None)
+    rng = np.random.default_rng(7)
+    dw = torch.as_tensor(rng.standard_normal((n, k)), dtype=torch.float64 if dtype == "f64" else torch.float32, device="cuda")
+    dx = ox.route_grad(x, ex, dw, **kw)
+    assert dx.dtype == x.dtype and dx.shape == x.shape
+    ref = eo.route_grad(xr, back(ex), back(dw), **host)
+    # every probability carries (|x - max| + 32) u, the bracket a few u of its two parts; the result one rounding
+    far = np.ptp(xr) if xr.size else 0.0
+    g = kw.get("scale", 1.0) * np.abs(back(dw)).max(initial=0.0)
+    one = np.exp(xr - xr.max(1, keepdims=True)) if kw.get("score", "softmax") == "softmax" else np.ones_like(xr)
+    tol = 2 * (far + 40) * unit(dtype) * 2 * g * np.minimum(one * e, 1.0) + half_step(dtype, ref) + 1e-37
+    assert (np.abs(back(dx) - ref) <= tol).all(), np.abs(back(dx) - ref).max()
+
+
+def test_route_ties_go_to_the_lowest_expert():
+    x = torch.zeros(3, 100, device="cuda", dtype=torch.bfloat16)
+    x[1, 40:60] = 1.0
+    x[2] = torch.arange(100, device="cuda") % 2
+    ex, w = ox.route(x, 5)
+    np.testing.assert_array_equal(back(ex), [[0, 1, 2, 3, 4], [40, 41, 42, 43, 44], [1, 3, 5, 7, 9]])
+    np.testing.assert_allclose(back(w), 0.2, rtol=2 * 2.0 ** -24)
+    ex, _ = ox.route(x, 5, bias=torch.zeros(100, device="cuda"), score="sigmoid", n_groups=10, top_groups=2)
+    np.testing.assert_array_equal(back(ex)[0], [0, 1, 2, 3, 4])
+    np.testing.assert_array_equal(back(ex)[1], [40, 41, 42, 43, 44])
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalise", [True, False])
+def test_route_infinities_nan_and_lowest_values(score, renormalise):
+    inf, nan, low = np.inf, np.nan, float(np.finfo(np.float32).min)
+    x = np.array([[1.0, -inf, 2.0, 0.0], [-inf, -inf, -inf, -inf], [1.0, nan, 2.0, 0.0], [inf, 1.0, 0.0, 0.0], [low, low, low, low],
+                  [low, 3.0, low, -inf], [nan, inf, 1.0, 2.0], [-200.0, -201.0, -300.0, -250.0]])
+    mask = np.ones_like(x, bool)
+    mask[6, :2] = False                                                  # NaN and infinity in masked places do no harm
+    t, m = tensor(x, "f32"), torch.as_tensor(mask, device="cuda")
+    kw = dict(score=score, renormalise=renormalise, mask=m)
+    ex, w = ox.route(t, 3, **kw)
+    er, wr = eo.route(back(t), 3, score=score, renormalise=renormalise, mask=mask)
+    np.testing.assert_array_equal(back(ex), er)
+    np.testing.assert_allclose(back(w), wr, rtol=64 * 2.0 ** -24, atol=1e-37)
+    dw = torch.ones(len(x), 3, device="cuda") * torch.arange(1, 4, device="cuda")
+    dx = back(ox.route_grad(t, ex, dw, **kw))
+    ref = eo.route_grad(back(t), er, back(dw), score=score, renormalise=renormalise, mask=mask)
+    assert (dx[1] == 0).all() and (dx[2] == 0).all() and (dx[3] == 0).all()    # rows without experts
+    np.testing.assert_allclose(dx, ref, rtol=64 * 2.0 ** -24, atol=256 * 2.0 ** -24)
+
+
+def test_route_strides_offsets_and_empty():
+    rng = np.random.default_rng(3)
+    base = tensor(rng.standard_normal((40, 50)), "bf16")
+    ex, w = ox.route(base.t(), 4)                                        # columns not consecutive
+    er, wr = eo.route(back(base).T, 4)
+    np.testing.assert_array_equal(back(ex), er)
+    one = base[:1].expand(9, 50)                                         # row stride 0
+    ex, _ = ox.route(one, 2)
+    np.testing.assert_array_equal(back(ex), np.repeat(eo.route(back(base[:1]), 2)[0], 9, 0))
+    ex, w = ox.route(base[:0], 4)
+    assert ex.shape == (0, 4) and w.shape == (0, 4)
+    assert ox.route_grad(base[:0], ex, w).shape == (0, 50)
+
+
+PLANS = [(0, 2, 5), (1, 1, 1), (3, 2, 16), (64, 1, 7), (1000, 6, 160), (4096, 4, 1024), (4097, 4, 24), (5000, 4, 1025), (40000, 2, 3),
+         (70001, 8, 333), (6000, 3, 4096)]
+
+
+@pytest.mark.parametrize("n,k,e", PLANS)
+def test_plan(n, k, e):
+    rng = np.random.default_rng(n + e)
+    ex = rng.integers(-1, e, (n, k))
+    ex[rng.random((n, k)) < 0.3] = e // 2                                # one much sought after
+    p = ox.plan(torch.as_tensor(ex, dtype=torch.int32, device="cuda"), e)
+    for got, ref in zip(p[:4], eo.plan(ex, e)):
+        np.testing.assert_array_equal(back(got), ref)
+    p64 = ox.plan(torch.as_tensor(ex, dtype=torch.int64, device="cuda"), e)
+    np.testing.assert_array_equal(back(p64.positions), back(p.positions))
+
+
+def test_plan_of_labels_and_of_numbers_that_are_no_experts():
+    labels = np.array([2, 0, 2, 1, 0, 2], dtype=np.int32)
+    p = ox.plan(torch.as_tensor(labels, device="cuda"), 3)
+    np.testing.assert_array_equal(back(p.rows), [1, 4, 3, 0, 2, 5])
+    np.testing.assert_array_equal(back(p.offsets), [0, 2, 3, 6])
+    assert p.positions.shape == (6,)
+    for dtype in (torch.int32, torch.int64):
+        odd = torch.as_tensor([[0, 7], [-5, 1], [2 ** 31 - 1, 2]], dtype=dtype, device="cuda")
+        p = ox.plan(odd, 3)
+        np.testing.assert_array_equal(back(p.positions), [[0, -1], [-1, 1], [-1, 2]])
+        np.testing.assert_array_equal(back(p.rows), [0, 1, 2, -1, -1, -1])
+    p = ox.plan(torch.as_tensor([2 ** 32, 0], dtype=torch.int64, device="cuda"), 3)
+    np.testing.assert_array_equal(back(p.positions), [-1, 0])
+
+
+MIXES = [(1, 1, 1, 1, "f32", 0), (3, 2, 16, 64, "f32", 0), (50, 2, 5, 17, "f64", 0), (200, 6, 40, 33, "bf16", 3), (129, 4, 7, 257, "f16", 1),
+         (64, 8, 8, 2048, "bf16", 0), (31, 3, 3, 4100, "f32", 5), (2500, 2, 24, 3, "bf16", 0), (10, 64, 64, 8, "f64", 0)]
+
+
+@pytest.mark.parametrize("n,k,e,c,dtype,pad", MIXES)
+def test_dispatch_combine_and_gradients(n, k, e, c, dtype, pad):
+    rng = np.random.default_rng(n * c + k)
+    ex = np.stack([rng.permutation(e)[:k] for _ in range(n)])
+    ex[rng.random((n, k)) < 0.2] = -1
+    p = ox.plan(torch.as_tensor(ex, dtype=torch.int32, device="cuda"), e)
+    used, pos = int(p.offsets[e]), back(p.positions)
+    wide = torch.float64 if dtype == "f64" else torch.float32
+    u = unit(dtype)
+    X = tensor(rng.standard_normal((n, c)), dtype, pad)
+    laid = ox.dispatch(X, p)
+    np.testing.assert_array_equal(back(laid), eo.dispatch(back(X), back(p.rows)))
+    F = tensor(rng.standard_normal((n * k, c)), dtype, pad)
+    F[used:] = float("nan")                                              # never read
+    w = torch.as_tensor(rng.standard_normal((n, k)), dtype=wide, device="cuda")
+    y = ox.combine(F, w, p)
+    Fr, wr = back(F), back(w)
+    ref = eo.combine(Fr, wr, pos)
+    size = eo.combine(np.abs(Fr), np.abs(wr), pos)
+    assert (np.abs(back(y) - ref) <= (k + 1) * u * size + half_step(dtype, ref)).all()
+    dy = tensor(rng.standard_normal((n, c)), dtype, pad)
+    dF, dw = ox.combine_grad(F, w, p, dy)
+    dFr, dwr = eo.combine_grad(np.where(np.isnan(Fr), 0.0, Fr), wr, pos, back(dy))
+    assert (np.abs(back(dF) - dFr) <= u * np.abs(dFr) + half_step(dtype, dFr)).all()
+    assert (back(dF)[used:] == 0).all()
+    _, sizes = eo.combine_grad(np.abs(np.where(np.isnan(Fr), 0.0, Fr)), wr, pos, np.abs(back(dy)))
+    assert (np.abs(back(dw) - dwr) <= (c / 8 + 20) * u * sizes).all() and dw.dtype == wide
+    dX = ox.dispatch_grad(F, p)
+    ones = np.ones((n, k))
+    dXr = eo.combine(Fr, ones, pos)
+    assert (np.abs(back(dX) - dXr) <= (k + 1) * u * eo.combine(np.abs(Fr), ones, pos) + half_step(dtype, dXr)).all()
+
+
+def test_combine_shows_the_weights_of_a_row_without_an_answer():
+    x = torch.tensor([[0.0, 1.0], [float("nan"), 0.0]], device="cuda")
+    ex, w = ox.route(x, 1)
+    p = ox.plan(ex, 2)
+    y = ox.combine(torch.ones(2, 3, device="cuda"), w, p)
+    assert (back(y)[0] == 1).all() and np.isnan(back(y)[1]).all()
+
+
+def test_mix_of_vectors_and_of_nothing():
+    p = ox.plan(torch.tensor([1, 0, 1], dtype=torch.int32, device="cuda"), 2)
+    X = torch.tensor([1.0, 2.0, 3.0], device="cuda")
+    laid = ox.dispatch(X, p)
+    np.testing.assert_array_equal(back(laid), [2, 1, 3])
+    np.testing.assert_array_equal(back(ox.combine(laid, torch.ones(3, 1, device="cuda"), p)), [1, 2, 3])
+    np.testing.assert_array_equal(back(ox.dispatch_grad(laid, p)), [1, 2, 3])
+    empty = ox.plan(torch.empty(0, 2, dtype=torch.int32, device="cuda"), 4)
+    assert ox.dispatch(torch.empty(0, 5, device="cuda"), empty).shape == (0, 5)
+    assert ox.dispatch(torch.empty(3, 0, device="cuda"), p).shape == (3, 0)
+
+
+def test_numpy_arrays_give_the_same_numbers():
+    rng = np.random.default_rng(11)
+    x, b = rng.standard_normal((77, 20)), rng.standard_normal(20) * 0.05
+    m = rng.random((77, 20)) < 0.6
+    for kw in (dict(), dict(score="sigmoid", bias=b, n_groups=4, top_groups=2), dict(renormalise=False, mask=m), dict(mask=m[0])):
+        ex, w = ox.route(x, 3, **kw)
+        er, wr = eo.route(x, 3, **kw)
+        np.testing.assert_array_equal(ex, er)
+        np.testing.assert_allclose(w, wr, rtol=1e-13, atol=1e-300)
+        kw = {k: v for k, v in kw.items() if k in ("score", "renormalise", "mask")}
+        dw = rng.standard_normal((77, 3))
+        np.testing.assert_allclose(ox.route_grad(x, ex, dw, **kw), eo.route_grad(x, er, dw, **kw), rtol=1e-12, atol=1e-14)
+    for shape, e in (((77, 3), 20), ((9000, 4), 50), ((30,), 4), ((0, 2), 3)):
+        ex = rng.integers(-1, e, shape)
+        p = ox.plan(ex, e)
+        for got, ref in zip(p[:4], eo.plan(ex, e)):
+            np.testing.assert_array_equal(got, ref)
+    ex = rng.integers(-1, 20, (77, 3))
+    p = ox.plan(ex, 20)
+    X, F, w, dy = rng.standard_normal((77, 5)), rng.standard_normal((231, 5)), rng.standard_normal((77, 3)), rng.standard_normal((77, 5))
+    np.testing.assert_array_equal(ox.dispatch(X, p), eo.dispatch(X, p.rows))
+    np.testing.assert_allclose(ox.combine(F, w, p), eo.combine(F, w, p.positions), rtol=1e-12, atol=1e-13)
+    for got, ref in zip(ox.combine_grad(F, w, p, dy), eo.combine_grad(F, w, p.positions, dy)):
+        np.testing.assert_allclose(got, ref, rtol=1e-12, atol=1e-13)
+    np.testing.assert_allclose(ox.dispatch_grad(F, p), eo.combine(F, np.ones((77, 3)), p.positions), rtol=1e-12, atol=1e-13)
+
+
+def test_gradients_against_differences():
+    """sum(c * combine(F, route(x))) differentiated through the calls of this module and by central differences (float64)."""
+    rng = np.random.default_rng(5)
+    n, e, k, c = 12, 9, 3, 4
+    x, coef = rng.standard_normal((n, e)) * 1.5, rng.standard_normal((n, c))
+    F = rng.standard_normal((n * k, c))
+    for kw in (dict(), dict(renormalise=False), dict(score="sigmoid", scale=1.7), dict(score="sigmoid", renormalise=False)):
+        ex, w = ox.route(x, k, **kw)
+        p = ox.plan(ex, e)
+        dF, dw = ox.combine_grad(F, w, p, coef)
+        dx = ox.route_grad(x, ex, dw, **kw)
+
+        def value(xx, ff):
+            ee, ww = ox.route(xx, k, **kw)
+            assert (ee == ex).all()
+            return (coef * ox.combine(ff, ww, p)).sum()
+
+        h = 1e-5
+        for i, j in ((0, ex[0, 0]), (3, ex[3, 1]), (7, ex[7, 2]), (5, int(np.argmin(x[5])))):
+            up, down = x.copy(), x.copy()
+            up[i, j] += h
+            down[i, j] -= h
+            assert abs((value(up, F) - value(down, F)) / (2 * h) - dx[i, j]) <= 1e-8
+        for s, j in ((0, 0), (20, 3)):
+            up, down = F.copy(), F.copy()
+            up[s, j] += h
+            down[s, j] -= h
+            assert abs((value(x, up) - value(x, down)) / (2 * h) - dF[s, j]) <= 1e-8
+
+
+def test_streams_and_captured_graphs():
+    """Another stream than the default one, and a captured step that is replayed on new inputs between eager work."""
+    rng = np.random.default_rng(2)
+    n, e, k, c = 3000, 40, 4, 96
+    x, X, dy = tensor(rng.standard_normal((n, e)), "f32"), tensor(rng.standard_normal((n, c)), "bf16"), tensor(rng.standard_normal((n, c)), "bf16")
+
+    def step():
+        ex, w = ox.route(x, k, renormalise=False)
+        p = ox.plan(ex, e)
+        laid = ox.dispatch(X, p)
+        y = ox.combine(laid, w, p)
+        dF, dw = ox.combine_grad(laid, w, p, dy)
+        return ex, w, p.rows, p.positions, p.offsets, laid, y, dF, dw, ox.route_grad(x, ex, dw, renormalise=False), ox.dispatch_grad(dF, p)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        other = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(step(), other):
+        assert torch.equal(a, b)
+    graph, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    with torch.cuda.graph(second):
+        held2 = step()
+    for seed in range(4):
+        x.copy_(tensor(np.random.default_rng(seed).standard_normal((n, e)), "f32"))
+        X.copy_(tensor(np.random.default_rng(seed + 50).standard_normal((n, c)), "bf16"))
+        graph.replay()
+        second.replay()
+        torch.cuda.synchronize()
+        for a, b, c2 in zip(step(), held, held2):
+            assert torch.equal(a, b) and torch.equal(a, c2)
