@@ -14,193 +14,310 @@ namespace oak {
 // route
 // ---------------------------------------------------------------------------------------------------------------------
 // A row belongs to a team of L lanes; lane l of the team holds the experts [l VPL, (l + 1) VPL) in registers, so that the row is read
-// once, in pieces of VPL consecutive scores.  The k best are taken one after the other: the largest key of the team, then the
-// lowest expert that has it (ties go to the lowest index), then that one is struck out.
+// once, in pieces of VPL consecutive scores.  The k best are taken one after the other: the largest key of the team, then that one is
+// struck out; lane j keeps the j-th (L >= k).
 //
-// Keys: the scores themselves where nothing is added to them -- softmax and sigmoid keep their order, and no rounding can tie what
-// differs.  With a bias (or group scores that add two probabilities) the keys are probabilities in 64 bits: scores next to each other
-// differ by less than the rounding of 32 bits often enough to matter (a few rows in ten thousand).
-template <typename T, int VPL> __device__ __forceinline__ void load_scores(const T* p, int base, int E, typename Num<T>::acc (&x)[VPL]) {
-    using acc = typename Num<T>::acc;
-    typedef T block __attribute__((ext_vector_type(VPL)));
-    typedef block block_at __attribute__((aligned(sizeof(T))));
-    if (base + VPL <= E) {
-        const block b = *reinterpret_cast<const block_at*>(p + base);
-#pragma unroll
-        for (int s = 0; s < VPL; ++s) x[s] = (acc)b[s];
-    } else {
-#pragma unroll
-        for (int s = 0; s < VPL; ++s) x[s] = base + s < E ? (acc)p[base + s] : (acc)0;
-    }
-}
+// Keys.  Where nothing is added to the scores the keys are the scores themselves: softmax and sigmoid keep their order, and no rounding
+// can tie what differs.  With a bias, or group scores that add two probabilities, the keys are probabilities in 64 bits: scores next to
+// each other differ by less than the rounding of 32 bits often enough to matter (a few rows in ten thousand).
+// A key carries its expert in its last bits, in the order that makes the larger key the lower expert, so that one maximum finds
+// both and ties resolve themselves:
+//   KEY_16   16-bit scores: a 32-bit integer, the score's bits in ascending order over 13 bits that no such score uses -- one instruction a step
+//   KEY_TAG  float scores and probabilities: a double whose last 10 of 52 bits are the tag (float scores do not reach them;
+//            probabilities closer than 2^-42 of their size count as tied)
+//   KEY_F64  double scores: all bits belong to the key, the expert is found in a second step
+// Bound by instruction issue (16384 x 256 bf16, sigmoid + bias, 4 of 8 groups, k = 8: 38 us before, see the table of measured times), not by memory.
+enum { KEY_16 = 0, KEY_TAG = 1, KEY_F64 = 2 };
 
 struct RouteDev {
     int64_t n, ld, ld_mask, ld_out;
-    int E, k, groups, top_groups, group_size;
-    int sigmoid, top2, renorm, bias_f64;
+    int E, k, groups, top_groups, group_size, lanes_per_group;
+    int dtype, sigmoid, top2, renorm, bias_f64;
     double scale;
     const void* scores; const void* bias; const unsigned char* mask;
     int* experts; void* weights;
     const void* dweights; void* dscores;
 };
 
-// log of the sigmoid, finite for every finite x
-__device__ __forceinline__ double log_sigmoid(double x) { return (x < 0.0 ? x : 0.0) - log1p(exp(-fabs(x))); }
+template <typename T, int VPL, typename A> __device__ __forceinline__ void load_pieces(const T* p, int base, int E, A (&x)[VPL], A out_of_range) {
+    typedef T four __attribute__((ext_vector_type(4)));
+    typedef four four_at __attribute__((aligned(sizeof(T))));
+#pragma unroll
+    for (int c = 0; c < VPL; c += 4) {
+        if (base + c + 4 <= E) {
+            const four b = *reinterpret_cast<const four_at*>(p + base + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[c + i] = (A)b[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[c + i] = base + c + i < E ? (A)p[base + c + i] : out_of_range;
+        }
+    }
+}
+// the lane's piece of a row of scores; the element type is a uniform branch: one kernel serves all of a kind
+template <int VPL> __device__ __forceinline__ void load_scores(const RouteDev& a, int64_t row, int base, float (&x)[VPL]) {
+    if (a.dtype == OAK_BF16) load_pieces<__bf16, VPL>(static_cast<const __bf16*>(a.scores) + row * a.ld, base, a.E, x, 0.0f);
+    else if (a.dtype == OAK_F16) load_pieces<_Float16, VPL>(static_cast<const _Float16*>(a.scores) + row * a.ld, base, a.E, x, 0.0f);
+    else load_pieces<float, VPL>(static_cast<const float*>(a.scores) + row * a.ld, base, a.E, x, 0.0f);
+}
+template <int VPL> __device__ __forceinline__ void load_scores(const RouteDev& a, int64_t row, int base, double (&x)[VPL]) {
+    load_pieces<double, VPL>(static_cast<const double*>(a.scores) + row * a.ld, base, a.E, x, 0.0);
+}
+template <typename A> __device__ __forceinline__ A score_at(const RouteDev& a, int64_t row, int e) { return (A)load_any(a.scores, a.dtype, row * a.ld + e); }
+
+// 2^y in the accuracy of A; exp(t) = 2^(t log2 e), the float form with log2 e in two parts (both positive: t = -inf gives 0)
+__device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(__builtin_fmaf(t, 1.44269502162933349609f, t * 1.92596299112661e-8f)); }
+// Cody-Waite reduction and the Taylor polynomial of degree 12 on |r| <= ln 2 / 2 (remainder 1.7e-16), without the special cases of exp()
+__device__ __forceinline__ double exp_of(double t) {
+    t = t > -800.0 ? t : -800.0;
+    const double n = __builtin_rint(t * 1.4426950408889634074);
+    const double r = __builtin_fma(n, -1.9082149292705877e-10, __builtin_fma(n, -6.93147180369123816490e-01, t));
+    double p = 1.0 / 479001600.0;
+    p = __builtin_fma(p, r, 1.0 / 39916800.0);
+    p = __builtin_fma(p, r, 1.0 / 3628800.0);
+    p = __builtin_fma(p, r, 1.0 / 362880.0);
+    p = __builtin_fma(p, r, 1.0 / 40320.0);
+    p = __builtin_fma(p, r, 1.0 / 5040.0);
+    p = __builtin_fma(p, r, 1.0 / 720.0);
+    p = __builtin_fma(p, r, 1.0 / 120.0);
+    p = __builtin_fma(p, r, 1.0 / 24.0);
+    p = __builtin_fma(p, r, 1.0 / 6.0);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    return __builtin_ldexp(p, (int)n);
+}
+// 1 / d for normal d: the reciprocal's estimate and two Newton steps
+__device__ __forceinline__ double inverse(double d) {
+    double r = __builtin_amdgcn_rcp(d);
+    r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+    return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+}
+__device__ __forceinline__ float inverse(float d) { return 1.0f / d; }
+// sigmoid; far below 0 (|x| > 700) what is left is 1e-304
+__device__ __forceinline__ double sigmoid_of(double x) { return inverse(1.0 + exp_of(x < -700.0 ? 700.0 : -x)); }
 
 // Bits of the team's scores that are open (in range, not masked, not -inf); *bad: an open one is NaN or +inf
 template <int L, int VPL, typename A>
 __device__ __forceinline__ unsigned open_scores(const RouteDev& a, bool live, int64_t row, int base, const A (&x)[VPL], bool* bad) {
-    unsigned open = 0, wrong = 0;
-    if (live) {
+    unsigned open = 0, wrong = 0, m[VPL];
 #pragma unroll
-        for (int s = 0; s < VPL; ++s) {
-            bool o = base + s < a.E;
-            if (o && a.mask != nullptr) o = a.mask[row * a.ld_mask + base + s] != 0;
-            o = o && !(x[s] == -INFINITY);
-            open |= o ? 1u << s : 0u;
-            wrong |= o && !(x[s] < INFINITY) ? 1u : 0u;
-        }
+    for (int s = 0; s < VPL; ++s) m[s] = 1;
+    if (live && a.mask != nullptr) load_pieces<unsigned char, VPL>(a.mask + row * a.ld_mask, base, a.E, m, 0u);
+#pragma unroll
+    for (int s = 0; s < VPL; ++s) {
+        const bool o = live && base + s < a.E && m[s] != 0 && !(x[s] == -INFINITY);
+        open |= o ? 1u << s : 0u;
+        wrong |= o && !(x[s] < INFINITY) ? 1u : 0u;
     }
-    *bad = lanes_reduce<L>((int)wrong, OpMax()) != 0;
+    *bad = lanes_reduce<L>(wrong, OpMax()) != 0;
     return open;
 }
 
-template <typename T, int L, int VPL, typename KEY>
+template <int KIND> struct Key;
+template <> struct Key<KEY_16> {
+    using type = unsigned;
+    static __device__ __forceinline__ unsigned closed() { return 0u; }
+    static __device__ __forceinline__ bool is_open(unsigned v) { return v != 0u; }
+    static __device__ __forceinline__ unsigned make(float x, int e) {
+        const unsigned b = __builtin_bit_cast(unsigned, x + 0.0f);                  // -0 is 0
+        const unsigned s = b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+        return (s & ~0x1fffu) | (unsigned)(1023 - e);
+    }
+    static __device__ __forceinline__ int expert(unsigned v) { return 1023 - (int)(v & 1023u); }
+};
+template <> struct Key<KEY_TAG> {
+    using type = double;
+    static __device__ __forceinline__ double closed() { return -1.7976931348623157e308; }
+    static __device__ __forceinline__ bool is_open(double v) { return v > -1.79e308; }
+    static __device__ __forceinline__ double make(double x, int e) {
+        const long long b = __builtin_bit_cast(long long, x + 0.0);
+        const long long tag = b < 0 ? e : 1023 - e;                                   // a larger magnitude is a smaller negative number
+        return __builtin_bit_cast(double, (b & ~1023ll) | tag);
+    }
+    static __device__ __forceinline__ int expert(double v) {
+        const long long b = __builtin_bit_cast(long long, v);
+        const int tag = (int)(b & 1023);
+        return b < 0 ? tag : 1023 - tag;
+    }
+};
+
+template <int KIND, int L, int VPL>
 __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
-    using acc = typename Num<T>::acc;
+    using acc = std::conditional_t<KIND == KEY_F64, double, float>;
     constexpr int TEAMS = 64 / L;
     extern __shared__ __align__(16) unsigned char lds[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, team = lane / L, l = lane & (L - 1);
     const int64_t row = ((int64_t)blockIdx.x * 4 + wave) * TEAMS + team;
     const bool live = row < a.n;
     const int base = l * VPL;
-    const size_t sel_bytes = (size_t)4 * TEAMS * a.k * sizeof(int);
-    int* sel = reinterpret_cast<int*>(lds) + (wave * TEAMS + team) * a.k;
-    const T* xrow = static_cast<const T*>(a.scores) + (live ? row : 0) * a.ld;
 
     acc x[VPL];
-    if (live) load_scores<T, VPL>(xrow, base, a.E, x);
-    else {
-#pragma unroll
-        for (int s = 0; s < VPL; ++s) x[s] = 0;
-    }
+    load_scores<VPL>(a, live ? row : a.n - 1, base, x);
     bool bad;
-    const unsigned open = open_scores<L, VPL>(a, live, row, base, x, &bad);
+    unsigned open = open_scores<L, VPL>(a, live, row, base, x, &bad);
 
-    // softmax over the open scores
+    // the softmax's maximum and sum, where something asks for them
+    const bool plain_keys = KIND == KEY_16 || (a.bias == nullptr && !(a.groups > 1 && a.top2));
     acc xmax = -INFINITY;
+    if (!a.sigmoid && (!a.renorm || !plain_keys)) {
 #pragma unroll
-    for (int s = 0; s < VPL; ++s) xmax = open >> s & 1 ? (x[s] > xmax ? x[s] : xmax) : xmax;
-    xmax = lanes_reduce<L>(xmax, OpMax());
-
-    // float keys are made for plain ones only (route_launch)
-    const bool plain_keys = sizeof(KEY) == 4 || (a.bias == nullptr && !(a.groups > 1 && a.top2));
-    KEY v[VPL];
-    if (plain_keys) {
-#pragma unroll
-        for (int s = 0; s < VPL; ++s) v[s] = open >> s & 1 ? (KEY)x[s] : (KEY)-INFINITY;
-    } else {
-        double p[VPL], inv = 1.0;
-        if (a.sigmoid) {
-#pragma unroll
-            for (int s = 0; s < VPL; ++s) p[s] = 1.0 / (1.0 + exp(-(double)x[s]));
-        } else {
-            double z = 0.0;
-#pragma unroll
-            for (int s = 0; s < VPL; ++s) { p[s] = open >> s & 1 ? exp((double)x[s] - (double)xmax) : 0.0; z += p[s]; }
-            z = lanes_reduce<L>(z, OpSum());
-            inv = z;
-        }
-#pragma unroll
-        for (int s = 0; s < VPL; ++s) {
-            double key = p[s] / inv;
-            if (a.bias != nullptr && base + s < a.E)
-                key += a.bias_f64 ? static_cast<const double*>(a.bias)[base + s] : (double)static_cast<const float*>(a.bias)[base + s];
-            v[s] = open >> s & 1 ? (KEY)key : (KEY)-INFINITY;
-        }
+        for (int s = 0; s < VPL; ++s) xmax = open >> s & 1 && x[s] > xmax ? x[s] : xmax;
+        xmax = lanes_reduce<L>(xmax, OpMax());
     }
-
-    if (a.groups > 1) {
-        // the team's keys through LDS: lane l scores the groups l, l + L, ...
-        KEY* keys = reinterpret_cast<KEY*>(lds + ((sel_bytes + 15) & ~(size_t)15)) + (size_t)(wave * TEAMS + team) * (a.E + a.groups);
-        KEY* gs = keys + a.E;
-#pragma unroll
-        for (int s = 0; s < VPL; ++s) if (base + s < a.E) keys[base + s] = v[s];
-        wave_sync();
-        for (int g = l; g < a.groups; g += L) {
-            KEY m1 = -INFINITY, m2 = -INFINITY;
-            for (int i = 0; i < a.group_size; ++i) {
-                const KEY t = keys[g * a.group_size + i];
-                if (t > m1) { m2 = m1; m1 = t; } else if (t > m2) m2 = t;
-            }
-            gs[g] = a.top2 && m2 > -INFINITY ? m1 + m2 : m1;
-        }
-        wave_sync();
-        unsigned long long kept = 0;
-        for (int g = l; g < a.groups; g += L) {
-            const KEY mine = gs[g];
-            int ahead = 0;
-            for (int h = 0; h < a.groups; ++h) { const KEY o = gs[h]; ahead += o > mine || (o == mine && h < g) ? 1 : 0; }
-            if (ahead < a.top_groups) kept |= 1ull << g;
-        }
-#pragma unroll
-        for (int m = 1; m < L; m <<= 1) kept |= __shfl_xor(kept, m, 64);
-        int g = base / a.group_size, r = base - g * a.group_size;
-#pragma unroll
-        for (int s = 0; s < VPL; ++s) {
-            if (g < a.groups && !(kept >> g & 1)) v[s] = -INFINITY;
-            if (++r == a.group_size) { r = 0; ++g; }
-        }
-    }
-
-    for (int j = 0; j < a.k; ++j) {
-        KEY m = -INFINITY;
-#pragma unroll
-        for (int s = 0; s < VPL; ++s) m = v[s] > m ? v[s] : m;
-        m = lanes_reduce<L>(m, OpMax());
-        int at = a.E;
-#pragma unroll
-        for (int s = VPL - 1; s >= 0; --s) at = v[s] == m ? base + s : at;
-        at = lanes_reduce<L>(at, OpMin());
-#pragma unroll
-        for (int s = 0; s < VPL; ++s) v[s] = base + s == at ? (KEY)-INFINITY : v[s];
-        if (l == 0) sel[j] = m > -INFINITY && !bad ? at : -1;
-    }
-    wave_sync();
-
-    // weights of the chosen, in acc (the sums of a sigmoid's renormalisation in 64 bits: all of them may be far below 1)
     acc z = 0;
     if (!a.sigmoid && !a.renorm) {
 #pragma unroll
-        for (int s = 0; s < VPL; ++s) z += open >> s & 1 ? exp(x[s] - xmax) : (acc)0;
+        for (int s = 0; s < VPL; ++s) z += open >> s & 1 ? exp_of(x[s] - xmax) : (acc)0;
         z = lanes_reduce<L>(z, OpSum());
     }
-    double top = -INFINITY, sum = 0.0;
-    if (a.renorm) {
-        for (int j = l; j < a.k; j += L) if (sel[j] >= 0) {
-            const double xe = (double)(acc)xrow[sel[j]], t = a.sigmoid ? log_sigmoid(xe) : xe;
-            top = t > top ? t : top;
+
+    // clean keys: what groups are ranked by
+    using clean = std::conditional_t<KIND == KEY_16, float, double>;
+    clean v[VPL];
+    if (KIND == KEY_16 || plain_keys) {
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) v[s] = open >> s & 1 ? (clean)x[s] : (clean)-INFINITY;
+    } else {
+        if (a.sigmoid) {
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) v[s] = (clean)sigmoid_of((double)x[s]);
+        } else {
+            double zz = 0.0;
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) { v[s] = (clean)(open >> s & 1 ? exp_of((double)x[s] - (double)xmax) : 0.0); zz += v[s]; }
+            const double inv = inverse(lanes_reduce<L>(zz, OpSum()));
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) v[s] = (clean)(v[s] * inv);
         }
-        top = lanes_reduce<L>(top, OpMax());
-        for (int j = l; j < a.k; j += L) if (sel[j] >= 0) {
-            const double xe = (double)(acc)xrow[sel[j]], t = a.sigmoid ? log_sigmoid(xe) : xe;
-            sum += exp(t - top);
+        if (a.bias != nullptr) {
+            double b[VPL];
+            if (a.bias_f64) load_pieces<double, VPL>(static_cast<const double*>(a.bias), base, a.E, b, 0.0);
+            else load_pieces<float, VPL>(static_cast<const float*>(a.bias), base, a.E, b, 0.0);
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) v[s] += (clean)b[s];
         }
-        sum = lanes_reduce<L>(sum, OpSum());
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) v[s] = open >> s & 1 ? v[s] : (clean)-INFINITY;
     }
-    if (!live) return;
-    for (int j = l; j < a.k; j += L) {
-        const int e = sel[j];
-        a.experts[row * a.k + j] = e;
-        acc w = 0;
-        if (bad) w = NAN;
-        else if (e >= 0) {
-            const acc xe = (acc)xrow[e];
-            if (a.renorm) w = (acc)(a.scale * (exp((a.sigmoid ? log_sigmoid((double)xe) : (double)xe) - top) / sum));
-            else if (a.sigmoid) w = (acc)(a.scale / (1.0 + exp(-(double)xe)));
-            else w = (acc)a.scale * (exp(xe - xmax) / z);
+
+    if (a.groups > 1) {
+        clean* gs = reinterpret_cast<clean*>(lds) + (size_t)(wave * TEAMS + team) * (a.lanes_per_group ? a.groups : a.E + a.groups);
+        if (a.lanes_per_group) {
+            // a group is the whole of lanes_per_group neighbouring lanes: its two best by lane, then across them
+            clean m1 = -INFINITY, m2 = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) {
+                const clean low = v[s] < m1 ? v[s] : m1;
+                m2 = low > m2 ? low : m2;
+                m1 = v[s] > m1 ? v[s] : m1;
+            }
+            auto join = [&](auto mc) {
+                constexpr int M = decltype(mc)::value;
+                if constexpr (M < L) {
+                    if (M < a.lanes_per_group) {
+                        const clean o1 = lane_swap<M>(m1), o2 = lane_swap<M>(m2);
+                        const clean low = o1 < m1 ? o1 : m1;
+                        m2 = m2 > o2 ? m2 : o2;
+                        m2 = low > m2 ? low : m2;
+                        m1 = o1 > m1 ? o1 : m1;
+                    }
+                }
+            };
+            join(std::integral_constant<int, 1>()); join(std::integral_constant<int, 2>()); join(std::integral_constant<int, 4>());
+            join(std::integral_constant<int, 8>()); join(std::integral_constant<int, 16>()); join(std::integral_constant<int, 32>());
+            const int g = l / a.lanes_per_group;
+            const clean mine = a.top2 && m2 > -INFINITY ? m1 + m2 : m1;
+            if (g < a.groups) gs[g] = mine;
+            wave_sync();
+            int ahead = 0;
+            for (int h = 0; h < a.groups; ++h) { const clean o = gs[h]; ahead += o > mine || (o == mine && h < g) ? 1 : 0; }
+            if (ahead >= a.top_groups) open = 0;
+        } else {
+            // any other size: the team's keys through LDS, lane l scores the groups l, l + L, ...
+            clean* keys = gs + a.groups;
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) if (base + s < a.E) keys[base + s] = v[s];
+            wave_sync();
+            for (int g = l; g < a.groups; g += L) {
+                clean m1 = -INFINITY, m2 = -INFINITY;
+                for (int i = 0; i < a.group_size; ++i) {
+                    const clean t = keys[g * a.group_size + i];
+                    if (t > m1) { m2 = m1; m1 = t; } else if (t > m2) m2 = t;
+                }
+                gs[g] = a.top2 && m2 > -INFINITY ? m1 + m2 : m1;
+            }
+            wave_sync();
+            unsigned long long kept = 0;
+            for (int g = l; g < a.groups; g += L) {
+                const clean mine = gs[g];
+                int ahead = 0;
+                for (int h = 0; h < a.groups; ++h) { const clean o = gs[h]; ahead += o > mine || (o == mine && h < g) ? 1 : 0; }
+                if (ahead < a.top_groups) kept |= 1ull << g;
+            }
+            kept = lanes_reduce<L>(kept, OpOr());
+            int g = base / a.group_size, r = base - g * a.group_size;
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) {
+                if (g < a.groups && !(kept >> g & 1)) open &= ~(1u << s);
+                if (++r == a.group_size) { r = 0; ++g; }
+            }
         }
-        static_cast<acc*>(a.weights)[row * a.k + j] = w;
+    }
+
+    // the k best; lane j of the team keeps the j-th
+    int mine = -1;
+    if constexpr (KIND == KEY_F64) {
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) v[s] = open >> s & 1 ? v[s] : -INFINITY;
+        for (int j = 0; j < a.k; ++j) {
+            double m = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) m = v[s] > m ? v[s] : m;
+            m = lanes_reduce<L>(m, OpMax());
+            int at = a.E;
+#pragma unroll
+            for (int s = VPL - 1; s >= 0; --s) at = v[s] == m ? base + s : at;
+            at = lanes_reduce<L>(at, OpMin());
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) v[s] = base + s == at ? -INFINITY : v[s];
+            if (l == j) mine = m > -INFINITY ? at : -1;
+        }
+    } else {
+        using K = Key<KIND>;
+        typename K::type key[VPL];
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) key[s] = open >> s & 1 ? K::make(v[s], base + s) : K::closed();
+        for (int j = 0; j < a.k; ++j) {
+            typename K::type m = key[0];
+#pragma unroll
+            for (int s = 1; s < VPL; ++s) m = OpMax()(m, key[s]);
+            m = lanes_reduce<L>(m, OpMax());
+#pragma unroll
+            for (int s = 0; s < VPL; ++s) key[s] = key[s] == m ? K::closed() : key[s];
+            if (l == j) mine = K::is_open(m) ? K::expert(m) : -1;
+        }
+    }
+    if (bad) mine = -1;
+
+    // weights: one slot a lane, in 64 bits except for the plain softmax (a sigmoid's sum may be far below 1)
+    const bool chosen = mine >= 0 && l < a.k;
+    acc w = 0;
+    const double xe = chosen ? (double)score_at<acc>(a, row, mine) : 0.0;
+    if (a.renorm) {
+        double top = chosen ? xe : -INFINITY;
+        top = lanes_reduce<L>(top, OpMax());
+        // below -40 a sigmoid is the exponential to 2^-57
+        double p = 0.0;
+        if (chosen) p = a.sigmoid && top > -40.0 ? sigmoid_of(xe) : exp_of(xe - top);
+        const double sum = lanes_reduce<L>(p, OpSum());
+        if (chosen) w = (acc)(a.scale * p * inverse(sum));
+    } else if (chosen) {
+        w = a.sigmoid ? (acc)(a.scale * (xe < -700.0 ? exp_of(xe) : sigmoid_of(xe))) : (acc)a.scale * (exp_of((acc)xe - xmax) / z);
+    }
+    if (live && l < a.k) {
+        a.experts[row * a.k + l] = mine;
+        static_cast<acc*>(a.weights)[row * a.k + l] = bad ? (acc)NAN : w;
     }
 }
 
@@ -209,102 +326,108 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
 //   softmax, renorm  r_i (g_i - sum_j r_j g_j)                    sigmoid, renorm  r_i (g_i - sum_j r_j g_j)(1 - p_i)
 // Only the first is dense; the chosen ones' terms go through an LDS row so that every row leaves in one coalesced piece.
 // A row without experts has gradient zero.
-template <typename T, int L, int VPL>
+template <typename A, int VPL, typename T> __device__ __forceinline__ void store_pieces(T* p, int base, int E, const A (&x)[VPL]) {
+    typedef T four __attribute__((ext_vector_type(4)));
+    typedef four four_at __attribute__((aligned(sizeof(T))));
+#pragma unroll
+    for (int c = 0; c < VPL; c += 4) {
+        if (base + c + 4 <= E) {
+            four b;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = (T)x[c + i];
+            *reinterpret_cast<four_at*>(p + base + c) = b;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (base + c + i < E) p[base + c + i] = (T)x[c + i];
+        }
+    }
+}
+
+template <typename acc, int L, int VPL>
 __global__ void __launch_bounds__(256) route_grad_kernel(RouteDev a) {
-    using acc = typename Num<T>::acc;
     constexpr int TEAMS = 64 / L;
     extern __shared__ __align__(16) unsigned char lds[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, team = lane / L, l = lane & (L - 1);
     const int64_t row = ((int64_t)blockIdx.x * 4 + wave) * TEAMS + team;
     const bool live = row < a.n;
+    const int64_t at = live ? row : a.n - 1;
     const int base = l * VPL;
-    acc* buf = reinterpret_cast<acc*>(lds) + (size_t)(wave * TEAMS + team) * a.E;
-    const T* xrow = static_cast<const T*>(a.scores) + (live ? row : 0) * a.ld;
-    const int* sel = a.experts + (live ? row : 0) * a.k;
-    const acc* dw = static_cast<const acc*>(a.dweights) + (live ? row : 0) * a.k;
+    acc* buf = reinterpret_cast<acc*>(lds) + (size_t)(wave * TEAMS + team) * (L * VPL);
     const bool dense = !a.sigmoid && !a.renorm;
 
-    acc x[VPL], xmax = -INFINITY, z = 0;
-    unsigned open = 0;
+    // this lane's slot (L >= k)
+    const int e = l < a.k ? a.experts[at * a.k + l] : -1;
+    const bool chosen = e >= 0 && e < a.E;
+    const acc xe = chosen ? score_at<acc>(a, at, e) : (acc)0;
+    const acc g = chosen ? (acc)a.scale * static_cast<const acc*>(a.dweights)[at * a.k + l] : (acc)0;
+
+    acc x[VPL], xmax = -INFINITY, inv = 0;
     if (dense) {
-        if (live) load_scores<T, VPL>(xrow, base, a.E, x);
-        else {
-#pragma unroll
-            for (int s = 0; s < VPL; ++s) x[s] = 0;
-        }
+        load_scores<VPL>(a, at, base, x);
         bool bad;
-        open = open_scores<L, VPL>(a, live, row, base, x, &bad);
+        const unsigned open = open_scores<L, VPL>(a, live, row, base, x, &bad);
 #pragma unroll
-        for (int s = 0; s < VPL; ++s) xmax = open >> s & 1 ? (x[s] > xmax ? x[s] : xmax) : xmax;
+        for (int s = 0; s < VPL; ++s) xmax = open >> s & 1 && x[s] > xmax ? x[s] : xmax;
         xmax = lanes_reduce<L>(xmax, OpMax());
+        acc z = 0;
 #pragma unroll
-        for (int s = 0; s < VPL; ++s) { x[s] = open >> s & 1 ? exp(x[s] - xmax) : (acc)0; z += x[s]; }
-        z = lanes_reduce<L>(z, OpSum());
+        for (int s = 0; s < VPL; ++s) { x[s] = open >> s & 1 ? exp_of(x[s] - xmax) : (acc)0; z += x[s]; }
+        inv = inverse(lanes_reduce<L>(z, OpSum()));
+    } else {
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) x[s] = 0;
+        xmax = lanes_reduce<L>(chosen ? xe : (acc)-INFINITY, OpMax());
     }
 #pragma unroll
-    for (int s = 0; s < VPL; ++s) if (base + s < a.E) buf[base + s] = 0;
+    for (int s = 0; s < VPL; ++s) buf[base + s] = 0;
     wave_sync();
 
-    double top = -INFINITY, sum = 0.0, dot = 0.0;
-    int some = 0;
-    if (live) {
-        for (int j = l; j < a.k; j += L) {
-            const int e = sel[j];
-            if (e < 0 || e >= a.E) continue;
-            some = 1;
-            const double xe = (double)(acc)xrow[e], t = a.sigmoid ? log_sigmoid(xe) : xe;
-            top = t > top ? t : top;
+    acc r = 0;
+    const acc p = inverse((acc)1 + exp_of(-xe)), not_p = inverse((acc)1 + exp_of(xe));     // sigmoid and 1 - sigmoid, each to its own size
+    if (chosen) r = a.sigmoid && (!a.renorm || xmax > (acc)-40) ? p : exp_of(xe - xmax);
+    if (dense) r *= inv;
+    else if (a.renorm) r *= inverse(lanes_reduce<L>(r, OpSum()));
+    const acc dot = lanes_reduce<L>(r * g, OpSum());
+    const bool some = lanes_reduce<L>(chosen ? 1u : 0u, OpMax()) != 0;
+    if (chosen) {
+        acc d = g;
+        if (!dense) {
+            d = a.renorm ? r * (g - dot) : r * g;
+            if (a.sigmoid) d *= not_p;
         }
-    }
-    top = lanes_reduce<L>(top, OpMax());
-    some = lanes_reduce<L>(some, OpMax());
-    if (live && (a.renorm || dense)) {
-        for (int j = l; j < a.k; j += L) {
-            const int e = sel[j];
-            if (e < 0 || e >= a.E) continue;
-            const double xe = (double)(acc)xrow[e], g = a.scale * (double)dw[j];
-            const double r = dense ? exp(xe - (double)xmax) / (double)z : exp((a.sigmoid ? log_sigmoid(xe) : xe) - top);
-            sum += r; dot += r * g;
-        }
-    }
-    sum = lanes_reduce<L>(sum, OpSum());
-    dot = lanes_reduce<L>(dot, OpSum());
-    if (live) {
-        for (int j = l; j < a.k; j += L) {
-            const int e = sel[j];
-            if (e < 0 || e >= a.E) continue;
-            const double xe = (double)(acc)xrow[e], g = a.scale * (double)dw[j];
-            double d;
-            if (dense) d = g;
-            else if (a.renorm) {
-                d = exp((a.sigmoid ? log_sigmoid(xe) : xe) - top) / sum * (g - dot / sum);
-                if (a.sigmoid) d *= 1.0 / (1.0 + exp(xe));
-            } else d = g / (1.0 + exp(-xe)) / (1.0 + exp(xe));
-            atomicAdd(&buf[e], (acc)d);
-        }
+        atomicAdd(&buf[e], d);
     }
     wave_sync();
-    if (!live) return;
-    T* out = static_cast<T*>(a.dscores) + row * a.ld_out;
+    acc out[VPL];
 #pragma unroll
     for (int s = 0; s < VPL; ++s) {
-        if (base + s >= a.E) break;
-        acc d = buf[base + s];
-        if (dense) d = some ? x[s] / z * (d - (acc)dot) : (acc)0;
-        out[base + s] = (T)d;
+        const acc d = buf[base + s];
+        out[s] = dense ? (some ? x[s] * inv * (d - dot) : (acc)0) : d;
     }
+    if (!live) return;
+    if constexpr (sizeof(acc) == 8) store_pieces<acc, VPL>(static_cast<double*>(a.dscores) + row * a.ld_out, base, a.E, out);
+    else if (a.dtype == OAK_BF16) store_pieces<acc, VPL>(static_cast<__bf16*>(a.dscores) + row * a.ld_out, base, a.E, out);
+    else if (a.dtype == OAK_F16) store_pieces<acc, VPL>(static_cast<_Float16*>(a.dscores) + row * a.ld_out, base, a.E, out);
+    else store_pieces<acc, VPL>(static_cast<float*>(a.dscores) + row * a.ld_out, base, a.E, out);
 }
 
-// lanes per row and scores per lane: the fewest lanes that hold a row with at most 16 scores each, so that the steps across lanes,
-// which a row of a team pays k times, are few
-template <typename F> static int with_team(int E, F&& fn) {
-    if (E <= 16) return fn(std::integral_constant<int, 4>(), std::integral_constant<int, 4>());
-    if (E <= 32) return fn(std::integral_constant<int, 4>(), std::integral_constant<int, 8>());
-    if (E <= 64) return fn(std::integral_constant<int, 4>(), std::integral_constant<int, 16>());
-    if (E <= 128) return fn(std::integral_constant<int, 8>(), std::integral_constant<int, 16>());
-    if (E <= 256) return fn(std::integral_constant<int, 16>(), std::integral_constant<int, 16>());
-    if (E <= 512) return fn(std::integral_constant<int, 32>(), std::integral_constant<int, 16>());
-    return fn(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
+// Lanes of a team and scores a lane: the fewest lanes that hold the row with at most 16 scores each -- the steps across lanes, which
+// a row pays k times, are few, and a wave serves many rows -- but at least k, so that every slot has a lane.
+template <typename F> static int with_team(int E, int k, F&& fn) {
+    auto by_vpl = [&](auto lc) {
+        constexpr int L = decltype(lc)::value;
+        const int per = (E + L - 1) / L;
+        if (per <= 4) return fn(lc, std::integral_constant<int, 4>());
+        if (per <= 8) return fn(lc, std::integral_constant<int, 8>());
+        if (per <= 12) return fn(lc, std::integral_constant<int, 12>());
+        return fn(lc, std::integral_constant<int, 16>());
+    };
+    const int need = (E + 15) / 16 > k ? (E + 15) / 16 : k;
+    if (need <= 4) return by_vpl(std::integral_constant<int, 4>());
+    if (need <= 8) return by_vpl(std::integral_constant<int, 8>());
+    if (need <= 16) return by_vpl(std::integral_constant<int, 16>());
+    if (need <= 32) return by_vpl(std::integral_constant<int, 32>());
+    return by_vpl(std::integral_constant<int, 64>());
 }
 
 static int route_check(const oak_route_args* a) {
@@ -331,7 +454,7 @@ static RouteDev route_dev(const oak_route_args* a) {
     RouteDev d{};
     d.n = a->n_rows; d.ld = a->ld_scores; d.ld_mask = a->ld_mask; d.ld_out = a->ld_dscores;
     d.E = a->n_experts; d.k = a->top_k; d.groups = a->n_groups; d.top_groups = a->top_groups; d.group_size = a->n_experts / a->n_groups;
-    d.sigmoid = a->score == OAK_SCORE_SIGMOID; d.top2 = a->group_score == OAK_GROUP_TOP2; d.renorm = a->renormalise != 0; d.bias_f64 = a->bias_f64;
+    d.sigmoid = a->score == OAK_SCORE_SIGMOID; d.top2 = a->group_score == OAK_GROUP_TOP2; d.dtype = a->dtype; d.renorm = a->renormalise != 0; d.bias_f64 = a->bias_f64;
     d.scale = a->scale; d.scores = a->scores; d.bias = a->bias; d.mask = a->mask; d.experts = a->experts; d.weights = a->weights;
     d.dweights = a->dweights; d.dscores = a->dscores;
     return d;
@@ -339,38 +462,38 @@ static RouteDev route_dev(const oak_route_args* a) {
 
 static int route_launch(hipStream_t stream, const oak_route_args* a) {
     if (a->n_rows == 0) return OAK_OK;
-    const RouteDev d = route_dev(a);
+    RouteDev d = route_dev(a);
     const bool plain_keys = d.bias == nullptr && !(d.groups > 1 && d.top2);
-    return with_dtype(a->dtype, [&](auto t) {
-        using T = decltype(t);
-        return with_team(d.E, [&](auto lc, auto vc) {
-            constexpr int L = decltype(lc)::value, VPL = decltype(vc)::value, TEAMS = 64 / L;
-            const dim3 grid((unsigned)((d.n + 4 * TEAMS - 1) / (4 * TEAMS)));
-            const size_t sel = ((size_t)4 * TEAMS * d.k * sizeof(int) + 15) & ~(size_t)15;
-            auto go = [&](auto key) {
-                using KEY = decltype(key);
-                const size_t lds = sel + (d.groups > 1 ? (size_t)4 * TEAMS * (d.E + d.groups) * sizeof(KEY) : 0);
-                auto kernel = route_kernel<T, L, VPL, KEY>;
-                if (lds > 64 * 1024) OAK_CHECK(ensure_dynamic_lds((const void*)kernel, 160 * 1024));
-                return launch(kernel, grid, dim3(256), lds, stream, d);
-            };
-            if constexpr (sizeof(T) < 8) { if (plain_keys) return go((float)0); }
-            return go((double)0);
-        });
+    return with_team(d.E, d.k, [&](auto lc, auto vc) {
+        constexpr int L = decltype(lc)::value, VPL = decltype(vc)::value, TEAMS = 64 / L;
+        const dim3 grid((unsigned)((d.n + 4 * TEAMS - 1) / (4 * TEAMS)));
+        // groups that are whole lanes, a power of two of them, are scored without LDS
+        const int lanes = d.group_size % VPL == 0 ? d.group_size / VPL : 0;
+        d.lanes_per_group = lanes > 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+        const size_t lds = d.groups > 1 ? (size_t)4 * TEAMS * (d.lanes_per_group ? d.groups : d.E + d.groups) * sizeof(double) : 0;
+        auto go = [&](auto kind) {
+            auto kernel = route_kernel<decltype(kind)::value, L, VPL>;
+            if (lds > 64 * 1024) OAK_CHECK(ensure_dynamic_lds((const void*)kernel, 160 * 1024));
+            return launch(kernel, grid, dim3(256), lds, stream, d);
+        };
+        if (d.dtype == OAK_F64) return go(std::integral_constant<int, KEY_F64>());
+        if (d.dtype != OAK_F32 && plain_keys) return go(std::integral_constant<int, KEY_16>());
+        return go(std::integral_constant<int, KEY_TAG>());
     });
 }
 
 static int route_grad_launch(hipStream_t stream, const oak_route_args* a) {
     if (a->n_rows == 0) return OAK_OK;
     const RouteDev d = route_dev(a);
-    return with_dtype(a->dtype, [&](auto t) {
-        using T = decltype(t);
-        return with_team(d.E, [&](auto lc, auto vc) {
-            constexpr int L = decltype(lc)::value, VPL = decltype(vc)::value, TEAMS = 64 / L;
-            const dim3 grid((unsigned)((d.n + 4 * TEAMS - 1) / (4 * TEAMS)));
-            const size_t lds = (size_t)4 * TEAMS * d.E * sizeof(typename Num<T>::acc);
-            return launch(route_grad_kernel<T, L, VPL>, grid, dim3(256), lds, stream, d);
-        });
+    return with_team(d.E, d.k, [&](auto lc, auto vc) {
+        constexpr int L = decltype(lc)::value, VPL = decltype(vc)::value, TEAMS = 64 / L;
+        const dim3 grid((unsigned)((d.n + 4 * TEAMS - 1) / (4 * TEAMS)));
+        auto go = [&](auto zero) {
+            using acc = decltype(zero);
+            const size_t lds = (size_t)4 * TEAMS * L * VPL * sizeof(acc);
+            return launch(route_grad_kernel<acc, L, VPL>, grid, dim3(256), lds, stream, d);
+        };
+        return d.dtype == OAK_F64 ? go((double)0) : go((float)0);
     });
 }
 

@@ -49,12 +49,43 @@ __device__ __forceinline__ double load_any(const void* p, int dtype, int64_t i) 
 
 // ---- reductions over L consecutive lanes (L a power of two up to 64); every lane gets the result --------------------------
 struct OpMax { template <typename A> __device__ __forceinline__ A operator()(A a, A b) const { return a > b ? a : b; } };
+template <> __device__ __forceinline__ double OpMax::operator()(double a, double b) const { return __builtin_fmax(a, b); }
+template <> __device__ __forceinline__ float OpMax::operator()(float a, float b) const { return __builtin_fmaxf(a, b); }
 struct OpMin { template <typename A> __device__ __forceinline__ A operator()(A a, A b) const { return a < b ? a : b; } };
 struct OpSum { template <typename A> __device__ __forceinline__ A operator()(A a, A b) const { return a + b; } };
+struct OpOr { template <typename A> __device__ __forceinline__ A operator()(A a, A b) const { return a | b; } };
+
+// The value of a lane in the other half of the block of 2 M lanes, M a constant power of two.  Within 16 lanes by a data-parallel
+// move (a mirror of the block for M = 4 and 8: WHICH lane of the other half does not matter to a reduction that has already made
+// each half agree), across rows of 16 and 32 by the row swaps -- none of it goes through LDS as a shuffle by index would.
+template <int M> __device__ __forceinline__ unsigned lane_swap32(unsigned v) {
+    if constexpr (M == 1) return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true);        // quad_perm 1 0 3 2
+    else if constexpr (M == 2) return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+    else if constexpr (M == 4) return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true);  // row_half_mirror
+    else if constexpr (M == 8) return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true);  // row_mirror
+    else {
+        // both operands v: the first result holds the even rows (halves) twice, the second the odd ones
+        const auto r = M == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        const unsigned lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+        return lane & M ? r[0] : r[1];
+    }
+}
+template <int M, typename A> __device__ __forceinline__ A lane_swap(A v) {
+    static_assert(sizeof(A) == 4 || sizeof(A) == 8, "32- and 64-bit values");
+    if constexpr (sizeof(A) == 4) return __builtin_bit_cast(A, lane_swap32<M>(__builtin_bit_cast(unsigned, v)));
+    else {
+        const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+        return __builtin_bit_cast(A, (unsigned long long)lane_swap32<M>((unsigned)(b >> 32)) << 32 | lane_swap32<M>((unsigned)b));
+    }
+}
 
 template <int L, typename Op, typename A> __device__ __forceinline__ A lanes_reduce(A v, Op op) {
-#pragma unroll
-    for (int m = 1; m < L; m <<= 1) v = op(v, __shfl_xor(v, m, 64));
+    if constexpr (L > 1) v = op(v, lane_swap<1>(v));
+    if constexpr (L > 2) v = op(v, lane_swap<2>(v));
+    if constexpr (L > 4) v = op(v, lane_swap<4>(v));
+    if constexpr (L > 8) v = op(v, lane_swap<8>(v));
+    if constexpr (L > 16) v = op(v, lane_swap<16>(v));
+    if constexpr (L > 32) v = op(v, lane_swap<32>(v));
     return v;
 }
 
