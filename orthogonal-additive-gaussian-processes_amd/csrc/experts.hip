@@ -14,19 +14,20 @@ namespace oak {
 // route
 // ---------------------------------------------------------------------------------------------------------------------
 // A row belongs to a team of L lanes; lane l of the team holds the experts [l VPL, (l + 1) VPL) in registers, so that the row is read
-// once, in pieces of VPL consecutive scores.  The k best are taken one after the other: the largest key of the team, then that one is
-// struck out; lane j keeps the j-th (L >= k).
+// once, in pieces of VPL consecutive scores; a closed score is -inf from there on.  The k best are taken one after the other, lane j of
+// the team keeps the j-th (L >= k).
 //
 // Keys.  Where nothing is added to the scores the keys are the scores themselves: softmax and sigmoid keep their order, and no rounding
 // can tie what differs.  With a bias, or group scores that add two probabilities, the keys are probabilities in 64 bits: scores next to
 // each other differ by less than the rounding of 32 bits often enough to matter (a few rows in ten thousand).
 // A key carries its expert in its last bits, in the order that makes the larger key the lower expert, so that one maximum finds
 // both and ties resolve themselves:
-//   KEY_16   16-bit scores: a 32-bit integer, the score's bits in ascending order over 13 bits that no such score uses -- one instruction a step
-//   KEY_TAG  float scores and probabilities: a double whose last 10 of 52 bits are the tag (float scores do not reach them;
-//            probabilities closer than 2^-42 of their size count as tied)
+//   KEY_16   16-bit scores: a 31-bit integer, the score's bits in ascending order over 12 bits that no such score uses.  The next best after m
+//            is the largest of key - m modulo 2^32: what is below m wraps to the upper half, and nothing has to be struck out
+//   KEY_TAG  float scores and probabilities: a double whose last 11 of 52 bits are the tag (float scores do not reach them;
+//            probabilities closer than 2^-41 of their size count as tied)
 //   KEY_F64  double scores: all bits belong to the key, the expert is found in a second step
-// Bound by instruction issue (16384 x 256 bf16, sigmoid + bias, 4 of 8 groups, k = 8: 38 us before, see the table of measured times), not by memory.
+// Bound by the issue of vector instructions, 4 cycles each (counted: 0.9 of the time), not by memory.
 enum { KEY_16 = 0, KEY_TAG = 1, KEY_F64 = 2 };
 
 struct RouteDev {
@@ -56,12 +57,12 @@ template <typename T, int VPL, typename A> __device__ __forceinline__ void load_
 }
 // the lane's piece of a row of scores; the element type is a uniform branch: one kernel serves all of a kind
 template <int VPL> __device__ __forceinline__ void load_scores(const RouteDev& a, int64_t row, int base, float (&x)[VPL]) {
-    if (a.dtype == OAK_BF16) load_pieces<__bf16, VPL>(static_cast<const __bf16*>(a.scores) + row * a.ld, base, a.E, x, 0.0f);
-    else if (a.dtype == OAK_F16) load_pieces<_Float16, VPL>(static_cast<const _Float16*>(a.scores) + row * a.ld, base, a.E, x, 0.0f);
-    else load_pieces<float, VPL>(static_cast<const float*>(a.scores) + row * a.ld, base, a.E, x, 0.0f);
+    if (a.dtype == OAK_BF16) load_pieces<__bf16, VPL>(static_cast<const __bf16*>(a.scores) + row * a.ld, base, a.E, x, -INFINITY);
+    else if (a.dtype == OAK_F16) load_pieces<_Float16, VPL>(static_cast<const _Float16*>(a.scores) + row * a.ld, base, a.E, x, -INFINITY);
+    else load_pieces<float, VPL>(static_cast<const float*>(a.scores) + row * a.ld, base, a.E, x, -INFINITY);
 }
 template <int VPL> __device__ __forceinline__ void load_scores(const RouteDev& a, int64_t row, int base, double (&x)[VPL]) {
-    load_pieces<double, VPL>(static_cast<const double*>(a.scores) + row * a.ld, base, a.E, x, 0.0);
+    load_pieces<double, VPL>(static_cast<const double*>(a.scores) + row * a.ld, base, a.E, x, (double)-INFINITY);
 }
 template <typename A> __device__ __forceinline__ A score_at(const RouteDev& a, int64_t row, int e) { return (A)load_any(a.scores, a.dtype, row * a.ld + e); }
 
@@ -97,50 +98,54 @@ __device__ __forceinline__ float inverse(float d) { return 1.0f / d; }
 // sigmoid; far below 0 (|x| > 700) what is left is 1e-304
 __device__ __forceinline__ double sigmoid_of(double x) { return inverse(1.0 + exp_of(x < -700.0 ? 700.0 : -x)); }
 
-// Bits of the team's scores that are open (in range, not masked, not -inf); *bad: an open one is NaN or +inf
-template <int L, int VPL, typename A>
-__device__ __forceinline__ unsigned open_scores(const RouteDev& a, bool live, int64_t row, int base, const A (&x)[VPL], bool* bad) {
-    unsigned open = 0, wrong = 0, m[VPL];
+// closes the masked scores (-inf); true if an open one is NaN or +inf
+template <int L, int VPL, typename A> __device__ __forceinline__ bool close_scores(const RouteDev& a, int64_t row, int base, A (&x)[VPL]) {
+    if (a.mask != nullptr) {
+        unsigned m[VPL];
+        load_pieces<unsigned char, VPL>(a.mask + row * a.ld_mask, base, a.E, m, 0u);
 #pragma unroll
-    for (int s = 0; s < VPL; ++s) m[s] = 1;
-    if (live && a.mask != nullptr) load_pieces<unsigned char, VPL>(a.mask + row * a.ld_mask, base, a.E, m, 0u);
-#pragma unroll
-    for (int s = 0; s < VPL; ++s) {
-        const bool o = live && base + s < a.E && m[s] != 0 && !(x[s] == -INFINITY);
-        open |= o ? 1u << s : 0u;
-        wrong |= o && !(x[s] < INFINITY) ? 1u : 0u;
+        for (int s = 0; s < VPL; ++s) x[s] = m[s] != 0 ? x[s] : (A)-INFINITY;
     }
-    *bad = lanes_reduce<L>(wrong, OpMax()) != 0;
-    return open;
+    bool wrong = false;
+#pragma unroll
+    for (int s = 0; s < VPL; ++s) wrong |= !(x[s] < (A)INFINITY);
+    return lanes_reduce<L>(wrong ? 1u : 0u, OpOr()) != 0;
 }
 
-template <int KIND> struct Key;
-template <> struct Key<KEY_16> {
-    using type = unsigned;
-    static __device__ __forceinline__ unsigned closed() { return 0u; }
-    static __device__ __forceinline__ bool is_open(unsigned v) { return v != 0u; }
-    static __device__ __forceinline__ unsigned make(float x, int e) {
-        const unsigned b = __builtin_bit_cast(unsigned, x + 0.0f);                  // -0 is 0
-        const unsigned s = b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
-        return (s & ~0x1fffu) | (unsigned)(1023 - e);
-    }
-    static __device__ __forceinline__ int expert(unsigned v) { return 1023 - (int)(v & 1023u); }
-};
-template <> struct Key<KEY_TAG> {
-    using type = double;
-    static __device__ __forceinline__ double closed() { return -1.7976931348623157e308; }
-    static __device__ __forceinline__ bool is_open(double v) { return v > -1.79e308; }
-    static __device__ __forceinline__ double make(double x, int e) {
-        const long long b = __builtin_bit_cast(long long, x + 0.0);
-        const long long tag = b < 0 ? e : 1023 - e;                                   // a larger magnitude is a smaller negative number
-        return __builtin_bit_cast(double, (b & ~1023ll) | tag);
-    }
-    static __device__ __forceinline__ int expert(double v) {
-        const long long b = __builtin_bit_cast(long long, v);
-        const int tag = (int)(b & 1023);
-        return b < 0 ? tag : 1023 - tag;
-    }
-};
+// expert l VPL + s <-> tag: larger for lower experts
+constexpr unsigned TAG_BITS = 2047;
+__device__ __forceinline__ unsigned lane_tag(int l) { return (unsigned)(63 - l) << 5; }
+template <int VPL> __device__ __forceinline__ int expert_of(unsigned tag) { return (63 - (int)(tag >> 5)) * VPL + 31 - (int)(tag & 31); }
+
+// 16-bit scores
+__device__ __forceinline__ unsigned key16(float x, unsigned lane, int s) {
+    const unsigned b = __builtin_bit_cast(unsigned, x + 0.0f);                          // -0 is 0
+    const unsigned up = (b ^ ((unsigned)((int)b >> 31) | 0x80000000u)) >> 1;
+    return (up & ~0xfffu) | lane | (unsigned)(31 - s);
+}
+constexpr unsigned KEY16_OPEN = 0x00800000u >> 1;                                       // the lowest finite score; -inf is below
+__device__ __forceinline__ float key16_score(unsigned key) {
+    const unsigned up = (key & ~0xfffu) << 1;
+    return __builtin_bit_cast(float, up & 0x80000000u ? up ^ 0x80000000u : ~(up | 0x1fffu));
+}
+
+// float scores and probabilities; closed and struck keys have the high word of the lowest double
+constexpr unsigned CLOSED_HI = 0xffefffffu;
+constexpr double CLOSED_BELOW = -1.79e308;
+__device__ __forceinline__ double with_hi(double v, unsigned hi) {
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | (unsigned)__builtin_bit_cast(unsigned long long, v));
+}
+__device__ __forceinline__ unsigned hi_of(double v) { return (unsigned)(__builtin_bit_cast(unsigned long long, v) >> 32); }
+__device__ __forceinline__ double key_tagged(double x, unsigned lane, int s) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, x + 0.0);
+    const unsigned sign = (unsigned)((int)(unsigned)(b >> 32) >> 31);                   // a larger magnitude is a smaller negative number
+    const unsigned lo = ((unsigned)b & ~TAG_BITS) | ((lane | (unsigned)(31 - s)) ^ (sign & TAG_BITS));
+    return __builtin_bit_cast(double, b >> 32 << 32 | lo);
+}
+__device__ __forceinline__ unsigned tag_of(double v) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+    return ((unsigned)b ^ (unsigned)((int)(unsigned)(b >> 32) >> 31)) & TAG_BITS;
+}
 
 template <int KIND, int L, int VPL>
 __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
@@ -148,91 +153,92 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
     constexpr int TEAMS = 64 / L;
     extern __shared__ __align__(16) unsigned char lds[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, team = lane / L, l = lane & (L - 1);
-    const int64_t row = ((int64_t)blockIdx.x * 4 + wave) * TEAMS + team;
-    const bool live = row < a.n;
+    const int64_t row = ((int64_t)blockIdx.x * 4 + wave) * TEAMS + team, at = row < a.n ? row : a.n - 1;
     const int base = l * VPL;
 
     acc x[VPL];
-    load_scores<VPL>(a, live ? row : a.n - 1, base, x);
-    bool bad;
-    unsigned open = open_scores<L, VPL>(a, live, row, base, x, &bad);
+    load_scores<VPL>(a, at, base, x);
+    const bool bad = close_scores<L, VPL>(a, at, base, x);
 
     // the softmax's maximum and sum, where something asks for them
     const bool plain_keys = KIND == KEY_16 || (a.bias == nullptr && !(a.groups > 1 && a.top2));
-    acc xmax = -INFINITY;
+    acc xmax = 0, z = 0;
     if (!a.sigmoid && (!a.renorm || !plain_keys)) {
+        xmax = x[0];
 #pragma unroll
-        for (int s = 0; s < VPL; ++s) xmax = open >> s & 1 && x[s] > xmax ? x[s] : xmax;
+        for (int s = 1; s < VPL; ++s) xmax = OpMax()(xmax, x[s]);
         xmax = lanes_reduce<L>(xmax, OpMax());
-    }
-    acc z = 0;
-    if (!a.sigmoid && !a.renorm) {
+        if (!a.renorm) {
 #pragma unroll
-        for (int s = 0; s < VPL; ++s) z += open >> s & 1 ? exp_of(x[s] - xmax) : (acc)0;
-        z = lanes_reduce<L>(z, OpSum());
+            for (int s = 0; s < VPL; ++s) z += exp_of(x[s] - xmax);
+            z = lanes_reduce<L>(z, OpSum());
+        }
     }
 
-    // clean keys: what groups are ranked by
+    // keys without their tags: what groups are ranked by
     using clean = std::conditional_t<KIND == KEY_16, float, double>;
     clean v[VPL];
-    if (KIND == KEY_16 || plain_keys) {
 #pragma unroll
-        for (int s = 0; s < VPL; ++s) v[s] = open >> s & 1 ? (clean)x[s] : (clean)-INFINITY;
-    } else {
+    for (int s = 0; s < VPL; ++s) v[s] = (clean)x[s];
+    if constexpr (KIND != KEY_16) if (!plain_keys) {
         if (a.sigmoid) {
 #pragma unroll
-            for (int s = 0; s < VPL; ++s) v[s] = (clean)sigmoid_of((double)x[s]);
+            for (int s = 0; s < VPL; ++s) v[s] = sigmoid_of((double)x[s]);
         } else {
             double zz = 0.0;
 #pragma unroll
-            for (int s = 0; s < VPL; ++s) { v[s] = (clean)(open >> s & 1 ? exp_of((double)x[s] - (double)xmax) : 0.0); zz += v[s]; }
+            for (int s = 0; s < VPL; ++s) { v[s] = exp_of((double)x[s] - (double)xmax); zz += x[s] == -INFINITY ? 0.0 : v[s]; }
             const double inv = inverse(lanes_reduce<L>(zz, OpSum()));
 #pragma unroll
-            for (int s = 0; s < VPL; ++s) v[s] = (clean)(v[s] * inv);
+            for (int s = 0; s < VPL; ++s) v[s] *= inv;
         }
         if (a.bias != nullptr) {
             double b[VPL];
             if (a.bias_f64) load_pieces<double, VPL>(static_cast<const double*>(a.bias), base, a.E, b, 0.0);
             else load_pieces<float, VPL>(static_cast<const float*>(a.bias), base, a.E, b, 0.0);
 #pragma unroll
-            for (int s = 0; s < VPL; ++s) v[s] += (clean)b[s];
+            for (int s = 0; s < VPL; ++s) v[s] += b[s];
         }
-#pragma unroll
-        for (int s = 0; s < VPL; ++s) v[s] = open >> s & 1 ? v[s] : (clean)-INFINITY;
     }
+    if constexpr (KIND != KEY_16) {
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) v[s] = with_hi(v[s], x[s] == -INFINITY ? CLOSED_HI : hi_of(v[s]));
+    }
+    constexpr clean CLOSED = KIND == KEY_16 ? (clean)-INFINITY : (clean)-1.7976931348623157e308;
+    auto is_open = [](clean t) { return KIND == KEY_16 ? t > (clean)-INFINITY : t > (clean)CLOSED_BELOW; };
 
     if (a.groups > 1) {
         clean* gs = reinterpret_cast<clean*>(lds) + (size_t)(wave * TEAMS + team) * (a.lanes_per_group ? a.groups : a.E + a.groups);
         if (a.lanes_per_group) {
             // a group is the whole of lanes_per_group neighbouring lanes: its two best by lane, then across them
-            clean m1 = -INFINITY, m2 = -INFINITY;
+            clean m1 = CLOSED, m2 = CLOSED;
 #pragma unroll
             for (int s = 0; s < VPL; ++s) {
-                const clean low = v[s] < m1 ? v[s] : m1;
-                m2 = low > m2 ? low : m2;
-                m1 = v[s] > m1 ? v[s] : m1;
+                m2 = OpMax()(m2, OpMin()(v[s], m1));
+                m1 = OpMax()(m1, v[s]);
             }
             auto join = [&](auto mc) {
                 constexpr int M = decltype(mc)::value;
                 if constexpr (M < L) {
                     if (M < a.lanes_per_group) {
                         const clean o1 = lane_swap<M>(m1), o2 = lane_swap<M>(m2);
-                        const clean low = o1 < m1 ? o1 : m1;
-                        m2 = m2 > o2 ? m2 : o2;
-                        m2 = low > m2 ? low : m2;
-                        m1 = o1 > m1 ? o1 : m1;
+                        m2 = OpMax()(OpMax()(m2, o2), OpMin()(o1, m1));
+                        m1 = OpMax()(m1, o1);
                     }
                 }
             };
             join(std::integral_constant<int, 1>()); join(std::integral_constant<int, 2>()); join(std::integral_constant<int, 4>());
             join(std::integral_constant<int, 8>()); join(std::integral_constant<int, 16>()); join(std::integral_constant<int, 32>());
             const int g = l / a.lanes_per_group;
-            const clean mine = a.top2 && m2 > -INFINITY ? m1 + m2 : m1;
+            const clean mine = a.top2 && is_open(m2) ? m1 + m2 : m1;
             if (g < a.groups) gs[g] = mine;
             wave_sync();
             int ahead = 0;
             for (int h = 0; h < a.groups; ++h) { const clean o = gs[h]; ahead += o > mine || (o == mine && h < g) ? 1 : 0; }
-            if (ahead >= a.top_groups) open = 0;
+            if (ahead >= a.top_groups) {
+#pragma unroll
+                for (int s = 0; s < VPL; ++s) v[s] = CLOSED;
+            }
         } else {
             // any other size: the team's keys through LDS, lane l scores the groups l, l + L, ...
             clean* keys = gs + a.groups;
@@ -240,12 +246,13 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
             for (int s = 0; s < VPL; ++s) if (base + s < a.E) keys[base + s] = v[s];
             wave_sync();
             for (int g = l; g < a.groups; g += L) {
-                clean m1 = -INFINITY, m2 = -INFINITY;
+                clean m1 = CLOSED, m2 = CLOSED;
                 for (int i = 0; i < a.group_size; ++i) {
                     const clean t = keys[g * a.group_size + i];
-                    if (t > m1) { m2 = m1; m1 = t; } else if (t > m2) m2 = t;
+                    m2 = OpMax()(m2, OpMin()(t, m1));
+                    m1 = OpMax()(m1, t);
                 }
-                gs[g] = a.top2 && m2 > -INFINITY ? m1 + m2 : m1;
+                gs[g] = a.top2 && is_open(m2) ? m1 + m2 : m1;
             }
             wave_sync();
             unsigned long long kept = 0;
@@ -259,54 +266,66 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
             int g = base / a.group_size, r = base - g * a.group_size;
 #pragma unroll
             for (int s = 0; s < VPL; ++s) {
-                if (g < a.groups && !(kept >> g & 1)) open &= ~(1u << s);
+                if (g < a.groups && !(kept >> g & 1)) v[s] = CLOSED;
                 if (++r == a.group_size) { r = 0; ++g; }
             }
         }
     }
 
-    // the k best; lane j of the team keeps the j-th
+    // the k best; lane j of the team keeps the j-th and, where the key is the score, that
     int mine = -1;
+    double xe = 0.0;
     if constexpr (KIND == KEY_F64) {
-#pragma unroll
-        for (int s = 0; s < VPL; ++s) v[s] = open >> s & 1 ? v[s] : -INFINITY;
         for (int j = 0; j < a.k; ++j) {
-            double m = -INFINITY;
+            double m = CLOSED;
 #pragma unroll
             for (int s = 0; s < VPL; ++s) m = v[s] > m ? v[s] : m;
             m = lanes_reduce<L>(m, OpMax());
-            int at = a.E;
+            int best = a.E;
 #pragma unroll
-            for (int s = VPL - 1; s >= 0; --s) at = v[s] == m ? base + s : at;
-            at = lanes_reduce<L>(at, OpMin());
+            for (int s = VPL - 1; s >= 0; --s) best = v[s] == m ? base + s : best;
+            best = lanes_reduce<L>(best, OpMin());
 #pragma unroll
-            for (int s = 0; s < VPL; ++s) v[s] = base + s == at ? -INFINITY : v[s];
-            if (l == j) mine = m > -INFINITY ? at : -1;
+            for (int s = 0; s < VPL; ++s) v[s] = base + s == best ? CLOSED : v[s];
+            if (l == j) mine = is_open(m) ? best : -1;
         }
-    } else {
-        using K = Key<KIND>;
-        typename K::type key[VPL];
+    } else if constexpr (KIND == KEY_16) {
+        const unsigned tag = lane_tag(l);
+        unsigned key[VPL], m = 0x80000000u, kept = 0;
 #pragma unroll
-        for (int s = 0; s < VPL; ++s) key[s] = open >> s & 1 ? K::make(v[s], base + s) : K::closed();
+        for (int s = 0; s < VPL; ++s) key[s] = key16(v[s], tag, s);
         for (int j = 0; j < a.k; ++j) {
-            typename K::type m = key[0];
+            unsigned below = 0;
 #pragma unroll
-            for (int s = 1; s < VPL; ++s) m = OpMax()(m, key[s]);
+            for (int s = 0; s < VPL; ++s) below = OpMax()(below, key[s] - m);
+            m += lanes_reduce<L>(below, OpMax());
+            kept = l == j ? m : kept;
+        }
+        if (kept >= KEY16_OPEN) { mine = expert_of<VPL>(kept & TAG_BITS); xe = (double)key16_score(kept); }
+    } else {
+        const unsigned tag = lane_tag(l);
+        double kept = CLOSED;
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) v[s] = key_tagged(v[s], tag, s);
+        for (int j = 0; j < a.k; ++j) {
+            double m = v[0];
+#pragma unroll
+            for (int s = 1; s < VPL; ++s) m = OpMax()(m, v[s]);
             m = lanes_reduce<L>(m, OpMax());
 #pragma unroll
-            for (int s = 0; s < VPL; ++s) key[s] = key[s] == m ? K::closed() : key[s];
-            if (l == j) mine = K::is_open(m) ? K::expert(m) : -1;
+            for (int s = 0; s < VPL; ++s) v[s] = with_hi(v[s], v[s] == m ? CLOSED_HI : hi_of(v[s]));
+            kept = l == j ? m : kept;
         }
+        if (is_open(kept)) { mine = expert_of<VPL>(tag_of(kept)); xe = __builtin_bit_cast(double, __builtin_bit_cast(long long, kept) & ~(long long)TAG_BITS); }
     }
     if (bad) mine = -1;
 
     // weights: one slot a lane, in 64 bits except for the plain softmax (a sigmoid's sum may be far below 1)
-    const bool chosen = mine >= 0 && l < a.k;
+    const bool chosen = mine >= 0;
+    if (chosen && (KIND == KEY_F64 || !plain_keys)) xe = (double)score_at<acc>(a, at, mine);
     acc w = 0;
-    const double xe = chosen ? (double)score_at<acc>(a, row, mine) : 0.0;
     if (a.renorm) {
-        double top = chosen ? xe : -INFINITY;
-        top = lanes_reduce<L>(top, OpMax());
+        const double top = lanes_reduce<L>(chosen ? xe : -INFINITY, OpMax());
         // below -40 a sigmoid is the exponential to 2^-57
         double p = 0.0;
         if (chosen) p = a.sigmoid && top > -40.0 ? sigmoid_of(xe) : exp_of(xe - top);
@@ -315,7 +334,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
     } else if (chosen) {
         w = a.sigmoid ? (acc)(a.scale * (xe < -700.0 ? exp_of(xe) : sigmoid_of(xe))) : (acc)a.scale * (exp_of((acc)xe - xmax) / z);
     }
-    if (live && l < a.k) {
+    if (row < a.n && l < a.k) {
         a.experts[row * a.k + l] = mine;
         static_cast<acc*>(a.weights)[row * a.k + l] = bad ? (acc)NAN : w;
     }
@@ -361,17 +380,17 @@ __global__ void __launch_bounds__(256) route_grad_kernel(RouteDev a) {
     const acc xe = chosen ? score_at<acc>(a, at, e) : (acc)0;
     const acc g = chosen ? (acc)a.scale * static_cast<const acc*>(a.dweights)[at * a.k + l] : (acc)0;
 
-    acc x[VPL], xmax = -INFINITY, inv = 0;
+    acc x[VPL], xmax, inv = 0;
     if (dense) {
         load_scores<VPL>(a, at, base, x);
-        bool bad;
-        const unsigned open = open_scores<L, VPL>(a, live, row, base, x, &bad);
+        close_scores<L, VPL>(a, at, base, x);
+        xmax = x[0];
 #pragma unroll
-        for (int s = 0; s < VPL; ++s) xmax = open >> s & 1 && x[s] > xmax ? x[s] : xmax;
+        for (int s = 1; s < VPL; ++s) xmax = OpMax()(xmax, x[s]);
         xmax = lanes_reduce<L>(xmax, OpMax());
         acc z = 0;
 #pragma unroll
-        for (int s = 0; s < VPL; ++s) { x[s] = open >> s & 1 ? exp_of(x[s] - xmax) : (acc)0; z += x[s]; }
+        for (int s = 0; s < VPL; ++s) { x[s] = exp_of(x[s] - xmax); z += x[s]; }
         inv = inverse(lanes_reduce<L>(z, OpSum()));
     } else {
 #pragma unroll
@@ -411,23 +430,31 @@ __global__ void __launch_bounds__(256) route_grad_kernel(RouteDev a) {
     else store_pieces<acc, VPL>(static_cast<float*>(a.dscores) + row * a.ld_out, base, a.E, out);
 }
 
-// Lanes of a team and scores a lane: the fewest lanes that hold the row with at most 16 scores each -- the steps across lanes, which
-// a row pays k times, are few, and a wave serves many rows -- but at least k, so that every slot has a lane.
-template <typename F> static int with_team(int E, int k, F&& fn) {
+// Lanes of a team and scores a lane.  Fewest lanes first, at most `most` scores each: the steps across lanes, which a row pays k
+// times, and the work per row and wave are then fewest (1048576 x 24 float32, k = 2: 49 us with 4 lanes of 8, ROWS_2 with 2 of 12).  At least
+// k lanes, so that every slot has one, and more of them while the rows fill less than 4 waves a SIMD and a lane has more than 4 scores:
+// one row of 64 then takes ONE_16 with 16 lanes instead of ONE_4 with 4.
+template <int MOST, typename F> static int with_team(int E, int k, int64_t rows, F&& fn) {
     auto by_vpl = [&](auto lc) {
         constexpr int L = decltype(lc)::value;
         const int per = (E + L - 1) / L;
         if (per <= 4) return fn(lc, std::integral_constant<int, 4>());
         if (per <= 8) return fn(lc, std::integral_constant<int, 8>());
         if (per <= 12) return fn(lc, std::integral_constant<int, 12>());
+        if constexpr (MOST > 16) { if (per > 16) return fn(lc, std::integral_constant<int, 24>()); }
         return fn(lc, std::integral_constant<int, 16>());
     };
-    const int need = (E + 15) / 16 > k ? (E + 15) / 16 : k;
-    if (need <= 4) return by_vpl(std::integral_constant<int, 4>());
-    if (need <= 8) return by_vpl(std::integral_constant<int, 8>());
-    if (need <= 16) return by_vpl(std::integral_constant<int, 16>());
-    if (need <= 32) return by_vpl(std::integral_constant<int, 32>());
-    return by_vpl(std::integral_constant<int, 64>());
+    int lanes = 2;
+    while (lanes < k || lanes * MOST < E) lanes *= 2;
+    while (lanes < 64 && lanes * 4 < E && rows * lanes < (int64_t)64 * 4096) lanes *= 2;
+    switch (lanes) {
+        case 2: return by_vpl(std::integral_constant<int, 2>());
+        case 4: return by_vpl(std::integral_constant<int, 4>());
+        case 8: return by_vpl(std::integral_constant<int, 8>());
+        case 16: return by_vpl(std::integral_constant<int, 16>());
+        case 32: return by_vpl(std::integral_constant<int, 32>());
+        default: return by_vpl(std::integral_constant<int, 64>());
+    }
 }
 
 static int route_check(const oak_route_args* a) {
@@ -464,28 +491,29 @@ static int route_launch(hipStream_t stream, const oak_route_args* a) {
     if (a->n_rows == 0) return OAK_OK;
     RouteDev d = route_dev(a);
     const bool plain_keys = d.bias == nullptr && !(d.groups > 1 && d.top2);
-    return with_team(d.E, d.k, [&](auto lc, auto vc) {
-        constexpr int L = decltype(lc)::value, VPL = decltype(vc)::value, TEAMS = 64 / L;
-        const dim3 grid((unsigned)((d.n + 4 * TEAMS - 1) / (4 * TEAMS)));
-        // groups that are whole lanes, a power of two of them, are scored without LDS
-        const int lanes = d.group_size % VPL == 0 ? d.group_size / VPL : 0;
-        d.lanes_per_group = lanes > 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
-        const size_t lds = d.groups > 1 ? (size_t)4 * TEAMS * (d.lanes_per_group ? d.groups : d.E + d.groups) * sizeof(double) : 0;
-        auto go = [&](auto kind) {
+    auto run = [&](auto kind, auto most) {
+        return with_team<decltype(most)::value>(d.E, d.k, d.n, [&](auto lc, auto vc) {
+            constexpr int L = decltype(lc)::value, VPL = decltype(vc)::value, TEAMS = 64 / L;
+            const dim3 grid((unsigned)((d.n + 4 * TEAMS - 1) / (4 * TEAMS)));
+            // groups that are whole lanes, a power of two of them, are scored without LDS
+            const int lanes = d.group_size % VPL == 0 ? d.group_size / VPL : 0;
+            d.lanes_per_group = lanes > 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+            const size_t lds = d.groups > 1 ? (size_t)4 * TEAMS * (d.lanes_per_group ? d.groups : d.E + d.groups) * sizeof(double) : 0;
             auto kernel = route_kernel<decltype(kind)::value, L, VPL>;
             if (lds > 64 * 1024) OAK_CHECK(ensure_dynamic_lds((const void*)kernel, 160 * 1024));
             return launch(kernel, grid, dim3(256), lds, stream, d);
-        };
-        if (d.dtype == OAK_F64) return go(std::integral_constant<int, KEY_F64>());
-        if (d.dtype != OAK_F32 && plain_keys) return go(std::integral_constant<int, KEY_16>());
-        return go(std::integral_constant<int, KEY_TAG>());
-    });
+        });
+    };
+    // 64-bit keys take twice the registers: at most 16 a lane
+    if (d.dtype == OAK_F64) return run(std::integral_constant<int, KEY_F64>(), std::integral_constant<int, 16>());
+    if (d.dtype != OAK_F32 && plain_keys) return run(std::integral_constant<int, KEY_16>(), std::integral_constant<int, 24>());
+    return run(std::integral_constant<int, KEY_TAG>(), std::integral_constant<int, 16>());
 }
 
 static int route_grad_launch(hipStream_t stream, const oak_route_args* a) {
     if (a->n_rows == 0) return OAK_OK;
     const RouteDev d = route_dev(a);
-    return with_team(d.E, d.k, [&](auto lc, auto vc) {
+    return with_team<16>(d.E, d.k, d.n, [&](auto lc, auto vc) {
         constexpr int L = decltype(lc)::value, VPL = decltype(vc)::value, TEAMS = 64 / L;
         const dim3 grid((unsigned)((d.n + 4 * TEAMS - 1) / (4 * TEAMS)));
         auto go = [&](auto zero) {

@@ -52,6 +52,8 @@ struct OpMax { template <typename A> __device__ __forceinline__ A operator()(A a
 template <> __device__ __forceinline__ double OpMax::operator()(double a, double b) const { return __builtin_fmax(a, b); }
 template <> __device__ __forceinline__ float OpMax::operator()(float a, float b) const { return __builtin_fmaxf(a, b); }
 struct OpMin { template <typename A> __device__ __forceinline__ A operator()(A a, A b) const { return a < b ? a : b; } };
+template <> __device__ __forceinline__ double OpMin::operator()(double a, double b) const { return __builtin_fmin(a, b); }
+template <> __device__ __forceinline__ float OpMin::operator()(float a, float b) const { return __builtin_fminf(a, b); }
 struct OpSum { template <typename A> __device__ __forceinline__ A operator()(A a, A b) const { return a + b; } };
 struct OpOr { template <typename A> __device__ __forceinline__ A operator()(A a, A b) const { return a | b; } };
 
