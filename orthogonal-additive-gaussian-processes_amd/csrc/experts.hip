@@ -40,19 +40,26 @@ struct RouteDev {
     const void* dweights; void* dscores;
 };
 
+// A lane's piece of a row.  No branch depends on the lane: what lies behind the row's end is read from inside the row and replaced, so
+// that all loads of a piece are in flight together (a branch around each would wait for its own).
 template <typename T, int VPL, typename A> __device__ __forceinline__ void load_pieces(const T* p, int base, int E, A (&x)[VPL], A out_of_range) {
-    typedef T four __attribute__((ext_vector_type(4)));
-    typedef four four_at __attribute__((aligned(sizeof(T))));
+    if ((E & 3) == 0) {
+        typedef T four __attribute__((ext_vector_type(4)));
+        typedef four four_at __attribute__((aligned(sizeof(T))));
+        four b[VPL / 4];
 #pragma unroll
-    for (int c = 0; c < VPL; c += 4) {
-        if (base + c + 4 <= E) {
-            const four b = *reinterpret_cast<const four_at*>(p + base + c);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[c + i] = (A)b[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[c + i] = base + c + i < E ? (A)p[base + c + i] : out_of_range;
+        for (int c = 0; c < VPL / 4; ++c) {
+            const int e = base + 4 * c < E ? base + 4 * c : E - 4;
+            b[c] = *reinterpret_cast<const four_at*>(p + e);
         }
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) x[s] = base + (s & ~3) < E ? (A)b[s / 4][s & 3] : out_of_range;
+    } else {
+        T b[VPL];
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) b[s] = p[base + s < E ? base + s : E - 1];
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) x[s] = base + s < E ? (A)b[s] : out_of_range;
     }
 }
 // the lane's piece of a row of scores; the element type is a uniform branch: one kernel serves all of a kind
@@ -98,14 +105,15 @@ __device__ __forceinline__ float inverse(float d) { return 1.0f / d; }
 // sigmoid; far below 0 (|x| > 700) what is left is 1e-304
 __device__ __forceinline__ double sigmoid_of(double x) { return inverse(1.0 + exp_of(x < -700.0 ? 700.0 : -x)); }
 
-// closes the masked scores (-inf); true if an open one is NaN or +inf
-template <int L, int VPL, typename A> __device__ __forceinline__ bool close_scores(const RouteDev& a, int64_t row, int base, A (&x)[VPL]) {
+// the piece with its masked scores closed (-inf); true if an open one of the row is NaN or +inf
+template <int L, int VPL, typename A> __device__ __forceinline__ bool open_scores(const RouteDev& a, int64_t row, int base, A (&x)[VPL]) {
     if (a.mask != nullptr) {
-        unsigned m[VPL];
-        load_pieces<unsigned char, VPL>(a.mask + row * a.ld_mask, base, a.E, m, 0u);
+        unsigned char m[VPL];
+        load_pieces<unsigned char, VPL, unsigned char>(a.mask + row * a.ld_mask, base, a.E, m, 0);
+        load_scores<VPL>(a, row, base, x);
 #pragma unroll
         for (int s = 0; s < VPL; ++s) x[s] = m[s] != 0 ? x[s] : (A)-INFINITY;
-    }
+    } else load_scores<VPL>(a, row, base, x);
     bool wrong = false;
 #pragma unroll
     for (int s = 0; s < VPL; ++s) wrong |= !(x[s] < (A)INFINITY);
@@ -157,8 +165,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
     const int base = l * VPL;
 
     acc x[VPL];
-    load_scores<VPL>(a, at, base, x);
-    const bool bad = close_scores<L, VPL>(a, at, base, x);
+    const bool bad = open_scores<L, VPL>(a, at, base, x);
 
     // the softmax's maximum and sum, where something asks for them
     const bool plain_keys = KIND == KEY_16 || (a.bias == nullptr && !(a.groups > 1 && a.top2));
@@ -382,8 +389,7 @@ __global__ void __launch_bounds__(256) route_grad_kernel(RouteDev a) {
 
     acc x[VPL], xmax, inv = 0;
     if (dense) {
-        load_scores<VPL>(a, at, base, x);
-        close_scores<L, VPL>(a, at, base, x);
+        open_scores<L, VPL>(a, at, base, x);
         xmax = x[0];
 #pragma unroll
         for (int s = 1; s < VPL; ++s) xmax = OpMax()(xmax, x[s]);
@@ -431,9 +437,10 @@ __global__ void __launch_bounds__(256) route_grad_kernel(RouteDev a) {
 }
 
 // Lanes of a team and scores a lane.  Fewest lanes first, at most `most` scores each: the steps across lanes, which a row pays k
-// times, and the work per row and wave are then fewest (1048576 x 24 float32, k = 2: 49 us with 4 lanes of 8, ROWS_2 with 2 of 12).  At least
-// k lanes, so that every slot has one, and more of them while the rows fill less than 4 waves a SIMD and a lane has more than 4 scores:
-// one row of 64 then takes ONE_16 with 16 lanes instead of ONE_4 with 4.
+// times, and the work per row and wave are then fewest (kernel time: 1048576 x 24 float32, k = 2: 49 us with 4 lanes of 8, 27 with 2 of 12; 65536 x 160 bf16, k = 6:
+// 17.5 us with 8 lanes of 24, 15.8 with 8 of 20; the gradient of those, which goes through LDS, 16.9 us with 16 of 12, 18.5 with 8 of 20, so
+// that it stays at 16 scores a lane).  At least k lanes, so that every slot has one, and more of them while the rows fill less than 4 waves a
+// SIMD and a lane has more than 4 scores: one row of 64 takes 2.4 us with 16 lanes, 3.1 with 8.
 template <int MOST, typename F> static int with_team(int E, int k, int64_t rows, F&& fn) {
     auto by_vpl = [&](auto lc) {
         constexpr int L = decltype(lc)::value;
@@ -441,7 +448,10 @@ template <int MOST, typename F> static int with_team(int E, int k, int64_t rows,
         if (per <= 4) return fn(lc, std::integral_constant<int, 4>());
         if (per <= 8) return fn(lc, std::integral_constant<int, 8>());
         if (per <= 12) return fn(lc, std::integral_constant<int, 12>());
-        if constexpr (MOST > 16) { if (per > 16) return fn(lc, std::integral_constant<int, 24>()); }
+        if constexpr (MOST > 16) {
+            if (per > 20) return fn(lc, std::integral_constant<int, 24>());
+            if (per > 16) return fn(lc, std::integral_constant<int, 20>());
+        }
         return fn(lc, std::integral_constant<int, 16>());
     };
     int lanes = 2;
