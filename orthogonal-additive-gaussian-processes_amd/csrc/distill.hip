@@ -7,9 +7,13 @@
 //            dL/ds_v = tau w q_v (log q_b - log p_b - L / (tau^2 w)),  b the outcome v belongs to
 // so the gradient is one coefficient times q_v on the rest and k values of their own on the top.
 //
-// q_r is summed over the rest itself (its own running maximum, the teacher's entries left out by a bit per class in LDS): taken
-// as 1 - sum q_k it would lose every digit where the student is sure of itself.  The sums over the classes run in 32 bits (64 for
-// double), everything per entry and per row in 64.
+// q_r is summed over the rest itself (the teacher's entries left out, found by a bit per class in LDS): taken as 1 - sum q_k it would lose
+// every digit where the student is sure of itself.  The sums over the classes run in 32 bits (64 for double), everything per entry
+// and per row in 64.
+//
+// A row stays in the registers of its team of NT threads, NV units of 16 bytes each, so that it is read once: the sum and the gradient
+// each walk the registers.  The team's first wave (all of a team of 16 or 64) does what concerns the entries.  Every sum over the entries is taken on
+// references known before the pass over the classes (the entries' own maximum), so that only one reduction per row waits for that pass.
 #include "lowp.h"
 
 namespace oak {
@@ -26,234 +30,296 @@ struct DistillDev {
 // exp(t / tau) for t <= 0.  float: 2^(t c) with c in two parts, since a c off by half a unit would put a common relative error of |t| c 2^-25
 // on all the terms of a sum (t = 20: 1e-6 in log z, more than a small divergence bears).  Both parts are positive: t = -inf gives 0, NaN stays NaN.
 __device__ __forceinline__ float exp_scaled(const DistillDev& a, float t) { return __builtin_amdgcn_exp2f(__builtin_fmaf(t, a.c_hi, t * a.c_lo)); }
-__device__ __forceinline__ double exp_scaled(const DistillDev& a, double t) { return exp(t * a.inv_tau); }
-
-template <int NT> __device__ __forceinline__ void row_sync() {
-    if constexpr (NT == 64) wave_sync(); else __syncthreads();
+__device__ __forceinline__ double exp_scaled(const DistillDev& a, double t) { return exp_of(t * a.inv_tau); }
+// for a gradient of type T: one part of c is enough for 16 bits
+template <typename T> __device__ __forceinline__ typename Num<T>::acc exp_gradient(const DistillDev& a, typename Num<T>::acc t) {
+    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(t * a.c_hi); else return exp_scaled(a, t);
 }
 
-// sums and maxima over the NT threads of a row, in a fixed order; scratch: NT / 64 doubles per value
-template <int NT, int Q> __device__ __forceinline__ void row_sum(double (&v)[Q], double* scratch) {
-#pragma unroll
-    for (int q = 0; q < Q; ++q) v[q] = lanes_reduce<64>(v[q], OpSum());
-    if constexpr (NT > 64) {
-        constexpr int W = NT / 64;
-        const int wave = threadIdx.x >> 6;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0)
-            for (int q = 0; q < Q; ++q) scratch[q * W + wave] = v[q];
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            double s = 0.0;
-            for (int i = 0; i < W; ++i) s += scratch[q * W + i];
-            v[q] = s;
-        }
-    }
-}
-template <int NT, int Q> __device__ __forceinline__ void row_max(double (&v)[Q], double* scratch) {
-#pragma unroll
-    for (int q = 0; q < Q; ++q) v[q] = lanes_reduce<64>(v[q], OpMax());
-    if constexpr (NT > 64) {
-        constexpr int W = NT / 64;
-        const int wave = threadIdx.x >> 6;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0)
-            for (int q = 0; q < Q; ++q) scratch[q * W + wave] = v[q];
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            double s = scratch[q * W];
-            for (int i = 1; i < W; ++i) s = s > scratch[q * W + i] ? s : scratch[q * W + i];
-            v[q] = s;
-        }
-    }
-}
-
-// LDS of one row: [bits: V / 32 words][log p: K doubles][student's entries: K doubles][scratch][class: K ints], in 8-byte steps
+// LDS of one team, in 8-byte steps: [bits: one a class][t - reference][p][exp((x - x_ref) / tau)][waves' maxima and sums, row's numbers][class]
+__host__ __device__ inline size_t distill_words(int V) { return ((size_t)V + 63) / 64 * 2; }
 __host__ __device__ inline size_t distill_lds(int V, int K, int NT) {
-    const size_t words = ((size_t)V + 63) / 64 * 2;
-    return words * 4 + (size_t)K * 16 + (NT > 64 ? (size_t)NT / 64 * 4 * 8 : 0) + ((size_t)K * 4 + 15) / 16 * 16;
+    return distill_words(V) * 4 + (size_t)K * 24 + (NT > 64 ? (size_t)(NT / 64 * 2 + 4) * 8 : 0) + ((size_t)K * 4 + 15) / 16 * 16;
 }
 
-template <typename T, int NT>
+// what the team does with its row's gradient
+enum { ROW_COMPUTE = 0, ROW_ZERO = 1, ROW_NAN = 2 };
+
+template <typename T, int NT, int NV>
 __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillDev a) {
     using acc = typename Num<T>::acc;
-    constexpr int VN = Vec<T>::N, ROWS = NT < 256 ? 256 / NT : 1;
+    using raw = typename Vec<T>::raw;
+    constexpr int VN = Vec<T>::N, ROWS = NT < 256 ? 256 / NT : 1, LEAD = NT < 64 ? NT : 64, WAVES = NT / 64;
+    constexpr acc LOWEST = sizeof(acc) == 8 ? (acc)-1.7976931348623157e308 : (acc)-3.402823466e38f;
     extern __shared__ __align__(16) unsigned char lds_all[];
     const int tid = threadIdx.x & (NT - 1);
-    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / NT;
-    if (row >= a.n) return;                            // ROWS > 1: whole waves, which only wait for themselves
-    unsigned char* lds = lds_all + (threadIdx.x / NT) * distill_lds(a.V, a.K, NT);
-    const int words = (a.V + 63) / 64 * 2;
+    unsigned char* lds = lds_all + (NT < 256 ? threadIdx.x / NT : 0) * distill_lds(a.V, a.K, NT);
+    const int words = (int)distill_words(a.V);
     unsigned* bits = reinterpret_cast<unsigned*>(lds);
-    double* logp = reinterpret_cast<double*>(lds + (size_t)words * 4);
-    double* xtop = logp + a.K;
-    double* scratch = xtop + a.K;
-    int* cls = reinterpret_cast<int*>(scratch + (NT > 64 ? NT / 64 * 4 : 0));
+    double* tk = reinterpret_cast<double*>(lds + (size_t)words * 4);
+    double* pk = tk + a.K;
+    double* ek = pk + a.K;
+    double* share = ek + a.K;
+    int* cls = reinterpret_cast<int*>(share + (NT > 64 ? WAVES * 2 + 4 : 0));
+    const int nvec = a.V / VN, tail = a.V - nvec * VN;
+    const bool lead = tid < LEAD;
+    auto team_sync = [] { if constexpr (NT <= 64) wave_sync(); else __syncthreads(); };
 
-    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
-    T* g = a.dlogits ? static_cast<T*>(a.dlogits) + row * a.ld_out : nullptr;
-    acc* loss = static_cast<acc*>(a.loss);
-    const int nvec = a.V / VN;
-    const double w = a.weight ? load_any(a.weight, a.weight_dtype, row) : 1.0;
-
-    auto fill = [&](T value) {
-        if (g == nullptr) return;
-        typename Vec<T>::raw z;
-        for (int i = 0; i < VN; ++i) z[i] = value;
-        for (int u = tid; u < nvec; u += NT) Vec<T>::store(g + (size_t)u * VN, z);
-        for (int v = nvec * VN + tid; v < a.V; v += NT) g[v] = value;
-    };
-    if (w == 0.0) { fill((T)0); if (tid == 0) loss[row] = 0; return; }
-
-    // ---- the teacher's entries -------------------------------------------------------------------------------------
     for (int i = tid; i < words; i += NT) bits[i] = 0;
-    row_sync<NT>();
-    double seen[3] = {0.0, 0.0, 0.0};                  // entries, entries of a class seen before, indices out of range
-    for (int k = tid; k < a.K; k += NT) {
-        const int64_t c = a.index_64 ? static_cast<const int64_t*>(a.index)[row * a.ld_index + k] : static_cast<const int32_t*>(a.index)[row * a.ld_index + k];
-        const double t = load_any(a.top, a.top_dtype, row * a.ld_top + k);
-        const bool in = c >= 0 && c < a.V, there = in && !(t == -INFINITY);
-        if (there) {
-            const unsigned before = atomicOr(&bits[c >> 5], 1u << (c & 31));
-            seen[0] += 1.0;
-            seen[1] += before >> (c & 31) & 1 ? 1.0 : 0.0;
-            logp[k] = t * a.inv_tau;
-            xtop[k] = (double)(acc)x[c];
-        }
-        if (!in && c != -1) seen[2] += 1.0;
-        cls[k] = there ? (int)c : -1;
-    }
-    row_sum<NT>(seen, scratch);
-    if (seen[2] > 0.0) { fill((T)NAN); if (tid == 0) loss[row] = NAN; return; }
-    if (seen[0] == 0.0) { fill((T)0); if (tid == 0) loss[row] = 0; return; }
-    row_sync<NT>();
-    if (seen[1] > 0.0) {
-        // entries of one class: the first takes the logarithm of their sum, the others become padding
-        constexpr int PER = (OAK_MAX_TEACHER + NT - 1) / NT;
-        double merged[PER]; int keep = 0;
-        int q = 0;
-        for (int k = tid; k < a.K; k += NT, ++q) {
-            const int c = cls[k];
-            bool first = c >= 0;
-            double m = -INFINITY, s = 0.0;
-            for (int i = 0; c >= 0 && i < a.K; ++i) {
-                if (cls[i] != c) continue;
-                if (i < k) first = false;
-                m = logp[i] > m ? logp[i] : m;
+    team_sync();
+
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + (NT < 256 ? threadIdx.x / NT : 0); row < a.n; row += (int64_t)gridDim.x * ROWS) {
+        const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+        T* g = a.dlogits ? static_cast<T*>(a.dlogits) + row * a.ld_out : nullptr;
+        const double w = a.weight ? load_any(a.weight, a.weight_dtype, row) : 1.0;
+        int todo = w == 0.0 ? ROW_ZERO : ROW_COMPUTE;
+
+        // this lane's place, forgotten by the compiler now and then: it would otherwise keep the NV addresses, offsets and bit positions of a
+        // lane in registers from row to row
+        int at = tid;
+        auto forget_place = [&] { asm volatile("" : "+v"(at)); };
+        forget_place();
+        // ---- the row into registers; units behind its end are read from inside it and not used -----------------------------
+        typedef int words4 __attribute__((ext_vector_type(4)));
+        words4 data[NV > 0 ? NV : 1];
+        acc last = -INFINITY;                          // one of the elements that do not fill a unit
+        if (todo == ROW_COMPUTE) {
+            if (NV > 0 && nvec > 0) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int u = i * NT + at;
+                    data[i] = __builtin_bit_cast(words4, Vec<T>::load(x + (size_t)(u < nvec ? u : nvec - 1) * VN));
+                }
             }
-            for (int i = 0; first && i < a.K; ++i) if (cls[i] == c) s += exp(logp[i] - m);
-            if (q < PER) merged[q] = m + log(s);
-            keep |= first ? 1 << q : 0;
+            if (tid < tail) last = (acc)x[nvec * VN + tid];
         }
-        row_sync<NT>();
-        q = 0;
-        for (int k = tid; k < a.K; k += NT, ++q) {
-            if (keep >> q & 1) logp[k] = merged[q]; else cls[k] = -1;
+
+        // ---- the teacher's entries ------------------------------------------------------------------------------------
+        double xref = -INFINITY, ref = 0.0, sums[6] = {0, 0, 0, 0, 0, 0};        // sum e, e (t - ref), e (x - xref); f, f (x - xref), f (t - ref)
+        bool some_rest = true;
+        if (lead && todo == ROW_COMPUTE) {
+            unsigned count = 0, again = 0, wrong = 0;
+            double tmax = -INFINITY;
+            for (int k = tid; k < a.K; k += LEAD) {
+                const int64_t c = a.index_64 ? static_cast<const int64_t*>(a.index)[row * a.ld_index + k] : static_cast<const int32_t*>(a.index)[row * a.ld_index + k];
+                const double t = load_any(a.top, a.top_dtype, row * a.ld_top + k) * a.inv_tau;
+                const bool in = c >= 0 && c < a.V, there = in && !(t == -INFINITY);
+                wrong |= !in && c != -1 ? 1u : 0u;
+                cls[k] = there ? (int)c : -1;
+                if (there) {
+                    const unsigned before = atomicOr(&bits[c >> 5], 1u << (c & 31));
+                    ++count;
+                    again += before >> (c & 31) & 1;
+                    const double xe = (double)(acc)x[c];
+                    tk[k] = t; ek[k] = xe;
+                    tmax = __builtin_fmax(tmax, t); xref = __builtin_fmax(xref, xe);
+                }
+            }
+            count = lanes_reduce<LEAD>(count, OpSum());
+            again = lanes_reduce<LEAD>(again, OpSum());
+            wrong = lanes_reduce<LEAD>(wrong, OpOr());
+            some_rest = count - again < (unsigned)a.V;
+            todo = wrong ? ROW_NAN : count == 0 ? ROW_ZERO : ROW_COMPUTE;
+            wave_sync();
+            if (again > 0) {
+                // entries of one class: the first takes the logarithm of their sum, the others become padding
+                for (int k = tid; k < a.K; k += LEAD) {
+                    const int c = cls[k];
+                    bool first = c >= 0;
+                    double m = -INFINITY, s = 0.0;
+                    for (int i = 0; c >= 0 && i < a.K; ++i) {
+                        if (cls[i] != c) continue;
+                        if (i < k) first = false;
+                        m = __builtin_fmax(m, tk[i]);
+                    }
+                    for (int i = 0; first && i < a.K; ++i) if (cls[i] == c) s += exp_of(tk[i] - m);
+                    pk[k] = first ? m + log_of(s) : -INFINITY;
+                }
+                wave_sync();
+                for (int k = tid; k < a.K; k += LEAD) {
+                    if (pk[k] == -INFINITY) cls[k] = -1; else { tk[k] = pk[k]; tmax = __builtin_fmax(tmax, pk[k]); }
+                }
+            }
+            ref = a.lse ? load_any(a.lse, a.lse_dtype, row) : lanes_reduce<LEAD>(tmax, OpMax());
+            xref = __builtin_fmax(lanes_reduce<LEAD>(xref, OpMax()), -1e300);
+            for (int k = tid; k < a.K; k += LEAD) if (cls[k] >= 0) {
+                const double dt = tk[k] - ref, dx = ek[k] - xref, e = exp_of(dt), f = exp_of(dx * a.inv_tau);
+                tk[k] = dt; pk[k] = e; ek[k] = f;
+                sums[0] += e;
+                if (e != 0.0) { sums[1] += e * dt; sums[2] += e * dx; }
+                sums[3] += f;
+                if (f != 0.0 && a.reverse) { sums[4] += f * dx; sums[5] += f * dt; }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sums[q] = lanes_reduce<LEAD>(sums[q], OpSum());
+            if (a.reverse) { sums[4] = lanes_reduce<LEAD>(sums[4], OpSum()); sums[5] = lanes_reduce<LEAD>(sums[5], OpSum()); }
         }
-        row_sync<NT>();
-    }
-    const bool some_rest = seen[0] - seen[1] < (double)a.V;
-    double zt = 0.0;
-    if (a.lse) zt = load_any(a.lse, a.lse_dtype, row);
-    else {
-        double m[1] = {-INFINITY}, s[1] = {0.0};
-        for (int k = tid; k < a.K; k += NT) if (cls[k] >= 0) m[0] = logp[k] > m[0] ? logp[k] : m[0];
-        row_max<NT>(m, scratch);
-        for (int k = tid; k < a.K; k += NT) if (cls[k] >= 0) s[0] += exp(logp[k] - m[0]);
-        row_sum<NT>(s, scratch);
-        zt = m[0] + log(s[0]);
-    }
+        if constexpr (NT > 64) {
+            if (tid == 0) share[WAVES * 2] = (double)todo;
+            __syncthreads();
+            todo = (int)share[WAVES * 2];
+        }
 
-    // ---- one pass over the classes: maximum and sum of the rest ------------------------------------------------------
-    constexpr acc LOWEST = sizeof(acc) == 8 ? (acc)-1.7976931348623157e308 : (acc)-3.402823466e38f;
-    acc m = LOWEST, z = 0;                             // a finite start: -inf - m stays -inf
-    auto take = [&](const acc (&v)[VN]) {
-        acc top = m;
+        acc m = LOWEST, z = 0;                         // a finite start: -inf - m stays -inf
+        if (todo == ROW_COMPUTE) {
+            auto forget = [&] {                         // the units, not their 32-bit forms, live from one walk to the next
 #pragma unroll
-        for (int i = 0; i < VN; ++i) top = v[i] > top ? v[i] : top;
-        z *= exp_scaled(a, m - top);
-        m = top;
+                for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(data[i]));
+                forget_place();
+            };
+            // ---- maximum and sum of the rest (without a rest outcome: of all classes) ----------------------------------------
+            const bool leave_out = a.lse != nullptr;
+            auto hide = [&](raw& r, int u) {            // the entries' classes become -inf; their gradients are written over at the end
+                const int v = u * VN;
+                const unsigned b = bits[v >> 5] >> (v & 31) & ((1u << VN) - 1);
+                if (__any(b != 0)) {
 #pragma unroll
-        for (int i = 0; i < VN; ++i) z += exp_scaled(a, v[i] - m);
-    };
-    auto bits_of = [&](int u) {                         // the VN bits of unit u
-        const int v = u * VN;
-        return bits[v >> 5] >> (v & 31);
-    };
-    for (int u = tid; u < nvec; u += NT) {
-        const auto r = Vec<T>::load(x + (size_t)u * VN);
-        const unsigned b = bits_of(u);
-        acc v[VN];
+                    for (int i = 0; i < VN; ++i) r[i] = b >> i & 1 ? (T)-INFINITY : r[i];
+                }
+            };
+            if (leave_out && tid < tail && (bits[(nvec * VN + tid) >> 5] >> ((nvec * VN + tid) & 31) & 1)) last = -INFINITY;
+            if constexpr (NV > 0) {
+                forget_place();
 #pragma unroll
-        for (int i = 0; i < VN; ++i) v[i] = b >> i & 1 ? (acc)-INFINITY : (acc)r[i];
-        take(v);
-    }
-    {
-        acc v[VN];
-        const int at = nvec * VN + tid;
+                for (int i = 0; i < NV; ++i) {
+                    const int u = i * NT + at;
+                    if (u < nvec) {
+                        raw r = __builtin_bit_cast(raw, data[i]);
+                        if (leave_out) { hide(r, u); data[i] = __builtin_bit_cast(words4, r); }
 #pragma unroll
-        for (int i = 0; i < VN; ++i) v[i] = -INFINITY;
-        if (at < a.V && tid < VN && !(bits[at >> 5] >> (at & 31) & 1)) v[0] = (acc)x[at];
-        if (tid < VN) take(v);
-    }
+                        for (int j = 0; j < VN; ++j) m = OpMax()(m, (acc)r[j]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);      // one unit at a time: the registers hold the row
+                }
+                m = OpMax()(m, last);
+                forget();
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    if (i * NT + at < nvec) {
+                        const raw r = __builtin_bit_cast(raw, data[i]);
+#pragma unroll
+                        for (int j = 0; j < VN; ++j) z += exp_scaled(a, (acc)r[j] - m);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                z += exp_scaled(a, last - m);
+                forget();
+            } else {
+                auto take = [&](raw r) {
+                    acc top = m;
+#pragma unroll
+                    for (int j = 0; j < VN; ++j) top = OpMax()(top, (acc)r[j]);
+                    z *= exp_scaled(a, m - top);
+                    m = top;
+#pragma unroll
+                    for (int j = 0; j < VN; ++j) z += exp_scaled(a, (acc)r[j] - m);
+                };
+                for (int u = tid; u < nvec; u += NT) {
+                    raw r = Vec<T>::load(x + (size_t)u * VN);
+                    if (leave_out) hide(r, u);
+                    take(r);
+                }
+                raw r;
+#pragma unroll
+                for (int j = 0; j < VN; ++j) r[j] = (T)-INFINITY;
+                r[0] = (T)last;
+                take(r);
+            }
+        }
+        // ---- across the team -------------------------------------------------------------------------------------------
+        acc mr = lanes_reduce<LEAD>(m, OpMax());
+        z = lanes_reduce<LEAD>(z * exp_scaled(a, m - mr), OpSum());
+        double zr = (double)z;
+        if constexpr (NT > 64) {
+            if ((tid & 63) == 0) { share[tid >> 6] = (double)mr; share[WAVES + (tid >> 6)] = zr; }
+            __syncthreads();
+            if (lead) {
+                // every block of WAVES lanes reduces the same numbers: all lanes have the result
+                const double mw = share[tid & (WAVES - 1)], all = lanes_reduce<WAVES>(mw, OpMax());
+                zr = lanes_reduce<WAVES>(share[WAVES + (tid & (WAVES - 1))] * exp_of((mw - all) * a.inv_tau), OpSum());
+                mr = (acc)all;
+            }
+        }
 
-    // ---- the row's numbers -----------------------------------------------------------------------------------------
-    double top2[2] = {(double)m, -INFINITY};
-    for (int k = tid; k < a.K; k += NT) if (cls[k] >= 0) top2[1] = xtop[k] > top2[1] ? xtop[k] : top2[1];
-    row_max<NT>(top2, scratch);
-    const double mr = top2[0], M = mr > top2[1] ? mr : top2[1];
-    double s3[3] = {(double)z * exp(((double)m - mr) * a.inv_tau), 0.0, 0.0};     // rest (on mr), top (on M), sum p
-    for (int k = tid; k < a.K; k += NT) if (cls[k] >= 0) {
-        s3[1] += exp((xtop[k] - M) * a.inv_tau);
-        s3[2] += exp(logp[k] - zt);
-    }
-    row_sum<NT>(s3, scratch);
-    const double logz = log(s3[0] * exp((mr - M) * a.inv_tau) + s3[1]);           // on M
-    const bool rest = a.lse != nullptr && some_rest;
-    double pr = 0.0;
-    const double lqr = (mr - M) * a.inv_tau + log(s3[0]) - logz, qr = some_rest ? exp(lqr) : 0.0;
-    if (rest) {
-        pr = 1.0 - s3[2];
-        pr = pr < 0.0 ? 0.0 : pr;
-    }
-    double kl[1] = {0.0};
-    for (int k = tid; k < a.K; k += NT) if (cls[k] >= 0) {
-        const double lp = logp[k] - zt, lq = (xtop[k] - M) * a.inv_tau - logz;
-        const double weight = exp(a.reverse ? lq : lp);
-        if (weight != 0.0) kl[0] += a.reverse ? weight * (lq - lp) : weight * (lp - lq);
-    }
-    row_sum<NT>(kl, scratch);
-    // the rest's gradient is mass_r e_v / sum e over the rest, e_v = exp((s_v - m_r) / tau): q_v (1 - p_r / q_r) would be 0 times infinity
-    // where the student is sure of itself
-    double mass_r = qr;
-    if (a.reverse) {
-        const double lr = rest ? lqr - log(pr > a.floor_rest ? pr : a.floor_rest) : 0.0;
-        if (qr != 0.0) kl[0] += qr * lr;
-        mass_r = qr * (lr - kl[0]);
-    } else if (rest && pr > 0.0) {
-        kl[0] += pr * (log(pr) - lqr);
-        mass_r = qr - pr;
-    }
-    if (tid == 0) loss[row] = (acc)(a.tau * a.tau * w * kl[0]);
-    if (g == nullptr) return;
-
-    // ---- the gradient: the rest's coefficient everywhere, then the entries' own values over it ------------------------
-    const acc coef = (acc)(s3[0] == 0.0 ? 0.0 : a.tau * w * mass_r / s3[0]), mm = (acc)mr;
-    for (int u = tid; u < nvec; u += NT) {
-        const auto r = Vec<T>::load(x + (size_t)u * VN);
-        typename Vec<T>::raw o;
+        // ---- the row's numbers -----------------------------------------------------------------------------------------
+        double log_z = 0.0, kl = 0.0, coef = 0.0, psum = 1.0;        // log_z on xref
+        if (lead && todo == ROW_COMPUTE) {
+            const double far = ((double)mr - xref) * a.inv_tau, log_zr = log_of(zr);
+            const bool rest = a.lse != nullptr && some_rest;
+            if (a.lse == nullptr) {
+                log_z = far + log_zr;
+                psum = sums[0];
+                kl = sums[1] / psum - log_of(psum) - sums[2] * a.inv_tau / psum + log_z;
+                coef = 1.0 / zr;
+            } else {
+                log_z = far > 0.0 ? far + log_of(zr + sums[3] * exp_of(-far)) : log_of(zr * exp_of(far) + sums[3]);
+                const double lqr = far + log_zr - log_z, qr = some_rest ? exp_of(lqr) : 0.0;
+                double pr = rest ? 1.0 - sums[0] : 0.0, mass = qr;
+                pr = pr < 0.0 ? 0.0 : pr;
+                if (a.reverse) {
+                    const double scale = exp_of(-log_z), lr = rest ? lqr - log_of(pr > a.floor_rest ? pr : a.floor_rest) : 0.0;
+                    kl = scale != 0.0 ? scale * (sums[4] * a.inv_tau - sums[5] - sums[3] * log_z) : 0.0;
+                    if (qr != 0.0) kl += qr * lr;
+                    mass = qr != 0.0 ? qr * (lr - kl) : 0.0;
+                } else {
+                    kl = sums[1] - sums[2] * a.inv_tau + sums[0] * log_z;
+                    if (pr > 0.0) { kl += pr * (log_of(pr) - lqr); mass = qr - pr; }
+                }
+                // mass e_v / sum e on the rest, e_v = exp((s_v - m_r) / tau): q_v (1 - p_r / q_r) would be 0 times infinity where the student is
+                // sure of itself
+                coef = zr == 0.0 ? 0.0 : mass / zr;
+            }
+            coef *= a.tau * w;
+        }
+        if (tid == 0) static_cast<acc*>(a.loss)[row] = todo == ROW_COMPUTE ? (acc)(a.tau * a.tau * w * kl) : todo == ROW_ZERO ? (acc)0 : (acc)NAN;
+        if (g != nullptr) {
+            if constexpr (NT > 64) {
+                if (tid == 0) { share[WAVES * 2 + 1] = coef; share[WAVES * 2 + 2] = (double)mr; }
+                __syncthreads();
+                coef = share[WAVES * 2 + 1]; mr = (acc)share[WAVES * 2 + 2];
+            }
+            // ---- the gradient: the rest's coefficient everywhere, then the entries' own values over it ------------------------
+            const acc cf = (acc)coef, fill = todo == ROW_NAN ? (acc)NAN : (acc)0;
+            auto put = [&](const raw& r, int u) {
+                raw o;
 #pragma unroll
-        for (int i = 0; i < VN; ++i) o[i] = (T)(coef * exp_scaled(a, (acc)r[i] - mm));
-        Vec<T>::store(g + (size_t)u * VN, o);
-    }
-    if (nvec * VN + tid < a.V && tid < VN) g[nvec * VN + tid] = (T)(coef * exp_scaled(a, (acc)x[nvec * VN + tid] - mm));
-    row_sync<NT>();
-    for (int k = tid; k < a.K; k += NT) if (cls[k] >= 0) {
-        const double lp = logp[k] - zt, lq = (xtop[k] - M) * a.inv_tau - logz, q = exp(lq);
-        const double d = a.reverse ? (q != 0.0 ? q * (lq - lp - kl[0]) : 0.0) : q - exp(lp);
-        g[cls[k]] = (T)(acc)(a.tau * w * d);
+                for (int j = 0; j < VN; ++j) o[j] = (T)(todo == ROW_COMPUTE ? cf * exp_gradient<T>(a, (acc)r[j] - mr) : fill);
+                Vec<T>::store(g + (size_t)u * VN, o);
+            };
+            if (NV > 0) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int u = i * NT + at;
+                    if (u < nvec) put(__builtin_bit_cast(raw, data[i]), u);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
+                for (int u = tid; u < nvec; u += NT) {
+                    raw r = {};
+                    if (todo == ROW_COMPUTE) r = Vec<T>::load(x + (size_t)u * VN);
+                    put(r, u);
+                }
+            }
+            if (tid < tail) g[nvec * VN + tid] = (T)(todo == ROW_COMPUTE ? cf * exp_gradient<T>(a, last - mr) : fill);
+            team_sync();
+            if (lead && todo == ROW_COMPUTE) {
+                const double scale = exp_of(-log_z), ip = 1.0 / psum;
+                for (int k = tid; k < a.K; k += LEAD) if (cls[k] >= 0) {
+                    const double q = ek[k] * scale;
+                    const double d = a.reverse ? (q != 0.0 ? q * (log_of(ek[k]) - log_z - tk[k] - kl) : 0.0) : q - pk[k] * ip;
+                    g[cls[k]] = (T)(acc)(a.tau * w * d);
+                }
+            }
+        }
+        // the bits back to 0 for the next row (a padded or wrong index has set none)
+        if (lead && row + (int64_t)gridDim.x * ROWS < a.n && w != 0.0) {
+            wave_sync();
+            for (int k = tid; k < a.K; k += LEAD) {
+                const int64_t c = a.index_64 ? static_cast<const int64_t*>(a.index)[row * a.ld_index + k] : static_cast<const int32_t*>(a.index)[row * a.ld_index + k];
+                if (c >= 0 && c < a.V) bits[c >> 5] = 0;
+            }
+        }
+        team_sync();
     }
 }
 
@@ -275,10 +341,10 @@ static int distill_check(const oak_distill_args* a) {
     return OAK_OK;
 }
 
-template <typename T, int NT> static int distill_run(hipStream_t stream, const DistillDev& d) {
+template <typename T, int NT, int NV> static int distill_run(hipStream_t stream, const DistillDev& d) {
     constexpr int ROWS = NT < 256 ? 256 / NT : 1;
-    const size_t lds = (distill_lds(d.V, d.K, NT)) * ROWS;
-    auto kernel = distill_kernel<T, NT>;
+    const size_t lds = distill_lds(d.V, d.K, NT) * ROWS;
+    auto kernel = distill_kernel<T, NT, NV>;
     if (lds > 64 * 1024) OAK_CHECK(ensure_dynamic_lds((const void*)kernel, 160 * 1024));
     return launch(kernel, dim3((unsigned)((d.n + ROWS - 1) / ROWS)), dim3(NT < 256 ? 256 : NT), lds, stream, d);
 }
@@ -297,8 +363,13 @@ static int distill_launch(hipStream_t stream, const oak_distill_args* a) {
     d.logits = a->logits; d.top = a->top; d.index = a->index; d.lse = a->top_lse; d.weight = a->row_weight; d.loss = a->loss; d.dlogits = a->dlogits;
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        if (d.V <= 1024 && d.K <= 256) return distill_run<T, 64>(stream, d);
-        return distill_run<T, 256>(stream, d);
+        const int units = (d.V + Vec<T>::N - 1) / Vec<T>::N;
+        if (units <= 64 && d.K <= 64) return distill_run<T, 16, 4>(stream, d);
+        if (units <= 256 && d.K <= 64) return distill_run<T, 16, 16>(stream, d);
+        if (units <= 1024 && d.K <= 256) return distill_run<T, 64, 16>(stream, d);
+        if (units <= 4096) return distill_run<T, 256, 16>(stream, d);
+        if (units <= 16384) return distill_run<T, 1024, 16>(stream, d);
+        return distill_run<T, 1024, 0>(stream, d);
     });
 }
 

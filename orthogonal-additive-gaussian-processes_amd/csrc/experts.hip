@@ -73,35 +73,6 @@ template <int VPL> __device__ __forceinline__ void load_scores(const RouteDev& a
 }
 template <typename A> __device__ __forceinline__ A score_at(const RouteDev& a, int64_t row, int e) { return (A)load_any(a.scores, a.dtype, row * a.ld + e); }
 
-// 2^y in the accuracy of A; exp(t) = 2^(t log2 e), the float form with log2 e in two parts (both positive: t = -inf gives 0)
-__device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(__builtin_fmaf(t, 1.44269502162933349609f, t * 1.92596299112661e-8f)); }
-// Cody-Waite reduction and the Taylor polynomial of degree 12 on |r| <= ln 2 / 2 (remainder 1.7e-16), without the special cases of exp()
-__device__ __forceinline__ double exp_of(double t) {
-    t = t > -800.0 ? t : -800.0;
-    const double n = __builtin_rint(t * 1.4426950408889634074);
-    const double r = __builtin_fma(n, -1.9082149292705877e-10, __builtin_fma(n, -6.93147180369123816490e-01, t));
-    double p = 1.0 / 479001600.0;
-    p = __builtin_fma(p, r, 1.0 / 39916800.0);
-    p = __builtin_fma(p, r, 1.0 / 3628800.0);
-    p = __builtin_fma(p, r, 1.0 / 362880.0);
-    p = __builtin_fma(p, r, 1.0 / 40320.0);
-    p = __builtin_fma(p, r, 1.0 / 5040.0);
-    p = __builtin_fma(p, r, 1.0 / 720.0);
-    p = __builtin_fma(p, r, 1.0 / 120.0);
-    p = __builtin_fma(p, r, 1.0 / 24.0);
-    p = __builtin_fma(p, r, 1.0 / 6.0);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
-    return __builtin_ldexp(p, (int)n);
-}
-// 1 / d for normal d: the reciprocal's estimate and two Newton steps
-__device__ __forceinline__ double inverse(double d) {
-    double r = __builtin_amdgcn_rcp(d);
-    r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
-    return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
-}
-__device__ __forceinline__ float inverse(float d) { return 1.0f / d; }
 // sigmoid; far below 0 (|x| > 700) what is left is 1e-304
 __device__ __forceinline__ double sigmoid_of(double x) { return inverse(1.0 + exp_of(x < -700.0 ? 700.0 : -x)); }
 

@@ -91,6 +91,63 @@ template <int L, typename Op, typename A> __device__ __forceinline__ A lanes_red
     return v;
 }
 
+// exp(t), the float form as 2^(t log2 e) with log2 e in two parts (both positive: t = -inf gives 0)
+__device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(__builtin_fmaf(t, 1.44269502162933349609f, t * 1.92596299112661e-8f)); }
+// a b + c with c a constant of the code, read from scalar registers.  The compiler would rather have the constant in vector registers, where a
+// polynomial's constants cost either a move per step or two registers each for as long as a loop lasts.
+__device__ __forceinline__ double fma_const(double a, double b, double c) {
+    double d;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+    return d;
+}
+// Cody-Waite reduction and the Taylor polynomial of degree 12 on |r| <= ln 2 / 2 (remainder 1.7e-16), without the special cases of exp();
+// for t < 709, NaN stays NaN
+__device__ __forceinline__ double exp_of(double t) {
+    t = t < -800.0 ? -800.0 : t;
+    const double n = __builtin_rint(t * 1.4426950408889634074);
+    const double r = __builtin_fma(n, -1.9082149292705877e-10, __builtin_fma(n, -6.93147180369123816490e-01, t));
+    double p = fma_const(r, 1.0 / 479001600.0, 1.0 / 39916800.0);
+    p = fma_const(p, r, 1.0 / 3628800.0);
+    p = fma_const(p, r, 1.0 / 362880.0);
+    p = fma_const(p, r, 1.0 / 40320.0);
+    p = fma_const(p, r, 1.0 / 5040.0);
+    p = fma_const(p, r, 1.0 / 720.0);
+    p = fma_const(p, r, 1.0 / 120.0);
+    p = fma_const(p, r, 1.0 / 24.0);
+    p = fma_const(p, r, 1.0 / 6.0);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    return __builtin_ldexp(p, (int)n);
+}
+// 1 / d for normal d: the reciprocal's estimate and two Newton steps
+__device__ __forceinline__ double inverse(double d) {
+    double r = __builtin_amdgcn_rcp(d);
+    r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+    return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+}
+__device__ __forceinline__ float inverse(float d) { return 1.0f / d; }
+// log x for x >= 0 (log 0 = -inf, NaN stays NaN): x = 2^n m, m in [1/sqrt 2, sqrt 2), log m = 2 atanh f, f = (m - 1) / (m + 1), |f| < 0.172,
+// by its series to f^21 (remainder 2e-18)
+__device__ __forceinline__ double log_of(double x) {
+    double m = __builtin_amdgcn_frexp_mant(x);
+    int n = __builtin_amdgcn_frexp_exp(x);
+    if (m < 0.70710678118654752440) { m *= 2.0; n -= 1; }
+    const double f = (m - 1.0) * inverse(m + 1.0), s = f * f;
+    double p = fma_const(s, 1.0 / 21.0, 1.0 / 19.0);
+    p = fma_const(p, s, 1.0 / 17.0);
+    p = fma_const(p, s, 1.0 / 15.0);
+    p = fma_const(p, s, 1.0 / 13.0);
+    p = fma_const(p, s, 1.0 / 11.0);
+    p = fma_const(p, s, 1.0 / 9.0);
+    p = fma_const(p, s, 1.0 / 7.0);
+    p = fma_const(p, s, 1.0 / 5.0);
+    p = fma_const(p, s, 1.0 / 3.0);
+    const double two_f = f + f;
+    const double r = __builtin_fma((double)n, 6.93147180369123816490e-01, __builtin_fma((double)n, 1.9082149292705877e-10, __builtin_fma(two_f * s, p, two_f)));
+    return x == 0.0 ? -INFINITY : r;
+}
+
 // order of LDS accesses between the lanes of one wave (no other wave is waited for)
 __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
