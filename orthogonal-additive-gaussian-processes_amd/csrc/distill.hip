@@ -12,7 +12,7 @@
 // and per row in 64.
 //
 // A row stays in the registers of its team of NT threads, NV units of 16 bytes each, so that it is read once: the sum and the gradient
-// each walk the registers.  The team's first wave (all of a team of 16 or 64) does what concerns the entries.  Every sum over the entries is taken on
+// each walk the registers (NV = 0: rows too long for that are read twice).  The team's first wave (all of a smaller team) does what concerns the entries.  Every sum over the entries is taken on
 // references known before the pass over the classes (the entries' own maximum), so that only one reduction per row waits for that pass.
 #include "lowp.h"
 
@@ -214,10 +214,16 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillDev
 #pragma unroll
                     for (int j = 0; j < VN; ++j) z += exp_scaled(a, (acc)r[j] - m);
                 };
-                for (int u = tid; u < nvec; u += NT) {
-                    raw r = Vec<T>::load(x + (size_t)u * VN);
-                    if (leave_out) hide(r, u);
-                    take(r);
+                constexpr int U = 4;
+                for (int u0 = tid; u0 < nvec; u0 += U * NT) {
+                    raw r[U];
+#pragma unroll
+                    for (int i = 0; i < U; ++i) { const int u = u0 + i * NT; r[i] = Vec<T>::load(x + (size_t)(u < nvec ? u : nvec - 1) * VN); }
+#pragma unroll
+                    for (int i = 0; i < U; ++i) {
+                        const int u = u0 + i * NT;
+                        if (u < nvec) { if (leave_out) hide(r[i], u); take(r[i]); }
+                    }
                 }
                 raw r;
 #pragma unroll
@@ -284,7 +290,9 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillDev
                 raw o;
 #pragma unroll
                 for (int j = 0; j < VN; ++j) o[j] = (T)(todo == ROW_COMPUTE ? cf * exp_gradient<T>(a, (acc)r[j] - mr) : fill);
-                Vec<T>::store(g + (size_t)u * VN, o);
+                // a long row's gradient passes the caches by (16384 x 8192 bf16: 140 us, otherwise 158); short rows end inside a cache line, which
+                // the next row fills there (262144 x 1000 float32: 430 us, otherwise 510)
+                if constexpr (NV == 0 || NT * NV >= 1024) Vec<T>::store_stream(g + (size_t)u * VN, o); else Vec<T>::store(g + (size_t)u * VN, o);
             };
             if (NV > 0) {
 #pragma unroll
@@ -294,10 +302,15 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillDev
                     __builtin_amdgcn_sched_barrier(0);
                 }
             } else {
-                for (int u = tid; u < nvec; u += NT) {
-                    raw r = {};
-                    if (todo == ROW_COMPUTE) r = Vec<T>::load(x + (size_t)u * VN);
-                    put(r, u);
+                constexpr int U = 4;
+                for (int u0 = tid; u0 < nvec; u0 += U * NT) {
+                    raw r[U] = {};
+                    if (todo == ROW_COMPUTE) {
+#pragma unroll
+                        for (int i = 0; i < U; ++i) { const int u = u0 + i * NT; r[i] = Vec<T>::load(x + (size_t)(u < nvec ? u : nvec - 1) * VN); }
+                    }
+#pragma unroll
+                    for (int i = 0; i < U; ++i) { const int u = u0 + i * NT; if (u < nvec) put(r[i], u); }
                 }
             }
             if (tid < tail) g[nvec * VN + tid] = (T)(todo == ROW_COMPUTE ? cf * exp_gradient<T>(a, last - mr) : fill);
@@ -364,12 +377,22 @@ static int distill_launch(hipStream_t stream, const oak_distill_args* a) {
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
         const int units = (d.V + Vec<T>::N - 1) / Vec<T>::N;
+        // the smallest team whose registers hold the row; few rows, with compute units to spare, are faster with many threads each
+        // (8 rows of 32768 bf16: 11.4 us with 512 threads that read the row twice, 13.1 with 256 that hold it)
+        if (d.n <= 256 && units > 64) return distill_run<T, 512, 0>(stream, d);
+        if (units <= 16 && d.K <= 16) return distill_run<T, 4, 4>(stream, d);
         if (units <= 64 && d.K <= 64) return distill_run<T, 16, 4>(stream, d);
-        if (units <= 256 && d.K <= 64) return distill_run<T, 16, 16>(stream, d);
-        if (units <= 1024 && d.K <= 256) return distill_run<T, 64, 16>(stream, d);
-        if (units <= 4096) return distill_run<T, 256, 16>(stream, d);
-        if (units <= 16384) return distill_run<T, 1024, 16>(stream, d);
-        return distill_run<T, 1024, 0>(stream, d);
+        if (units <= 128 && d.K <= 64) return distill_run<T, 16, 8>(stream, d);
+        if (units <= 256 && d.K <= 32) return distill_run<T, 16, 16>(stream, d);       // 65536 x 1000 float32: k = 10 120 us, with 64 threads 138;
+        if (units <= 256) return distill_run<T, 64, 4>(stream, d);                     //   k = 64 237 us, with 64 threads 174
+        if (units <= 512) return distill_run<T, 64, 8>(stream, d);
+        if (units <= 1024) return distill_run<T, 64, 16>(stream, d);
+        if (units <= 2048) return distill_run<T, 256, 8>(stream, d);
+        if (units <= 4096) return distill_run<T, 256, 16>(stream, d);                  // 4096 x 32768 bf16: 119 us, read twice 146
+        // longer rows are read twice, the second time out of the last cache: two workgroups a compute unit keep 2 x 256 rows in flight, which it
+        // holds up to 2^18 bf16 classes, and the gradient passes it by (2048 x 131072 bf16: 272 us; a row in the registers of 1024 threads,
+        // one workgroup a unit: 330)
+        return distill_run<T, 512, 0>(stream, d);
     });
 }
 
