@@ -12,7 +12,8 @@
 // and per row in 64.
 //
 // A row stays in the registers of its team of NT threads, NV units of 16 bytes each, so that it is read once: the sum and the gradient
-// each walk the registers (NV = 0: rows too long for that are read twice).  The team's first wave (all of a smaller team) does what concerns the entries.  Every sum over the entries is taken on
+// each walk the registers (LONG: what does not fit is read twice).  The team's first wave (all of a smaller team) does what concerns the entries.
+// Every sum over the entries is taken on
 // references known before the pass over the classes (the entries' own maximum), so that only one reduction per row waits for that pass.
 #include "lowp.h"
 
@@ -45,8 +46,8 @@ __host__ __device__ inline size_t distill_lds(int V, int K, int NT) {
 // what the team does with its row's gradient
 enum { ROW_COMPUTE = 0, ROW_ZERO = 1, ROW_NAN = 2 };
 
-template <typename T, int NT, int NV>
-__global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillDev a) {
+template <typename T, int NT, int NV, bool LONG>
+__global__ void __launch_bounds__(NT < 256 ? 256 : NT, LONG ? 4 : 1) distill_kernel(DistillDev a) {
     using acc = typename Num<T>::acc;
     using raw = typename Vec<T>::raw;
     constexpr int VN = Vec<T>::N, ROWS = NT < 256 ? 256 / NT : 1, LEAD = NT < 64 ? NT : 64, WAVES = NT / 64;
@@ -81,10 +82,10 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillDev
         forget_place();
         // ---- the row into registers; units behind its end are read from inside it and not used -----------------------------
         typedef int words4 __attribute__((ext_vector_type(4)));
-        words4 data[NV > 0 ? NV : 1];
+        words4 data[NV];
         acc last = -INFINITY;                          // one of the elements that do not fill a unit
         if (todo == ROW_COMPUTE) {
-            if (NV > 0 && nvec > 0) {
+            if (nvec > 0) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     const int u = i * NT + at;
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillDev
                 }
             };
             if (leave_out && tid < tail && (bits[(nvec * VN + tid) >> 5] >> ((nvec * VN + tid) & 31) & 1)) last = -INFINITY;
-            if constexpr (NV > 0) {
+            {
                 forget_place();
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
@@ -204,7 +205,8 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillDev
                 }
                 z += exp_scaled(a, last - m);
                 forget();
-            } else {
+            }
+            if constexpr (LONG) {
                 auto take = [&](raw r) {
                     acc top = m;
 #pragma unroll
@@ -215,7 +217,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillDev
                     for (int j = 0; j < VN; ++j) z += exp_scaled(a, (acc)r[j] - m);
                 };
                 constexpr int U = 4;
-                for (int u0 = tid; u0 < nvec; u0 += U * NT) {
+                for (int u0 = NV * NT + tid; u0 < nvec; u0 += U * NT) {
                     raw r[U];
 #pragma unroll
                     for (int i = 0; i < U; ++i) { const int u = u0 + i * NT; r[i] = Vec<T>::load(x + (size_t)(u < nvec ? u : nvec - 1) * VN); }
@@ -225,11 +227,6 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillDev
                         if (u < nvec) { if (leave_out) hide(r[i], u); take(r[i]); }
                     }
                 }
-                raw r;
-#pragma unroll
-                for (int j = 0; j < VN; ++j) r[j] = (T)-INFINITY;
-                r[0] = (T)last;
-                take(r);
             }
         }
         // ---- across the team -------------------------------------------------------------------------------------------
@@ -292,18 +289,19 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) distill_kernel(DistillDev
                 for (int j = 0; j < VN; ++j) o[j] = (T)(todo == ROW_COMPUTE ? cf * exp_gradient<T>(a, (acc)r[j] - mr) : fill);
                 // a long row's gradient passes the caches by (16384 x 8192 bf16: 140 us, otherwise 158); short rows end inside a cache line, which
                 // the next row fills there (262144 x 1000 float32: 430 us, otherwise 510)
-                if constexpr (NV == 0 || NT * NV >= 1024) Vec<T>::store_stream(g + (size_t)u * VN, o); else Vec<T>::store(g + (size_t)u * VN, o);
+                if constexpr (LONG || NT * NV >= 1024) Vec<T>::store_stream(g + (size_t)u * VN, o); else Vec<T>::store(g + (size_t)u * VN, o);
             };
-            if (NV > 0) {
+            {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     const int u = i * NT + at;
                     if (u < nvec) put(__builtin_bit_cast(raw, data[i]), u);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-            } else {
+            }
+            if constexpr (LONG) {
                 constexpr int U = 4;
-                for (int u0 = tid; u0 < nvec; u0 += U * NT) {
+                for (int u0 = NV * NT + tid; u0 < nvec; u0 += U * NT) {
                     raw r[U] = {};
                     if (todo == ROW_COMPUTE) {
 #pragma unroll
@@ -354,10 +352,10 @@ static int distill_check(const oak_distill_args* a) {
     return OAK_OK;
 }
 
-template <typename T, int NT, int NV> static int distill_run(hipStream_t stream, const DistillDev& d) {
+template <typename T, int NT, int NV, bool LONG = false> static int distill_run(hipStream_t stream, const DistillDev& d) {
     constexpr int ROWS = NT < 256 ? 256 / NT : 1;
     const size_t lds = distill_lds(d.V, d.K, NT) * ROWS;
-    auto kernel = distill_kernel<T, NT, NV>;
+    auto kernel = distill_kernel<T, NT, NV, LONG>;
     if (lds > 64 * 1024) OAK_CHECK(ensure_dynamic_lds((const void*)kernel, 160 * 1024));
     return launch(kernel, dim3((unsigned)((d.n + ROWS - 1) / ROWS)), dim3(NT < 256 ? 256 : NT), lds, stream, d);
 }
@@ -378,8 +376,8 @@ static int distill_launch(hipStream_t stream, const oak_distill_args* a) {
         using T = decltype(t);
         const int units = (d.V + Vec<T>::N - 1) / Vec<T>::N;
         // the smallest team whose registers hold the row; few rows, with compute units to spare, are faster with many threads each
-        // (8 rows of 32768 bf16: 11.4 us with 512 threads that read the row twice, 13.1 with 256 that hold it)
-        if (d.n <= 256 && units > 64) return distill_run<T, 512, 0>(stream, d);
+        // (8 rows of 32768 bf16: 11.2 us with 512 threads, 13.1 with 256)
+        if (d.n <= 256 && units > 64) return distill_run<T, 512, 8, true>(stream, d);
         if (units <= 16 && d.K <= 16) return distill_run<T, 4, 4>(stream, d);
         if (units <= 64 && d.K <= 64) return distill_run<T, 16, 4>(stream, d);
         if (units <= 128 && d.K <= 64) return distill_run<T, 16, 8>(stream, d);
@@ -389,10 +387,10 @@ static int distill_launch(hipStream_t stream, const oak_distill_args* a) {
         if (units <= 1024) return distill_run<T, 64, 16>(stream, d);
         if (units <= 2048) return distill_run<T, 256, 8>(stream, d);
         if (units <= 4096) return distill_run<T, 256, 16>(stream, d);                  // 4096 x 32768 bf16: 119 us, read twice 146
-        // longer rows are read twice, the second time out of the last cache: two workgroups a compute unit keep 2 x 256 rows in flight, which it
-        // holds up to 2^18 bf16 classes, and the gradient passes it by (2048 x 131072 bf16: 272 us; a row in the registers of 1024 threads,
-        // one workgroup a unit: 330)
-        return distill_run<T, 512, 0>(stream, d);
+        // Longer rows: what 512 threads can hold with two workgroups a compute unit, the rest is read twice, the second time out of the last cache
+        // (2 x 256 rows in flight fit it up to 2^18 bf16 classes, and the gradient passes it by).  2048 x 131072 bf16: 265 us; all of it
+        // read twice 279; the whole row in the registers of 1024 threads, one workgroup a unit, 330.
+        return distill_run<T, 512, 8, true>(stream, d);
     });
 }
 
