@@ -512,6 +512,9 @@ static int route_grad_launch(hipStream_t stream, const oak_route_args* a) {
 // Every wave owns one consecutive piece of the slots, so that the order inside an expert is the slots' own without any atomic
 // whose order could show: pieces are counted, the counts are summed in piece order, and each wave then places its slots 64 at a
 // time -- a slot's rank among the 64 is the number of lower lanes with the same expert (one ballot per bit of the expert's number).
+constexpr int64_t PLAN_SMALL_SLOTS = 16384;
+constexpr int PLAN_MAX_PIECES = 2048;
+
 struct PlanDev {
     int64_t slots, piece;
     int k, E, npieces, bits;
@@ -597,21 +600,24 @@ __global__ void __launch_bounds__(256) plan_count_kernel(PlanDev a) {
     if (piece < a.npieces) for (int e = lane; e < a.E; e += 64) a.ws[(int64_t)e * a.npieces + piece] = mine[e];
 }
 
-// one wave per expert: counts of its pieces -> what lies before each piece
+// one workgroup per expert: counts of its pieces -> what lies before each piece
 __global__ void __launch_bounds__(256) plan_scan_kernel(PlanDev a) {
-    const int e = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (e >= a.E) return;
+    __shared__ int wsum[4];
+    const int e = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     int* col = a.ws + (int64_t)e * a.npieces;
-    int before = 0;
-    for (int p0 = 0; p0 < a.npieces; p0 += 64) {
-        const int p = p0 + lane;
-        const int c = p < a.npieces ? col[p] : 0;
-        int incl = c;
-        for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
-        if (p < a.npieces) col[p] = before + incl - c;
-        before += __shfl(incl, 63, 64);
-    }
-    if (lane == 0) a.counts[e] = before;
+    constexpr int PER = PLAN_MAX_PIECES / 256;
+    int c[PER], mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) { c[i] = tid * PER + i < a.npieces ? col[tid * PER + i] : 0; mine += c[i]; }
+    int incl = mine;
+    for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
+    if (lane == 63) wsum[wave] = incl;
+    __syncthreads();
+    int before = incl - mine;
+    for (int w = 0; w < wave; ++w) before += wsum[w];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) { if (tid * PER + i < a.npieces) col[tid * PER + i] = before; before += c[i]; }
+    if (tid == 255) a.counts[e] = before;
 }
 
 __global__ void __launch_bounds__(256) plan_place_kernel(PlanDev a) {
@@ -646,12 +652,10 @@ __global__ void __launch_bounds__(256) plan_place_kernel(PlanDev a) {
     }
 }
 
-constexpr int64_t PLAN_SMALL_SLOTS = 16384;
-constexpr int PLAN_MAX_PIECES = 2048;
-
 static void plan_pieces(int64_t slots, int E, int64_t* piece, int* npieces, bool* small) {
     *small = slots <= PLAN_SMALL_SLOTS && E <= 1024;
-    const int want = *small ? 16 : PLAN_MAX_PIECES;
+    // 8 waves a compute unit; with many experts fewer, so that the table of counts stays within 2^20 integers
+    const int want = *small ? 16 : E <= 512 ? PLAN_MAX_PIECES : (1 << 20) / E;
     int64_t p = (slots + want - 1) / want;
     const int64_t least = *small ? 64 : 256;
     p = p < least ? least : (p + 63) / 64 * 64;
@@ -687,19 +691,20 @@ static int plan_launch(hipStream_t stream, const oak_plan_args* a) {
         OAK_CHECK(ensure_dynamic_lds((const void*)plan_place_kernel, 128 * 1024));
     }
     OAK_CHECK(launch(plan_count_kernel, dim3(wgs), dim3(256), (size_t)4 * d.E * sizeof(int), stream, d));
-    OAK_CHECK(launch(plan_scan_kernel, dim3((unsigned)((d.E + 3) / 4)), dim3(256), 0, stream, d));
+    OAK_CHECK(launch(plan_scan_kernel, dim3((unsigned)d.E), dim3(256), 0, stream, d));
     return launch(plan_place_kernel, dim3(wgs), dim3(256), lds, stream, d);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // dispatch, combine and their gradients
 // ---------------------------------------------------------------------------------------------------------------------
-// All of them walk rows: a row is read or written once where the slots' order would touch it k times.  TPR threads share a row; a
-// unit is 16 bytes, the row's last elements that do not fill one are units of their own.
+// All of them walk rows: a row is read or written once where the slots' order would touch it k times.  tpr threads share a row; a unit is
+// 16 bytes, the row's last elements that do not fill one are units of their own.  A thread asks for the places, then for the answers of up
+// to 4 slots before it adds the first.  Bound by memory: 32768 rows, k = 6, 2048 bf16 columns at MIX_RATES.
 struct MixDev {
     int64_t n, slots, ld_rows, ld_slots, ld_grad;
     int64_t units;              // 16-byte units of a row, then its last elements
-    int C, k, nvec, E, tpr_log2;
+    int C, k, nvec, E, tpr, inv_tpr, rows_per_wg, tpr_log2;
     const int* positions; const int* offsets; const void* weights;
     const void* src; void* dst; const void* dout; void* dslots; void* dweights;
 };
@@ -715,14 +720,22 @@ __device__ __forceinline__ int64_t place_of(const MixDev& a, int64_t n, int j) {
     return p >= 0 && p < a.slots ? p : -1;
 }
 
+// row and first unit of this thread: 256 / tpr rows a workgroup, the threads left over have none (-1)
+__device__ __forceinline__ int64_t mix_row(const MixDev& a, int* unit) {
+    const int r = (int)(((unsigned)threadIdx.x * (unsigned)a.inv_tpr) >> 16);
+    *unit = (int)threadIdx.x - r * a.tpr;
+    const int64_t n = (int64_t)blockIdx.x * a.rows_per_wg + r;
+    return r < a.rows_per_wg && n < a.n ? n : -1;
+}
+
 template <typename T> __global__ void __launch_bounds__(256) dispatch_kernel(MixDev a) {
-    const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x, n = g >> a.tpr_log2;
-    const int tpr = 1 << a.tpr_log2, t = (int)(g & (tpr - 1));
-    if (n >= a.n) return;
+    int t;
+    const int64_t n = mix_row(a, &t);
+    if (n < 0) return;
     const T* src = static_cast<const T*>(a.src) + n * a.ld_rows;
     T* dst = static_cast<T*>(a.dst);
     const int used = a.offsets[a.E];
-    for (int64_t u = t; u < a.units; u += tpr) {
+    for (int64_t u = t; u < a.units; u += a.tpr) {
         if (u < a.nvec) {
             const auto v = Vec<T>::load(src + u * Vec<T>::N);
             for (int j = 0; j < a.k; ++j) { const int64_t p = place_of(a, n, j); if (p >= 0) Vec<T>::store(dst + p * a.ld_slots + u * Vec<T>::N, v); }
@@ -731,47 +744,50 @@ template <typename T> __global__ void __launch_bounds__(256) dispatch_kernel(Mix
             const T v = src[c];
             for (int j = 0; j < a.k; ++j) { const int64_t p = place_of(a, n, j); if (p >= 0) dst[p * a.ld_slots + c] = v; }
         }
-        for (int j = 0; j < a.k; ++j) if (n * a.k + j >= used) zero_unit<T>(a, dst + (n * a.k + j) * a.ld_slots, u);
+        if (n * a.k + a.k > used)
+            for (int j = 0; j < a.k; ++j) if (n * a.k + j >= used) zero_unit<T>(a, dst + (n * a.k + j) * a.ld_slots, u);
     }
 }
 
-template <typename T> __global__ void __launch_bounds__(256) combine_kernel(MixDev a) {
+template <typename T, int CHUNK> __global__ void __launch_bounds__(256) combine_kernel(MixDev a) {
     using acc = typename Num<T>::acc;
-    const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x, n = g >> a.tpr_log2;
-    const int tpr = 1 << a.tpr_log2, t = (int)(g & (tpr - 1));
-    if (n >= a.n) return;
+    int t;
+    const int64_t n = mix_row(a, &t);
+    if (n < 0) return;
     const T* src = static_cast<const T*>(a.src);
     T* dst = static_cast<T*>(a.dst) + n * a.ld_rows;
     const acc* w = static_cast<const acc*>(a.weights);
-    for (int64_t u = t; u < a.units; u += tpr) {
-        if (u < a.nvec) {
-            acc y[Vec<T>::N] = {};
-            for (int j = 0; j < a.k; ++j) {
-                const int64_t p = place_of(a, n, j);
-                const acc wj = w ? w[n * a.k + j] : (acc)1;
-                if (p < 0) {                           // no expert: weight times nothing (a NaN weight still shows)
-                    if (w) for (int i = 0; i < Vec<T>::N; ++i) y[i] += wj * (acc)0;
-                    continue;
-                }
-                const auto f = Vec<T>::load(src + p * a.ld_slots + u * Vec<T>::N);
+    for (int64_t u = t; u < a.units; u += a.tpr) {
+        const bool whole = u < a.nvec;
+        const int64_t c = whole ? u * Vec<T>::N : a.nvec * (int64_t)Vec<T>::N + (u - a.nvec);
+        acc y[Vec<T>::N] = {};
+        for (int j0 = 0; j0 < a.k; j0 += CHUNK) {
+            int64_t p[CHUNK];
+            acc wj[CHUNK];
+            typename Vec<T>::raw f[CHUNK];
 #pragma unroll
-                for (int i = 0; i < Vec<T>::N; ++i) y[i] += wj * (acc)f[i];
+            for (int i = 0; i < CHUNK; ++i) {
+                p[i] = j0 + i < a.k ? place_of(a, n, j0 + i) : -1;
+                wj[i] = j0 + i < a.k && w ? w[n * a.k + j0 + i] : (acc)(j0 + i < a.k);
             }
+#pragma unroll
+            for (int i = 0; i < CHUNK; ++i) {
+                const T* at = src + p[i] * a.ld_slots + c;
+                f[i] = typename Vec<T>::raw{};
+                if (p[i] >= 0) { if (whole) f[i] = Vec<T>::load(at); else f[i][0] = *at; }
+            }
+            // no expert: the weight times nothing (a NaN weight still shows)
+#pragma unroll
+            for (int i = 0; i < CHUNK; ++i)
+#pragma unroll
+                for (int e = 0; e < Vec<T>::N; ++e) y[e] += wj[i] * (acc)f[i][e];
+        }
+        if (whole) {
             typename Vec<T>::raw o;
 #pragma unroll
-            for (int i = 0; i < Vec<T>::N; ++i) o[i] = (T)y[i];
-            Vec<T>::store(dst + u * Vec<T>::N, o);
-        } else {
-            const int64_t c = a.nvec * (int64_t)Vec<T>::N + (u - a.nvec);
-            acc y = 0;
-            for (int j = 0; j < a.k; ++j) {
-                const int64_t p = place_of(a, n, j);
-                const acc wj = w ? w[n * a.k + j] : (acc)1;
-                if (p >= 0) y += wj * (acc)src[p * a.ld_slots + c];
-                else if (w) y += wj * (acc)0;
-            }
-            dst[c] = (T)y;
-        }
+            for (int e = 0; e < Vec<T>::N; ++e) o[e] = (T)y[e];
+            Vec<T>::store(dst + c, o);
+        } else dst[c] = (T)y[0];
     }
 }
 
@@ -833,13 +849,15 @@ static int mix_launch(hipStream_t stream, const oak_mix_args* a, int what /* 0 d
     d.E = a->n_experts; d.nvec = d.C / vec; d.units = d.nvec + d.C % vec;
     d.positions = a->positions; d.offsets = a->offsets; d.weights = a->weights; d.src = a->src; d.dst = a->dst; d.dout = a->dout;
     d.dslots = a->dslots; d.dweights = a->dweights;
-    const int most = what == 2 ? 6 : 8;
-    while (d.tpr_log2 < most && ((int64_t)1 << d.tpr_log2) < d.units) ++d.tpr_log2;
-    const int64_t wgs = ((d.n << d.tpr_log2) + 255) / 256;
-    OAK_REQUIRE(wgs < ((int64_t)1 << 31), "mixture: %lld rows are too many for one launch", (long long)d.n);
+    // combine_grad: a power of two within a wave; the others: as many threads as the row has units
+    while (d.tpr_log2 < 6 && ((int64_t)1 << d.tpr_log2) < d.units) ++d.tpr_log2;
+    d.tpr = d.units < 256 ? (int)d.units : 256;
+    d.rows_per_wg = what == 2 ? 256 >> d.tpr_log2 : 256 / d.tpr;
+    d.inv_tpr = (65536 + d.tpr - 1) / d.tpr;           // t / tpr = t inv_tpr >> 16 for t < 256
+    const int64_t wgs = (d.n + d.rows_per_wg - 1) / d.rows_per_wg;
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        auto kernel = what == 0 ? dispatch_kernel<T> : what == 1 ? combine_kernel<T> : combine_grad_kernel<T>;
+        auto kernel = what == 0 ? dispatch_kernel<T> : what == 2 ? combine_grad_kernel<T> : d.k <= 2 ? combine_kernel<T, 2> : combine_kernel<T, 4>;
         return launch(kernel, dim3((unsigned)wgs), dim3(256), 0, stream, d);
     });
 }
