@@ -52,13 +52,13 @@ class Device:
 
     @property
     def stream(self) -> int:
-        return self.torch.cuda.current_stream(self.device).cuda_stream
+        # the handle alone: building a torch.cuda.Stream around it takes as long as a small kernel
+        raw = getattr(self.torch._C, "_cuda_getCurrentRawStream", None)
+        return raw(self.index) if raw is not None else self.torch.cuda.current_stream(self.device).cuda_stream
 
     def tensor(self, a, what: str):
-        if not on_device(a):
-            raise ValueError(f"{what} must be on {self.device} like the other arrays of the call")
-        if a.device != self.device:
-            raise ValueError(f"{what} is on {a.device}, the call runs on {self.device}")
+        if not on_device(a) or a.device != self.device:
+            raise ValueError(f"{what} must be on {self.device} like the first array of the call")
         if a.requires_grad and self.torch.is_grad_enabled():
             raise ValueError(f"{what} requires grad: the operators record no graph, their gradients are calls of their own; pass {what}.detach()")
         return a
