@@ -357,7 +357,9 @@ template <typename T, int NT, int NV, bool LONG = false> static int distill_run(
     const size_t lds = distill_lds(d.V, d.K, NT) * ROWS;
     auto kernel = distill_kernel<T, NT, NV, LONG>;
     if (lds > 64 * 1024) OAK_CHECK(ensure_dynamic_lds((const void*)kernel, 160 * 1024));
-    return launch(kernel, dim3((unsigned)((d.n + ROWS - 1) / ROWS)), dim3(NT < 256 ? 256 : NT), lds, stream, d);
+    // a launch has fewer than 2^32 threads; the kernel walks on from row to row
+    const int64_t wgs = (d.n + ROWS - 1) / ROWS, most = (int64_t)1 << 22;
+    return launch(kernel, dim3((unsigned)(wgs < most ? wgs : most)), dim3(NT < 256 ? 256 : NT), lds, stream, d);
 }
 
 static int distill_launch(hipStream_t stream, const oak_distill_args* a) {

@@ -31,7 +31,7 @@ namespace oak {
 enum { KEY_16 = 0, KEY_TAG = 1, KEY_F64 = 2 };
 
 struct RouteDev {
-    int64_t n, ld, ld_mask, ld_out;
+    int64_t row0, n, ld, ld_mask, ld_out;
     int E, k, groups, top_groups, group_size, lanes_per_group;
     int dtype, sigmoid, top2, renorm, bias_f64;
     double scale;
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
     constexpr int TEAMS = 64 / L;
     extern __shared__ __align__(16) unsigned char lds[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, team = lane / L, l = lane & (L - 1);
-    const int64_t row = ((int64_t)blockIdx.x * 4 + wave) * TEAMS + team, at = row < a.n ? row : a.n - 1;
+    const int64_t row = a.row0 + ((int64_t)blockIdx.x * 4 + wave) * TEAMS + team, at = row < a.n ? row : a.n - 1;
     const int base = l * VPL;
 
     acc x[VPL];
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(256) route_grad_kernel(RouteDev a) {
     constexpr int TEAMS = 64 / L;
     extern __shared__ __align__(16) unsigned char lds[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, team = lane / L, l = lane & (L - 1);
-    const int64_t row = ((int64_t)blockIdx.x * 4 + wave) * TEAMS + team;
+    const int64_t row = a.row0 + ((int64_t)blockIdx.x * 4 + wave) * TEAMS + team;
     const bool live = row < a.n;
     const int64_t at = live ? row : a.n - 1;
     const int base = l * VPL;
@@ -468,6 +468,16 @@ static RouteDev route_dev(const oak_route_args* a) {
     return d;
 }
 
+// a launch has fewer than 2^32 threads: more rows than 2^23 workgroups of 256 take are done in several
+template <typename Args> static int launch_rows(void (*kernel)(Args), int rows_per_wg, size_t lds, hipStream_t stream, Args& d) {
+    const int64_t most = (int64_t)rows_per_wg << 23;
+    for (d.row0 = 0; d.row0 < d.n; d.row0 += most) {
+        const int64_t rows = d.n - d.row0 < most ? d.n - d.row0 : most;
+        OAK_CHECK(launch(kernel, dim3((unsigned)((rows + rows_per_wg - 1) / rows_per_wg)), dim3(256), lds, stream, d));
+    }
+    return OAK_OK;
+}
+
 static int route_launch(hipStream_t stream, const oak_route_args* a) {
     if (a->n_rows == 0) return OAK_OK;
     RouteDev d = route_dev(a);
@@ -475,14 +485,13 @@ static int route_launch(hipStream_t stream, const oak_route_args* a) {
     auto run = [&](auto kind, auto most) {
         return with_team<decltype(most)::value>(d.E, d.k, d.n, [&](auto lc, auto vc) {
             constexpr int L = decltype(lc)::value, VPL = decltype(vc)::value, TEAMS = 64 / L;
-            const dim3 grid((unsigned)((d.n + 4 * TEAMS - 1) / (4 * TEAMS)));
             // groups that are whole lanes, a power of two of them, are scored without LDS
             const int lanes = d.group_size % VPL == 0 ? d.group_size / VPL : 0;
             d.lanes_per_group = lanes > 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
             const size_t lds = d.groups > 1 ? (size_t)4 * TEAMS * (d.lanes_per_group ? d.groups : d.E + d.groups) * sizeof(double) : 0;
             auto kernel = route_kernel<decltype(kind)::value, L, VPL>;
             if (lds > 64 * 1024) OAK_CHECK(ensure_dynamic_lds((const void*)kernel, 160 * 1024));
-            return launch(kernel, grid, dim3(256), lds, stream, d);
+            return launch_rows(kernel, 4 * TEAMS, lds, stream, d);
         });
     };
     // 64-bit keys take twice the registers: at most 16 a lane
@@ -493,14 +502,13 @@ static int route_launch(hipStream_t stream, const oak_route_args* a) {
 
 static int route_grad_launch(hipStream_t stream, const oak_route_args* a) {
     if (a->n_rows == 0) return OAK_OK;
-    const RouteDev d = route_dev(a);
+    RouteDev d = route_dev(a);
     return with_team<16>(d.E, d.k, d.n, [&](auto lc, auto vc) {
         constexpr int L = decltype(lc)::value, VPL = decltype(vc)::value, TEAMS = 64 / L;
-        const dim3 grid((unsigned)((d.n + 4 * TEAMS - 1) / (4 * TEAMS)));
         auto go = [&](auto zero) {
             using acc = decltype(zero);
             const size_t lds = (size_t)4 * TEAMS * L * VPL * sizeof(acc);
-            return launch(route_grad_kernel<acc, L, VPL>, grid, dim3(256), lds, stream, d);
+            return launch_rows(route_grad_kernel<acc, L, VPL>, 4 * TEAMS, lds, stream, d);
         };
         return d.dtype == OAK_F64 ? go((double)0) : go((float)0);
     });
@@ -702,7 +710,7 @@ static int plan_launch(hipStream_t stream, const oak_plan_args* a) {
 // 16 bytes, the row's last elements that do not fill one are units of their own.  A thread asks for the places, then for the answers of up
 // to 4 slots before it adds the first.  Bound by memory: 32768 rows, k = 6, 2048 bf16 columns at MIX_RATES.
 struct MixDev {
-    int64_t n, slots, ld_rows, ld_slots, ld_grad;
+    int64_t row0, n, slots, ld_rows, ld_slots, ld_grad;
     int64_t units;              // 16-byte units of a row, then its last elements
     int C, k, nvec, E, tpr, inv_tpr, rows_per_wg, tpr_log2;
     const int* positions; const int* offsets; const void* weights;
@@ -724,7 +732,7 @@ __device__ __forceinline__ int64_t place_of(const MixDev& a, int64_t n, int j) {
 __device__ __forceinline__ int64_t mix_row(const MixDev& a, int* unit) {
     const int r = (int)(((unsigned)threadIdx.x * (unsigned)a.inv_tpr) >> 16);
     *unit = (int)threadIdx.x - r * a.tpr;
-    const int64_t n = (int64_t)blockIdx.x * a.rows_per_wg + r;
+    const int64_t n = a.row0 + (int64_t)blockIdx.x * a.rows_per_wg + r;
     return r < a.rows_per_wg && n < a.n ? n : -1;
 }
 
@@ -795,8 +803,8 @@ template <typename T, int CHUNK> __global__ void __launch_bounds__(256) combine_
 // finished inside a wave.
 template <typename T> __global__ void __launch_bounds__(256) combine_grad_kernel(MixDev a) {
     using acc = typename Num<T>::acc;
-    const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x, n = g >> a.tpr_log2;
-    const int tpr = 1 << a.tpr_log2, t = (int)(g & (tpr - 1));
+    const int64_t n = a.row0 + (int64_t)blockIdx.x * a.rows_per_wg + (threadIdx.x >> a.tpr_log2);
+    const int tpr = 1 << a.tpr_log2, t = (int)(threadIdx.x & (tpr - 1));
     const bool live = n < a.n;                         // whole waves stay for the shuffles
     const T* F = static_cast<const T*>(a.src);
     const T* dy = static_cast<const T*>(a.dout) + (live ? n : 0) * a.ld_grad;
@@ -854,11 +862,10 @@ static int mix_launch(hipStream_t stream, const oak_mix_args* a, int what /* 0 d
     d.tpr = d.units < 256 ? (int)d.units : 256;
     d.rows_per_wg = what == 2 ? 256 >> d.tpr_log2 : 256 / d.tpr;
     d.inv_tpr = (65536 + d.tpr - 1) / d.tpr;           // t / tpr = t inv_tpr >> 16 for t < 256
-    const int64_t wgs = (d.n + d.rows_per_wg - 1) / d.rows_per_wg;
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
         auto kernel = what == 0 ? dispatch_kernel<T> : what == 2 ? combine_grad_kernel<T> : d.k <= 2 ? combine_kernel<T, 2> : combine_kernel<T, 4>;
-        return launch(kernel, dim3((unsigned)wgs), dim3(256), 0, stream, d);
+        return launch_rows(kernel, d.rows_per_wg, 0, stream, d);
     });
 }
 

@@ -87,6 +87,14 @@ class Device:
         return self.torch.empty(shape, dtype=dtype, device=self.device)
 
 
+def whole(value, what: str, low: int, high: int) -> int:
+    """An integer in [low, high]; checked here, before it sizes an array or is cut to 32 bits on its way to the library."""
+    number = int(value)
+    if number != value or not low <= number <= high:
+        raise ValueError(f"{what} = {value!r} is not an integer in {low} .. {high}")
+    return number
+
+
 def ptr(a) -> int | None:
     """Address of a tensor or array, None for None and for empty ones."""
     if a is None:

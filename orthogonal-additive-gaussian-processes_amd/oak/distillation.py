@@ -16,6 +16,7 @@ import numpy as np
 from . import _arrays as A
 from . import _capi
 
+MAX_CLASSES, MAX_TEACHER = 1 << 20, 1024
 _DIRECTIONS = {"forward": 0, "reverse": 1}
 
 
@@ -60,6 +61,8 @@ def _distill(logits, top, index, top_lse, temperature, direction, row_weight, gr
     k = top.shape[1]
     if top.shape[0] != n:
         raise ValueError(f"top has {top.shape[0]} rows, logits {n}")
+    if not (1 <= v <= MAX_CLASSES and 1 <= k <= MAX_TEACHER):
+        raise ValueError(f"{v} classes and {k} entries; 1 .. {MAX_CLASSES} classes and 1 .. {MAX_TEACHER} entries are supported")
     a = _capi.DistillArgs(n_rows=n, n_classes=v, top_k=k, temperature=float(temperature), direction=_DIRECTIONS[direction])
     if device:
         a.dtype, a.top_dtype = A.code_of(logits, "logits"), A.code_of(top, "top")

@@ -24,6 +24,7 @@ import numpy as np
 from . import _arrays as A
 from . import _capi
 
+MAX_EXPERTS, MAX_PLAN_EXPERTS, MAX_TOP_K = 1024, 4096, 64
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORES = {"max": 0, "top2": 1}
 
@@ -37,9 +38,13 @@ def _code(table, value, what):
 
 def _route_args(scores, top_k, score, n_groups, top_groups, group_score, renormalise, scale, code, ld):
     n, e = scores.shape
-    a = _capi.RouteArgs(n_rows=n, ld_scores=ld, n_experts=e, top_k=int(top_k), n_groups=int(n_groups),
-                        top_groups=int(n_groups if top_groups is None else top_groups), dtype=code, score=_code(_SCORES, score, "score"),
-                        group_score=_code(_GROUP_SCORES, group_score, "group_score"), renormalise=1 if renormalise else 0, scale=float(scale))
+    if not 1 <= e <= MAX_EXPERTS:
+        raise ValueError(f"scores has {e} columns; 1 .. {MAX_EXPERTS} experts are supported")
+    n_groups = A.whole(n_groups, "n_groups", 1, 64)
+    a = _capi.RouteArgs(n_rows=n, ld_scores=ld, n_experts=e, top_k=A.whole(top_k, "top_k", 1, min(e, MAX_TOP_K)), n_groups=n_groups,
+                        top_groups=n_groups if top_groups is None else A.whole(top_groups, "top_groups", 1, n_groups), dtype=code,
+                        score=_code(_SCORES, score, "score"), group_score=_code(_GROUP_SCORES, group_score, "group_score"),
+                        renormalise=1 if renormalise else 0, scale=float(scale))
     a.scores = A.ptr(scores)
     return a
 
@@ -96,7 +101,7 @@ def route(scores, top_k: int, *, score: str = "softmax", bias=None, n_groups: in
             if bias.dtype not in (d.torch.float32, d.torch.float64):
                 bias = bias.to(d.torch.float32)
             a.bias_f64, a.bias = int(bias.dtype == d.torch.float64), A.ptr(bias)
-        experts, weights = d.empty((n, max(a.top_k, 0)), d.torch.int32), d.empty((n, max(a.top_k, 0)), d.wide(code))
+        experts, weights = d.empty((n, a.top_k), d.torch.int32), d.empty((n, a.top_k), d.wide(code))
         a.experts, a.weights = A.ptr(experts), A.ptr(weights)
         _capi.call_device("route", d.index, d.stream, a)
         return experts, weights
@@ -109,7 +114,7 @@ def route(scores, top_k: int, *, score: str = "softmax", bias=None, n_groups: in
         if not np.isfinite(bias).all():
             raise ValueError("bias is not finite")
         a.bias_f64, a.bias = 1, A.ptr(bias)
-    experts, weights = np.empty((n, max(a.top_k, 0)), dtype=np.int32), np.empty((n, max(a.top_k, 0)))
+    experts, weights = np.empty((n, a.top_k), dtype=np.int32), np.empty((n, a.top_k))
     a.experts, a.weights = A.ptr(experts), A.ptr(weights)
     _capi.default_context().call("route", a)
     return experts, weights
@@ -187,23 +192,25 @@ def plan(experts, n_experts: int) -> Plan:
     Slots keep their order within an expert, so the layout depends on nothing but its input.  A slot whose expert is -1 has no place.  On a device any
     other value outside 0 .. n_experts - 1 has none either; in a NumPy array it is refused.  At most 4096 experts.
     """
-    n_experts = int(n_experts)
+    n_experts = A.whole(n_experts, "n_experts", 1, MAX_PLAN_EXPERTS)
     shape = tuple(experts.shape) if hasattr(experts, "shape") else np.shape(experts)
     if len(shape) not in (1, 2):
         raise ValueError(f"experts has shape {shape}, expected [N, k] or [N]")
-    n, k = shape[0], shape[1] if len(shape) == 2 else 1
+    n, k = shape[0], A.whole(shape[1], "k", 1, MAX_TOP_K) if len(shape) == 2 else 1
+    if n * k >= 1 << 31:
+        raise ValueError(f"{n} rows x {k} experts pass 2^31 slots")
     a = _capi.PlanArgs(n_rows=n, top_k=k, n_experts=n_experts)
     if A.on_device(experts):
         d = A.Device(experts)
         experts = _device_experts(d, experts, shape, n_experts)
         i32 = d.torch.int32
-        out = [d.empty((n * k,), i32), d.empty(shape, i32), d.empty((max(n_experts, 0),), i32), d.empty((max(n_experts, 0) + 1,), i32)]
+        out = [d.empty((n * k,), i32), d.empty(shape, i32), d.empty((n_experts,), i32), d.empty((n_experts + 1,), i32)]
         a.workspace_ints = _capi.plan_workspace(n, k, n_experts)
         workspace = d.empty((a.workspace_ints,), i32) if a.workspace_ints else None
         a.workspace = A.ptr(workspace)
     else:
         experts = A.host_index(experts, "experts", -1, n_experts)
-        out = [np.empty(s, dtype=np.int32) for s in ((n * k,), shape, (max(n_experts, 0),), (max(n_experts, 0) + 1,))]
+        out = [np.empty(s, dtype=np.int32) for s in ((n * k,), shape, (n_experts,), (n_experts + 1,))]
     a.experts = A.ptr(experts)
     a.rows, a.positions, a.counts, a.offsets = map(A.ptr, out)
     if A.on_device(experts):
@@ -225,7 +232,10 @@ def _mix(name, plan, first, what, slots_in, weights=None, dout=None):
     rows_in = n * k if slots_in else n
     if len(shape) not in (1, 2) or shape[0] != rows_in:
         raise ValueError(f"{what} has shape {shape}, the plan expects {rows_in} rows")
-    flat, c = len(shape) == 1, 1 if len(shape) == 1 else shape[1]
+    flat, c = len(shape) == 1, 1 if len(shape) == 1 else A.whole(shape[1], f"the number of columns of {what}", 0, 1 << 30)
+    for part, size in ((plan.positions, n * k), (plan.offsets, plan.n_experts + 1)):
+        if not str(part.dtype).endswith("int32") or (part.numel() if device else part.size) != size:
+            raise ValueError("plan has been altered: its arrays do not fit its sizes")
     a = _capi.MixArgs(n_rows=n, top_k=k, n_experts=plan.n_experts, n_cols=c, ld_rows=c, ld_slots=c, ld_grad=c)
 
     def two(x):
@@ -235,7 +245,7 @@ def _mix(name, plan, first, what, slots_in, weights=None, dout=None):
         d = A.Device(first)
         src = d.matrix(two(first), what)
         a.dtype = A.code_of(src, what)
-        d.tensor(plan.positions, "the plan")
+        positions, offsets = d.tensor(plan.positions, "the plan").contiguous(), d.tensor(plan.offsets, "the plan").contiguous()
         wide = d.wide(a.dtype)
         if weights is not None:
             weights = d.dense(weights, "weights", (n, k), wide)
@@ -249,6 +259,7 @@ def _mix(name, plan, first, what, slots_in, weights=None, dout=None):
         stride = src.stride(0)
     else:
         src = A.host(two(np.asarray(first)), what)
+        positions, offsets = np.ascontiguousarray(plan.positions), np.ascontiguousarray(plan.offsets)
         if weights is not None:
             weights = A.host(weights, "weights", (n, k))
         if dout is not None:
@@ -262,7 +273,7 @@ def _mix(name, plan, first, what, slots_in, weights=None, dout=None):
     else:
         a.ld_rows = stride
     a.src, a.weights, a.dout = A.ptr(src), A.ptr(weights), A.ptr(dout)
-    a.positions, a.offsets = A.ptr(plan.positions), A.ptr(plan.offsets)
+    a.positions, a.offsets = A.ptr(positions), A.ptr(offsets)
     if name == "combine_grad":
         out, dweights = empty(n * k), empty_w()
         a.dslots, a.dweights = A.ptr(out), A.ptr(dweights)

@@ -217,3 +217,44 @@ def test_streams_and_captured_graphs():
         torch.cuda.synchronize()
         for a, b in zip(od.distill_grad(s, top, idx, top_lse=lse), held):
             assert torch.equal(a, b)
+
+
+def test_offsets_beyond_32_bits():
+    far = (1 << 30) + 3
+    store = torch.zeros(2 * far + 5000, device="cuda", dtype=torch.bfloat16)
+    s = store.as_strided((3, 5000), (far, 1))
+    small, top, idx, lse = problem(3, 5000, 9, "bf16", True, seed=4)
+    s.copy_(small)
+    compare(s, top, idx, lse, 1.0, "forward", None, "bf16")
+
+
+@pytest.mark.parametrize("n,v", [((1 << 28) + 70, 2), ((1 << 22) + 3, 9000)])
+def test_more_rows_than_one_launch_takes(n, v):
+    """Beyond 2^22 workgroups a workgroup walks on to further rows; the rows are one row n times over (row stride 0)."""
+    s, top, idx, lse = problem(1, v, 1, "f16", True)
+    one = od.distill(s, top, idx, top_lse=lse)
+    loss = od.distill(s.expand(n, v), top.expand(n, 1), idx.expand(n, 1), top_lse=lse.expand(n))
+    assert bool((loss == one).all())
+
+
+def test_rows_differ_from_launch_to_launch_row():
+    """A workgroup's second row must not see the first one's entries: rows with entries in different places, few workgroups' worth each."""
+    for n, v, k in ((3000, 40, 3), (700, 600, 20), (300, 9000, 40)):
+        s, top, idx, lse = problem(n, v, k, "f32", True, seed=n)
+        compare(s, top, idx, lse, 1.0, "forward", None, "f32")
+
+
+def test_refusals_on_the_device():
+    s, top, idx, lse = problem(4, 30, 3, "f32", True)
+    cases = [
+        lambda: od.distill(s.clone().requires_grad_(), top, idx), lambda: od.distill(s, top.cpu(), idx), lambda: od.distill(s, back(top), idx),
+        lambda: od.distill(s, top, idx.float()), lambda: od.distill(s, top, idx[:, :2]), lambda: od.distill(s, top[:3], idx[:3]),
+        lambda: od.distill(s, top, idx, top_lse=lse[:3]), lambda: od.distill(s, top, idx, direction="reverse"),
+        lambda: od.distill(s, top, idx, temperature=0.0), lambda: od.distill(s, top, idx, row_weight=lse[:, None]),
+        lambda: od.distill(s.to(torch.int32), top, idx), lambda: od.distill(s[0], top, idx),
+        lambda: od.distill(torch.zeros(1, (1 << 20) + 1, device="cuda"), top[:1], idx[:1]),
+    ]
+    for i, call in enumerate(cases):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"case {i} was not refused")

@@ -347,3 +347,94 @@ def test_streams_and_captured_graphs():
         torch.cuda.synchronize()
         for a, b, c2 in zip(step(), held, held2):
             assert torch.equal(a, b) and torch.equal(a, c2)
+
+
+def test_offsets_beyond_32_bits():
+    """Rows whose offset in elements passes 2^31: strided scores, a laid-out array of more than 2^32 bytes."""
+    rng = np.random.default_rng(9)
+    far = (1 << 30) + 7
+    store = torch.zeros(2 * far + 64, device="cuda", dtype=torch.bfloat16)
+    x = store.as_strided((3, 64), (far, 1))
+    x.copy_(tensor(rng.standard_normal((3, 64)), "bf16"))
+    ex, w = ox.route(x, 4)
+    er, wr = eo.route(back(x), 4)
+    np.testing.assert_array_equal(back(ex), er)
+    p = ox.plan(ex, 64)
+    laid = ox.dispatch(x, p)
+    np.testing.assert_array_equal(back(laid), eo.dispatch(back(x), back(p.rows)))
+    del store, x
+    n, c = 300_000, 8192                                                 # 2.46e9 elements laid out
+    ex = torch.arange(n, device="cuda", dtype=torch.int32).flip(0) % 7
+    p = ox.plan(ex, 7)
+    X = torch.arange(n, device="cuda", dtype=torch.float32).remainder(251).to(torch.bfloat16)[:, None].expand(n, c)
+    laid = ox.dispatch(X, p)
+    rows = p.rows.long()
+    at = torch.tensor([0, 1, n // 2, n - 2, n - 1], device="cuda")
+    assert torch.equal(laid[at], X[rows[at]])
+    y = ox.combine(laid, torch.ones(n, 1, device="cuda"), p)
+    assert torch.equal(y[at], X[at])
+    dF, dw = ox.combine_grad(laid, torch.ones(n, 1, device="cuda"), p, y)
+    assert torch.equal(dF[at], laid[at])
+    np.testing.assert_allclose(back(dw[at, 0]), c * back(X[at, 0]) ** 2, rtol=1e-5)
+
+
+def test_more_rows_than_one_launch_takes():
+    """The rows of a call are walked in several launches beyond 2^23 workgroups (inputs with row stride 0 keep them small)."""
+    n = (1 << 30) + 5
+    ex, w = ox.route(torch.tensor([[1.0, 3.0]], device="cuda", dtype=torch.float16).expand(n, 2), 1)
+    for part in (slice(0, 3), slice((1 << 30) - 3, (1 << 30) + 5)):
+        assert (ex[part] == 1).all() and (w[part] == 1).all()
+    assert int(ex.min()) == 1
+    del ex, w
+    n, c = (1 << 23) + 3, 1032                                           # 129 units a row: one row a workgroup
+    p = ox.plan(torch.zeros(n, device="cuda", dtype=torch.int32), 1)
+    y = ox.combine(torch.full((1, c), 2.0, device="cuda", dtype=torch.bfloat16).expand(n, c), torch.full((n, 1), 3.0, device="cuda"), p)
+    assert (y[-4:] == 6).all() and (y[:2] == 6).all() and bool((y[:, 0] == 6).all())
+
+
+def test_refusals_on_the_device():
+    x = torch.randn(4, 6, device="cuda")
+    ex, w = ox.route(x, 2)
+    p = ox.plan(ex, 6)
+    cases = [
+        lambda: ox.route(x.clone().requires_grad_(), 2), lambda: ox.route(x, 2, bias=np.zeros(6)), lambda: ox.route(x, 2, bias=torch.zeros(6)),
+        lambda: ox.route(x.to(torch.int32), 2), lambda: ox.route(x, 7), lambda: ox.route(x, 0), lambda: ox.route(x, 2 ** 32 + 1),
+        lambda: ox.route(x, 1.5), lambda: ox.route(x, 2, mask=torch.ones(4, 5, device="cuda", dtype=torch.bool)),
+        lambda: ox.route(x, 2, mask=torch.ones(4, 6, device="cuda")), lambda: ox.route(torch.randn(2, 1025, device="cuda"), 2),
+        lambda: ox.route_grad(x, ex, w[:, :1]), lambda: ox.route_grad(x, ex.float(), w), lambda: ox.route_grad(x, back(ex), w),
+        lambda: ox.plan(ex, 2 ** 32 + 6), lambda: ox.plan(ex.float(), 6), lambda: ox.plan(ex[:, None], 6), lambda: ox.plan(ex, 5000),
+        lambda: ox.dispatch(back(x), p), lambda: ox.dispatch(x[:3], p), lambda: ox.combine(x, w, p), lambda: ox.combine(torch.zeros(8, 3), w, p),
+        lambda: ox.combine(torch.zeros(8, 3, device="cuda"), w, p._replace(positions=p.positions[:2])),
+        lambda: ox.combine(torch.zeros(8, 3, device="cuda"), w, p._replace(positions=p.positions.long())),
+        lambda: ox.combine(torch.zeros(8, 3, device="cuda"), w, p._replace(n_experts=9)),
+        lambda: ox.combine_grad(torch.zeros(8, 3, device="cuda"), w, p, torch.zeros(4, 2, device="cuda")),
+    ]
+    for i, call in enumerate(cases):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"case {i} was not refused")
+
+
+def test_two_threads_at_once():
+    """Device calls share no state: two threads on streams of their own get what one gets."""
+    import threading
+    rng = np.random.default_rng(0)
+    xs = [tensor(rng.standard_normal((5000, 48)), "bf16") for _ in range(2)]
+    ref = [ox.route(x, 4, renormalise=False) for x in xs]
+    plans = [ox.plan(r[0], 48) for r in ref]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                ex, w = ox.route(xs[i], 4, renormalise=False)
+                p = ox.plan(ex, 48)
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(ex, ref[i][0]) and torch.equal(w, ref[i][1]) and torch.equal(p.positions, plans[i].positions)):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
