@@ -413,10 +413,11 @@ int oak_kmeans_plusplus(oak_ctx* ctx, const double* X, int64_t N, int32_t D, int
 /* ---- mixtures of models: routing, dispatch, combination ------------------------------------------ */
 /* The operators of this section and the next come in two forms.  oak_X(ctx, args): the arrays are on the host, contiguous and
    float64 like everywhere else; the call copies them, runs on the context's stream and returns when the outputs are there.
-   oak_X_device(device, stream, args): the arrays are in the memory of `device`, of any of the types below, rows `ld` elements apart
-   (their columns are consecutive; rows may start anywhere); the call enqueues its kernels on `stream` (a hipStream_t, NULL is
-   the default stream) and returns.  It allocates nothing, keeps nothing, waits for nothing and may be captured into a graph.  The arrays must belong to
-   the HIP runtime this library is linked against (oak_device_pointer_check).
+   oak_X_device(ctx, stream, args): the arrays are in the memory of ctx's device, of any of the types below, rows `ld` elements apart
+   (their columns are consecutive; rows may start anywhere); the call enqueues its kernels on `stream` (a hipStream_t of that device, NULL is
+   the default stream) and returns.  It takes nothing but the device from ctx, so that any number of threads may share one for these calls; it
+   allocates nothing, keeps nothing, waits for nothing, leaves the thread's current device as it was and may be captured into a graph.  The
+   arrays must belong to the HIP runtime this library is linked against (oak_device_pointer_check).
    Sums, weights, losses and softmax statistics are float64 for float64 arrays and float32 otherwise: "wide" below. */
 #define OAK_F64   0
 #define OAK_F32   1
@@ -432,8 +433,8 @@ int oak_kmeans_plusplus(oak_ctx* ctx, const double* X, int64_t N, int32_t D, int
 #define OAK_GROUP_MAX     0         /* a group's score: its highest key ...                      */
 #define OAK_GROUP_TOP2    1         /* ... or the sum of its two highest (the one, if it has one) */
 
-/* OAK_OK if p is memory of `device` known to this library's HIP runtime (a process can hold two copies of that runtime). */
-int oak_device_pointer_check(int32_t device, const void* p);
+/* OAK_OK if p is memory of ctx's device known to this library's HIP runtime (a process can hold two copies of that runtime). */
+int oak_device_pointer_check(oak_ctx* ctx, const void* p);
 
 /* Each row's experts.  p = softmax over the row's open scores, or sigmoid; a score is open unless its mask is 0 or it is -inf.
    key = p + bias where there is a bias (it moves the choice, not the weights), else the score itself.  With n_groups > 1 only the
@@ -455,9 +456,9 @@ typedef struct oak_route_args {
     void* dscores;             /* oak_route_grad: [n_rows, n_experts] dtype, out      */
 } oak_route_args;
 int oak_route(oak_ctx* ctx, const oak_route_args* args);
-int oak_route_device(int32_t device, void* stream, const oak_route_args* args);
+int oak_route_device(oak_ctx* ctx, void* stream, const oak_route_args* args);
 int oak_route_grad(oak_ctx* ctx, const oak_route_args* args);
-int oak_route_grad_device(int32_t device, void* stream, const oak_route_args* args);
+int oak_route_grad_device(oak_ctx* ctx, void* stream, const oak_route_args* args);
 
 /* The order of slots by expert.  Slot n top_k + j is row n's j-th expert.  counts[e] slots belong to expert e and are the places
    offsets[e] .. offsets[e + 1) - 1 of the order, in slot order.  positions[slot] is the slot's place (-1: its expert is not in
@@ -473,9 +474,9 @@ typedef struct oak_plan_args {
     int32_t* offsets;          /* [n_experts + 1] out  */
     int32_t* workspace;
 } oak_plan_args;
-int64_t oak_plan_workspace(int64_t n_rows, int32_t top_k, int32_t n_experts);
+int64_t oak_plan_workspace(oak_ctx* ctx, int64_t n_rows, int32_t top_k, int32_t n_experts);   /* 0 for ctx NULL */
 int oak_plan(oak_ctx* ctx, const oak_plan_args* args);
-int oak_plan_device(int32_t device, void* stream, const oak_plan_args* args);
+int oak_plan_device(oak_ctx* ctx, void* stream, const oak_plan_args* args);
 
 /* Row arrays have n_rows rows (ld_rows apart), slot arrays n_rows top_k rows (ld_slots apart) in the plan's order; places behind
    the last used one (offsets[n_experts]) are written as zeros where a slot array is an output.
@@ -496,11 +497,11 @@ typedef struct oak_mix_args {
     void* dweights;            /* wide */
 } oak_mix_args;
 int oak_dispatch(oak_ctx* ctx, const oak_mix_args* args);
-int oak_dispatch_device(int32_t device, void* stream, const oak_mix_args* args);
+int oak_dispatch_device(oak_ctx* ctx, void* stream, const oak_mix_args* args);
 int oak_combine(oak_ctx* ctx, const oak_mix_args* args);
-int oak_combine_device(int32_t device, void* stream, const oak_mix_args* args);
+int oak_combine_device(oak_ctx* ctx, void* stream, const oak_mix_args* args);
 int oak_combine_grad(oak_ctx* ctx, const oak_mix_args* args);
-int oak_combine_grad_device(int32_t device, void* stream, const oak_mix_args* args);
+int oak_combine_grad_device(oak_ctx* ctx, void* stream, const oak_mix_args* args);
 
 /* ---- distillation ------------------------------------------------------------------------------- */
 /* Divergence of a student's class distribution q = softmax(logits / temperature) from a teacher of which only the top_k highest logits
@@ -530,7 +531,7 @@ typedef struct oak_distill_args {
     void* dlogits;             /* [n_rows, n_classes] dtype, out, or NULL   */
 } oak_distill_args;
 int oak_distill(oak_ctx* ctx, const oak_distill_args* args);
-int oak_distill_device(int32_t device, void* stream, const oak_distill_args* args);
+int oak_distill_device(oak_ctx* ctx, void* stream, const oak_distill_args* args);
 
 /* Measurement hooks (oak_bench_*: resident Gram pass, the tail's Cholesky and the many-row triangular solve on their own) are not part
    of the drop-in surface: include/oak_hip_bench.h. */

@@ -402,8 +402,9 @@ using namespace oak;
 
 extern "C" {
 
-int oak_device_pointer_check(int32_t device, const void* p) {
+int oak_device_pointer_check(oak_ctx* ctx, const void* p) {
     return c_entry([&] {
+        OAK_REQUIRE(ctx != nullptr, "ctx is NULL");
         OAK_REQUIRE(p != nullptr, "the pointer is NULL");
         hipPointerAttribute_t at{};
         const hipError_t e = hipPointerGetAttributes(&at, p);
@@ -411,17 +412,17 @@ int oak_device_pointer_check(int32_t device, const void* p) {
             (void)hipGetLastError();
             OAK_REQUIRE(false, "%p is not memory of this library's HIP runtime (%s)", p, hipGetErrorString(e));
         }
-        OAK_REQUIRE((at.type == hipMemoryTypeDevice || at.type == hipMemoryTypeManaged) && at.device == device,
-                    "%p is not memory of device %d known to this library's HIP runtime", p, device);
+        OAK_REQUIRE((at.type == hipMemoryTypeDevice || at.type == hipMemoryTypeManaged) && at.device == ctx->device,
+                    "%p is not memory of device %d known to this library's HIP runtime", p, ctx->device);
         return (int)OAK_OK;
     });
 }
 
-int oak_distill_device(int32_t device, void* stream, const oak_distill_args* a) {
+int oak_distill_device(oak_ctx* ctx, void* stream, const oak_distill_args* a) {
     return c_entry([&] {
         OAK_CHECK(distill_check(a));
         DeviceGuard g;
-        OAK_CHECK(g.enter(device));
+        OAK_CHECK(g.enter(ctx));
         return distill_launch((hipStream_t)stream, a);
     });
 }

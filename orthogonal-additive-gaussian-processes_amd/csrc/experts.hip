@@ -671,6 +671,13 @@ static void plan_pieces(int64_t slots, int E, int64_t* piece, int* npieces, bool
     *npieces = (int)((slots + p - 1) / p);
 }
 
+static int64_t plan_workspace(int64_t n_rows, int32_t top_k, int32_t n_experts) {
+    if (n_rows <= 0 || top_k <= 0 || n_experts <= 0) return 0;
+    int64_t piece; int np; bool small;
+    plan_pieces(n_rows * top_k, n_experts, &piece, &np, &small);
+    return small ? 0 : (int64_t)np * n_experts;
+}
+
 static int plan_check(const oak_plan_args* a) {
     OAK_REQUIRE(a != nullptr, "plan: arguments are NULL");
     OAK_REQUIRE(a->n_rows >= 0 && a->top_k >= 1 && a->top_k <= OAK_MAX_TOP_K, "plan: %lld rows of %d experts", (long long)a->n_rows, a->top_k);
@@ -875,23 +882,23 @@ using namespace oak;
 
 extern "C" {
 
-int oak_route_device(int32_t device, void* stream, const oak_route_args* a) {
+int oak_route_device(oak_ctx* ctx, void* stream, const oak_route_args* a) {
     return c_entry([&] {
         OAK_CHECK(route_check(a));
         OAK_REQUIRE(a->n_rows == 0 || a->weights, "route: weights are NULL");
         DeviceGuard g;
-        OAK_CHECK(g.enter(device));
+        OAK_CHECK(g.enter(ctx));
         return route_launch((hipStream_t)stream, a);
     });
 }
 
-int oak_route_grad_device(int32_t device, void* stream, const oak_route_args* a) {
+int oak_route_grad_device(oak_ctx* ctx, void* stream, const oak_route_args* a) {
     return c_entry([&] {
         OAK_CHECK(route_check(a));
         OAK_REQUIRE(a->n_rows == 0 || (a->dweights && a->dscores), "route_grad: dweights or dscores are NULL");
         OAK_REQUIRE(a->n_rows <= 1 || a->ld_dscores >= a->n_experts, "route_grad: rows of dscores overlap");
         DeviceGuard g;
-        OAK_CHECK(g.enter(device));
+        OAK_CHECK(g.enter(ctx));
         return route_grad_launch((hipStream_t)stream, a);
     });
 }
@@ -930,21 +937,18 @@ static int route_host(oak_ctx* ctx, const oak_route_args* args, bool grad) {
 int oak_route(oak_ctx* ctx, const oak_route_args* a) { return c_entry([&] { return route_host(ctx, a, false); }); }
 int oak_route_grad(oak_ctx* ctx, const oak_route_args* a) { return c_entry([&] { return route_host(ctx, a, true); }); }
 
-int64_t oak_plan_workspace(int64_t n_rows, int32_t top_k, int32_t n_experts) {
-    if (n_rows <= 0 || top_k <= 0 || n_experts <= 0) return 0;
-    int64_t piece; int np; bool small;
-    plan_pieces(n_rows * top_k, n_experts, &piece, &np, &small);
-    return small ? 0 : (int64_t)np * n_experts;
+int64_t oak_plan_workspace(oak_ctx* ctx, int64_t n_rows, int32_t top_k, int32_t n_experts) {
+    return ctx ? plan_workspace(n_rows, top_k, n_experts) : 0;
 }
 
-int oak_plan_device(int32_t device, void* stream, const oak_plan_args* a) {
+int oak_plan_device(oak_ctx* ctx, void* stream, const oak_plan_args* a) {
     return c_entry([&] {
         OAK_CHECK(plan_check(a));
-        const int64_t ints = oak_plan_workspace(a->n_rows, a->top_k, a->n_experts);
+        const int64_t ints = plan_workspace(a->n_rows, a->top_k, a->n_experts);
         OAK_REQUIRE(ints == 0 || (a->workspace && a->workspace_ints >= ints), "plan: the workspace holds %lld of the %lld integers asked for by oak_plan_workspace",
                     (long long)a->workspace_ints, (long long)ints);
         DeviceGuard g;
-        OAK_CHECK(g.enter(device));
+        OAK_CHECK(g.enter(ctx));
         return plan_launch((hipStream_t)stream, a);
     });
 }
@@ -963,7 +967,7 @@ int oak_plan(oak_ctx* ctx, const oak_plan_args* args) {
         OAK_CHECK(st.out("ex_positions", a.positions, slots * 4));
         OAK_CHECK(st.out("ex_counts", a.counts, (size_t)a.n_experts * 4));
         OAK_CHECK(st.out("ex_offsets", a.offsets, (size_t)(a.n_experts + 1) * 4));
-        a.workspace_ints = oak_plan_workspace(a.n_rows, a.top_k, a.n_experts);
+        a.workspace_ints = plan_workspace(a.n_rows, a.top_k, a.n_experts);
         void* ws = nullptr;
         OAK_CHECK(get_buf(ctx, "ex_plan_ws", (size_t)a.workspace_ints * 4, &ws));
         a.workspace = (int32_t*)ws;
@@ -987,11 +991,11 @@ static int mix_arrays(const char* name, const oak_mix_args* a, int what) {
     return OAK_OK;
 }
 
-static int mix_device(const char* name, int32_t device, void* stream, const oak_mix_args* a, int what) {
+static int mix_device(const char* name, oak_ctx* ctx, void* stream, const oak_mix_args* a, int what) {
     return c_entry([&] {
         OAK_CHECK(mix_arrays(name, a, what));
         DeviceGuard g;
-        OAK_CHECK(g.enter(device));
+        OAK_CHECK(g.enter(ctx));
         return mix_launch((hipStream_t)stream, a, what);
     });
 }
@@ -1032,8 +1036,8 @@ static int mix_host(const char* name, oak_ctx* ctx, const oak_mix_args* args, in
 int oak_dispatch(oak_ctx* ctx, const oak_mix_args* a) { return mix_host("dispatch", ctx, a, 0); }
 int oak_combine(oak_ctx* ctx, const oak_mix_args* a) { return mix_host("combine", ctx, a, 1); }
 int oak_combine_grad(oak_ctx* ctx, const oak_mix_args* a) { return mix_host("combine_grad", ctx, a, 2); }
-int oak_dispatch_device(int32_t device, void* stream, const oak_mix_args* a) { return mix_device("dispatch", device, stream, a, 0); }
-int oak_combine_device(int32_t device, void* stream, const oak_mix_args* a) { return mix_device("combine", device, stream, a, 1); }
-int oak_combine_grad_device(int32_t device, void* stream, const oak_mix_args* a) { return mix_device("combine_grad", device, stream, a, 2); }
+int oak_dispatch_device(oak_ctx* ctx, void* stream, const oak_mix_args* a) { return mix_device("dispatch", ctx, stream, a, 0); }
+int oak_combine_device(oak_ctx* ctx, void* stream, const oak_mix_args* a) { return mix_device("combine", ctx, stream, a, 1); }
+int oak_combine_grad_device(oak_ctx* ctx, void* stream, const oak_mix_args* a) { return mix_device("combine_grad", ctx, stream, a, 2); }
 
 }  // extern "C"

@@ -173,12 +173,13 @@ template <typename F> inline int c_entry(F&& fn) {
     catch (...) { set_error("unknown C++ exception"); return OAK_E_HIP; }
 }
 
-// the device entry points run on whatever device and stream their caller names and leave the thread's current device as it was
+// the device entry points run on the context's device and leave the thread's current one as it was
 struct DeviceGuard {
     int before = -1; bool switched = false;
-    int enter(int device) {
+    int enter(const oak_ctx* ctx) {
+        OAK_REQUIRE(ctx != nullptr, "ctx is NULL");
         OAK_HIP_CHECK(hipGetDevice(&before));
-        if (before != device) { OAK_HIP_CHECK(hipSetDevice(device)); switched = true; }
+        if (before != ctx->device) { OAK_HIP_CHECK(hipSetDevice(ctx->device)); switched = true; }
         return OAK_OK;
     }
     ~DeviceGuard() { if (switched) (void)hipSetDevice(before); }

@@ -14,7 +14,7 @@ from . import _capi
 
 F64, F32, BF16, F16 = 0, 1, 2, 3
 _codes = {}                 # torch dtype -> element type of the C interface
-_checked = set()            # devices whose torch memory the library's HIP runtime is known to see
+_contexts = {}              # contexts of the devices whose torch memory the library's HIP runtime is known to see
 
 
 def on_device(a) -> bool:
@@ -42,13 +42,26 @@ class Device:
         torch = _torch()
         self.torch, self.device = torch, t.device
         self.index = t.device.index
-        if self.index not in _checked and t.numel() > 0:
+        self.ctx = _contexts.get(self.index)
+        if self.ctx is None or self.ctx._h is None:
+            self.ctx = self._first(t)
+
+    def _first(self, t):
+        """The first call on a device: its context, and whether the tensor's memory is the library's to see."""
+        two = "torch and the OAK library hold different copies of the HIP runtime; import torch before the first use of the oak package"
+        if len(_capi.hip_runtimes()) > 1:
+            raise _capi.OakHipError(two)
+        if self.torch.cuda.is_current_stream_capturing():
+            raise _capi.OakHipError("the first call on a device makes its context, which a stream cannot capture: make one call before the capture")
+        with self.torch.cuda.device(self.device):           # making a context changes the current device
+            ctx = _capi.device_context(self.index)
+        if t.numel() > 0:
             try:
-                _capi.check_device_pointer(self.index, t.data_ptr())
+                _capi.check_device_pointer(ctx, t.data_ptr())
             except ValueError as e:
-                raise _capi.OakHipError(f"{e}: torch and the OAK library hold different copies of the HIP runtime; import torch before the "
-                                        "first use of the oak package") from None
-            _checked.add(self.index)
+                raise _capi.OakHipError(f"{e}: {two}") from None
+            _contexts[self.index] = ctx
+        return ctx
 
     @property
     def stream(self) -> int:

@@ -11,6 +11,7 @@ import ctypes as C
 import weakref
 import itertools
 import os
+import threading
 from pathlib import Path
 from typing import Optional, Sequence
 
@@ -166,13 +167,13 @@ SIGNATURES = {
                              _D, _I]),
 }
 
-# oak_X(ctx, args) on host arrays, oak_X_device(device, stream, args) on device arrays
+# oak_X(ctx, args) on host arrays, oak_X_device(ctx, stream, args) on device arrays
 for _name, _args in (("route", RouteArgs), ("route_grad", RouteArgs), ("plan", PlanArgs), ("dispatch", MixArgs), ("combine", MixArgs),
                      ("combine_grad", MixArgs), ("distill", DistillArgs)):
     SIGNATURES[f"oak_{_name}"] = (C.c_int, [_CTX, C.POINTER(_args)])
-    SIGNATURES[f"oak_{_name}_device"] = (C.c_int, [C.c_int32, C.c_void_p, C.POINTER(_args)])
-SIGNATURES["oak_plan_workspace"] = (C.c_int64, [C.c_int64, C.c_int32, C.c_int32])
-SIGNATURES["oak_device_pointer_check"] = (C.c_int, [C.c_int32, C.c_void_p])
+    SIGNATURES[f"oak_{_name}_device"] = (C.c_int, [_CTX, C.c_void_p, C.POINTER(_args)])
+SIGNATURES["oak_plan_workspace"] = (C.c_int64, [_CTX, C.c_int64, C.c_int32, C.c_int32])
+SIGNATURES["oak_device_pointer_check"] = (C.c_int, [_CTX, C.c_void_p])
 
 _lib = None
 
@@ -975,20 +976,43 @@ def default_context() -> HipContext:
     return _default_ctx
 
 
-def call_device(name: str, device: int, stream: int, args):
-    """One operator of the ``oak_X_device(device, stream, args)`` form; enqueued, not waited for."""
-    status = getattr(_lib or load_library(), f"oak_{name}_device")(device, stream, C.byref(args))
+_device_ctx = {}
+_device_ctx_lock = threading.Lock()
+
+
+def device_context(device: int) -> HipContext:
+    """The process-wide context the operators use for arrays on this device (the default context on its own device)."""
+    ctx = _device_ctx.get(device)
+    if ctx is None or ctx._h is None:
+        with _device_ctx_lock:
+            ctx = _device_ctx.get(device)
+            if ctx is None or ctx._h is None:
+                default = default_context()
+                ctx = _device_ctx[device] = default if default.device == device and default._h is not None else HipContext(device)
+    return ctx
+
+
+def call_device(name: str, ctx: Optional[HipContext], stream: int, args):
+    """One operator of the ``oak_X_device(ctx, stream, args)`` form; enqueued, not waited for."""
+    status = getattr(_lib or load_library(), f"oak_{name}_device")(ctx and ctx._h, stream, C.byref(args))
     if status != OAK_OK:
         _check(status)
 
 
-def plan_workspace(n_rows: int, top_k: int, n_experts: int) -> int:
-    return load_library().oak_plan_workspace(n_rows, top_k, n_experts)
+def plan_workspace(ctx: Optional[HipContext], n_rows: int, top_k: int, n_experts: int) -> int:
+    return load_library().oak_plan_workspace(ctx and ctx._h, n_rows, top_k, n_experts)
 
 
-def check_device_pointer(device: int, pointer: int):
-    """Raises unless ``pointer`` is memory of ``device`` known to the HIP runtime the library runs on."""
-    _check(load_library().oak_device_pointer_check(device, pointer))
+def hip_runtimes() -> set:
+    """Paths of the HIP runtimes mapped into this process.  More than one (the library was loaded before torch, which brings its own copy)
+    means that neither knows the other's memory and streams."""
+    with open("/proc/self/maps") as f:
+        return {line.split()[-1] for line in f if "/libamdhip64.so" in line}
+
+
+def check_device_pointer(ctx: Optional[HipContext], pointer: int):
+    """Raises unless ``pointer`` is memory of the context's device known to the HIP runtime the library runs on."""
+    _check(load_library().oak_device_pointer_check(ctx and ctx._h, pointer))
 
 
 def debug_state() -> str:

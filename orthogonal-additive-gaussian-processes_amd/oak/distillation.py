@@ -92,7 +92,7 @@ def _distill(logits, top, index, top_lse, temperature, direction, row_weight, gr
     a.logits, a.top, a.index, a.top_lse, a.row_weight = A.ptr(logits), A.ptr(top), A.ptr(index), A.ptr(top_lse), A.ptr(row_weight)
     a.loss, a.dlogits = A.ptr(loss), A.ptr(dlogits)
     if device:
-        _capi.call_device("distill", d.index, d.stream, a)
+        _capi.call_device("distill", d.ctx, d.stream, a)
     else:
         _capi.default_context().call("distill", a)
     return loss, dlogits

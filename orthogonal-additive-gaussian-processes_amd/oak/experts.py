@@ -103,7 +103,7 @@ def route(scores, top_k: int, *, score: str = "softmax", bias=None, n_groups: in
             a.bias_f64, a.bias = int(bias.dtype == d.torch.float64), A.ptr(bias)
         experts, weights = d.empty((n, a.top_k), d.torch.int32), d.empty((n, a.top_k), d.wide(code))
         a.experts, a.weights = A.ptr(experts), A.ptr(weights)
-        _capi.call_device("route", d.index, d.stream, a)
+        _capi.call_device("route", d.ctx, d.stream, a)
         return experts, weights
     scores = A.host(scores, "scores")
     n, e = scores.shape
@@ -138,7 +138,7 @@ def route_grad(scores, experts, dweights, *, score: str = "softmax", renormalise
         mask = _device_mask(d, mask, n, e, a)
         out = d.empty((n, e), scores.dtype)
         a.experts, a.dweights, a.dscores, a.ld_dscores = A.ptr(experts), A.ptr(dweights), A.ptr(out), e
-        _capi.call_device("route_grad", d.index, d.stream, a)
+        _capi.call_device("route_grad", d.ctx, d.stream, a)
         return out
     scores = A.host(scores, "scores")
     n, e = scores.shape
@@ -205,7 +205,7 @@ def plan(experts, n_experts: int) -> Plan:
         experts = _device_experts(d, experts, shape, n_experts)
         i32 = d.torch.int32
         out = [d.empty((n * k,), i32), d.empty(shape, i32), d.empty((n_experts,), i32), d.empty((n_experts + 1,), i32)]
-        a.workspace_ints = _capi.plan_workspace(n, k, n_experts)
+        a.workspace_ints = _capi.plan_workspace(d.ctx, n, k, n_experts)
         workspace = d.empty((a.workspace_ints,), i32) if a.workspace_ints else None
         a.workspace = A.ptr(workspace)
     else:
@@ -214,7 +214,7 @@ def plan(experts, n_experts: int) -> Plan:
     a.experts = A.ptr(experts)
     a.rows, a.positions, a.counts, a.offsets = map(A.ptr, out)
     if A.on_device(experts):
-        _capi.call_device("plan", d.index, d.stream, a)
+        _capi.call_device("plan", d.ctx, d.stream, a)
     else:
         _capi.default_context().call("plan", a)
     return Plan(*out, n, k, n_experts)
@@ -284,7 +284,7 @@ def _mix(name, plan, first, what, slots_in, weights=None, dout=None):
         if dweights is not None:
             dweights[...] = 0
     elif device:
-        _capi.call_device(name, d.index, d.stream, a)
+        _capi.call_device(name, d.ctx, d.stream, a)
     else:
         _capi.default_context().call(name, a)
     out = out[:, 0] if flat else out

@@ -11,7 +11,7 @@ FAKE = ctypes.create_string_buffer(64)          # an address that is never read:
 
 def refused(name, args, match):
     with pytest.raises(ValueError, match=match):
-        _capi.call_device(name, 0, 0, args)
+        _capi.call_device(name, None, 0, args)
 
 
 def route_args(**kw):
@@ -95,10 +95,12 @@ def test_null_arguments_and_contexts():
     lib = _capi.load_library()
     for name in ("route", "route_grad", "plan", "dispatch", "combine", "combine_grad", "distill"):
         assert getattr(lib, f"oak_{name}")(None, None) == _capi.OAK_E_ARG
-        assert getattr(lib, f"oak_{name}_device")(0, None, None) == _capi.OAK_E_ARG
+        assert getattr(lib, f"oak_{name}_device")(None, None, None) == _capi.OAK_E_ARG
     with pytest.raises(ValueError):
-        _capi.check_device_pointer(0, 0)
-    assert _capi.plan_workspace(-1, 1, 1) == 0 and _capi.plan_workspace(10, 2, 4) == 0 and _capi.plan_workspace(1 << 20, 2, 24) > 0
+        _capi.check_device_pointer(None, ctypes.addressof(FAKE))
+    assert _capi.plan_workspace(None, 1 << 20, 2, 24) == 0
+    for name, args in (("route", route_args()), ("plan", plan_args()), ("combine", mix_args()), ("distill", distill_args())):
+        refused(name, args, "ctx is NULL")
 
 
 def test_python_layer_refuses():
@@ -145,3 +147,15 @@ def test_a_library_without_a_device_says_so():
         experts.route(np.zeros((4, 6)), 2)
     with pytest.raises(_capi.OakHipError):
         distillation.distill(np.zeros((4, 6)), np.zeros((4, 2)), np.zeros((4, 2), int))
+
+
+@pytest.mark.parametrize("torch_first", [True, False])
+def test_a_second_copy_of_the_hip_runtime_is_noticed(torch_first):
+    """torch brings its own HIP runtime: loaded first it serves the library too, loaded second there are two (nothing here touches a device)."""
+    import subprocess
+    import sys
+    lines = ["import torch", "from oak import _capi; _capi.load_library()"]
+    code = "; ".join((lines if torch_first else lines[::-1]) + ["from oak import _capi; print(len(_capi.hip_runtimes()))"])
+    out = subprocess.run([sys.executable, "-c", f"import sys; sys.path.insert(0, {str(_capi._PKG_ROOT)!r}); {code}"], capture_output=True, text=True)
+    assert out.returncode == 0, out.stderr
+    assert int(out.stdout) == (1 if torch_first else 2)
