@@ -18,7 +18,7 @@ _contexts = {}              # contexts of the devices whose torch memory the lib
 
 
 def on_device(a) -> bool:
-    return getattr(a, "is_cuda", False) is True and hasattr(a, "data_ptr")
+    return getattr(a, "is_cuda", False) is True
 
 
 def _torch():
@@ -38,10 +38,11 @@ def code_of(t, what: str) -> int:
 class Device:
     """The device and stream of one call, with its checks of every tensor."""
 
+    __slots__ = ("torch", "index", "ctx", "like")
+
     def __init__(self, t):
-        torch = _torch()
-        self.torch, self.device = torch, t.device
-        self.index = t.device.index
+        self.torch, self.like = _torch(), t
+        self.index = t.get_device()
         self.ctx = _contexts.get(self.index)
         if self.ctx is None or self.ctx._h is None:
             self.ctx = self._first(t)
@@ -53,7 +54,7 @@ class Device:
             raise _capi.OakHipError(two)
         if self.torch.cuda.is_current_stream_capturing():
             raise _capi.OakHipError("the first call on a device makes its context, which a stream cannot capture: make one call before the capture")
-        with self.torch.cuda.device(self.device):           # making a context changes the current device
+        with self.torch.cuda.device(self.index):            # making a context changes the current device
             ctx = _capi.device_context(self.index)
         if t.numel() > 0:
             try:
@@ -66,12 +67,18 @@ class Device:
     @property
     def stream(self) -> int:
         # the handle alone: building a torch.cuda.Stream around it takes as long as a small kernel
-        raw = getattr(self.torch._C, "_cuda_getCurrentRawStream", None)
-        return raw(self.index) if raw is not None else self.torch.cuda.current_stream(self.device).cuda_stream
+        try:
+            return self.torch._C._cuda_getCurrentRawStream(self.index)
+        except AttributeError:
+            return self.torch.cuda.current_stream(self.index).cuda_stream
 
     def tensor(self, a, what: str):
-        if not on_device(a) or a.device != self.device:
-            raise ValueError(f"{what} must be on {self.device} like the first array of the call")
+        try:
+            here = a.get_device() == self.index
+        except AttributeError:
+            here = False
+        if not here:
+            raise ValueError(f"{what} must be on {self.like.device} like the first array of the call")
         if a.requires_grad and self.torch.is_grad_enabled():
             raise ValueError(f"{what} requires grad: the operators record no graph, their gradients are calls of their own; pass {what}.detach()")
         return a
@@ -79,14 +86,14 @@ class Device:
     def matrix(self, a, what: str, shape=None):
         """A 2-D tensor whose columns are consecutive (copied if they are not)."""
         a = self.tensor(a, what)
-        if a.dim() != 2 or (shape is not None and tuple(a.shape) != shape):
+        if a.dim() != 2 or (shape is not None and a.shape != shape):
             raise ValueError(f"{what} has shape {tuple(a.shape)}, expected {'two dimensions' if shape is None else shape}")
         return a if a.stride(1) == 1 or a.shape[1] <= 1 else a.contiguous()
 
     def dense(self, a, what: str, shape, dtype=None):
         """A contiguous tensor of this shape (and type)."""
         a = self.tensor(a, what)
-        if tuple(a.shape) != shape:
+        if a.shape != shape:
             raise ValueError(f"{what} has shape {tuple(a.shape)}, expected {shape}")
         if dtype is not None and a.dtype != dtype:
             a = a.to(dtype)
@@ -97,7 +104,7 @@ class Device:
         return self.torch.float64 if code == F64 else self.torch.float32
 
     def empty(self, shape, dtype):
-        return self.torch.empty(shape, dtype=dtype, device=self.device)
+        return self.like.new_empty(shape, dtype=dtype)
 
 
 def whole(value, what: str, low: int, high: int) -> int:

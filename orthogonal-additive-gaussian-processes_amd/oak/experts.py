@@ -224,62 +224,60 @@ def _mix(name, plan, first, what, slots_in, weights=None, dout=None):
     """Common body of dispatch (rows -> slots), combine (slots -> rows) and combine_grad."""
     if not isinstance(plan, Plan):
         raise ValueError("plan must come from oak.experts.plan")
+    _, positions, _, offsets, n, k, n_experts = plan
     device = A.on_device(first)
-    if device != A.on_device(plan.positions):
+    if device != A.on_device(positions) or device != A.on_device(offsets):
         raise ValueError(f"{what} and the plan must both be device arrays or both be host arrays")
-    n, k = plan.n_rows, plan.top_k
-    shape = tuple(first.shape) if hasattr(first, "shape") else np.shape(first)
+    d = A.Device(first) if device else None
+    if not device:
+        first = np.asarray(first)
+    shape = first.shape
     rows_in = n * k if slots_in else n
+    flat = len(shape) == 1
     if len(shape) not in (1, 2) or shape[0] != rows_in:
-        raise ValueError(f"{what} has shape {shape}, the plan expects {rows_in} rows")
-    flat, c = len(shape) == 1, 1 if len(shape) == 1 else A.whole(shape[1], f"the number of columns of {what}", 0, 1 << 30)
-    for part, size in ((plan.positions, n * k), (plan.offsets, plan.n_experts + 1)):
-        if not str(part.dtype).endswith("int32") or (part.numel() if device else part.size) != size:
-            raise ValueError("plan has been altered: its arrays do not fit its sizes")
-    a = _capi.MixArgs(n_rows=n, top_k=k, n_experts=plan.n_experts, n_cols=c, ld_rows=c, ld_slots=c, ld_grad=c)
-
-    def two(x):
-        return x[:, None] if flat and x.ndim == 1 else x
-
+        raise ValueError(f"{what} has shape {tuple(shape)}, the plan expects {rows_in} rows")
+    if flat:
+        first = first[:, None]
+        dout = dout if dout is None else (dout if device else np.asarray(dout))[:, None]
+    c = first.shape[1]
+    if c > 1 << 30:
+        raise ValueError(f"{what} has {c} columns; at most 2^30 are supported")
     if device:
-        d = A.Device(first)
-        src = d.matrix(two(first), what)
-        a.dtype = A.code_of(src, what)
-        positions, offsets = d.tensor(plan.positions, "the plan").contiguous(), d.tensor(plan.offsets, "the plan").contiguous()
-        wide = d.wide(a.dtype)
+        i32 = d.torch.int32
+        altered = positions.dtype != i32 or offsets.dtype != i32 or positions.numel() != n * k or offsets.numel() != n_experts + 1
+        if altered or not (positions.is_contiguous() and offsets.is_contiguous()):
+            raise ValueError("plan has been altered: its arrays do not fit its sizes")
+        d.tensor(positions, "the plan")
+        d.tensor(offsets, "the plan")
+        src = d.matrix(first, what)
+        code = A.code_of(src, what)
+        wide, row_stride, grad_stride = d.wide(code), src.stride(0), c
         if weights is not None:
             weights = d.dense(weights, "weights", (n, k), wide)
         if dout is not None:
-            dout = d.matrix(two(dout), "dout", (n, c))
+            dout = d.matrix(dout, "dout", (n, c))
             if dout.dtype != src.dtype:
                 dout = dout.to(src.dtype)
-            a.ld_grad = dout.stride(0)
-        empty = lambda m: d.empty((m, c), src.dtype)                                   # noqa: E731
-        empty_w = lambda: d.empty((n, k), wide)                                        # noqa: E731
-        stride = src.stride(0)
+            grad_stride = dout.stride(0)
     else:
-        src = A.host(two(np.asarray(first)), what)
-        positions, offsets = np.ascontiguousarray(plan.positions), np.ascontiguousarray(plan.offsets)
+        positions, offsets = A.host_index(positions, "positions", -1, max(n * k, 1)), A.host_index(offsets, "offsets", 0, n * k + 1)
+        if positions.size != n * k or offsets.size != n_experts + 1:
+            raise ValueError("plan has been altered: its arrays do not fit its sizes")
+        src = A.host(first, what)
+        code, wide, row_stride, grad_stride = A.F64, np.float64, c, c
         if weights is not None:
             weights = A.host(weights, "weights", (n, k))
         if dout is not None:
-            dout = A.host(two(np.asarray(dout)), "dout", (n, c))
-        a.dtype = A.F64
-        empty = lambda m: np.empty((m, c))                                             # noqa: E731
-        empty_w = lambda: np.empty((n, k))                                             # noqa: E731
-        stride = c
-    if slots_in:
-        a.ld_slots = stride
-    else:
-        a.ld_rows = stride
-    a.src, a.weights, a.dout = A.ptr(src), A.ptr(weights), A.ptr(dout)
-    a.positions, a.offsets = A.ptr(positions), A.ptr(offsets)
-    if name == "combine_grad":
-        out, dweights = empty(n * k), empty_w()
-        a.dslots, a.dweights = A.ptr(out), A.ptr(dweights)
-    else:
-        out, dweights = empty(n if slots_in else n * k), None
-        a.dst = A.ptr(out)
+            dout = A.host(dout, "dout", (n, c))
+
+    def empty(rows, columns, dtype):
+        return d.empty((rows, columns), dtype) if device else np.empty((rows, columns), dtype)
+
+    out = empty(n if slots_in and dout is None else n * k, c, src.dtype)
+    dweights = None if dout is None else empty(n, k, wide)
+    a = _capi.MixArgs(n, c if slots_in else row_stride, row_stride if slots_in else c, grad_stride, k, n_experts, c, code,
+                      A.ptr(positions), A.ptr(offsets), A.ptr(weights), A.ptr(src), None if dweights is not None else A.ptr(out), A.ptr(dout),
+                      A.ptr(out) if dweights is not None else None, A.ptr(dweights))
     if c == 0:
         if dweights is not None:
             dweights[...] = 0
@@ -287,7 +285,8 @@ def _mix(name, plan, first, what, slots_in, weights=None, dout=None):
         _capi.call_device(name, d.ctx, d.stream, a)
     else:
         _capi.default_context().call(name, a)
-    out = out[:, 0] if flat else out
+    if flat:
+        out = out[:, 0]
     return out if dweights is None else (out, dweights)
 
 
