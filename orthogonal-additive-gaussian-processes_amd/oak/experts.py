@@ -204,7 +204,8 @@ def plan(experts, n_experts: int) -> Plan:
         d = A.Device(experts)
         experts = _device_experts(d, experts, shape, n_experts)
         i32 = d.torch.int32
-        out = [d.empty((n * k,), i32), d.empty(shape, i32), d.empty((n_experts,), i32), d.empty((n_experts + 1,), i32)]
+        out = d.empty((2 * n * k + 2 * n_experts + 1,), i32).split_with_sizes((n * k, n * k, n_experts, n_experts + 1))   # one allocation
+        out = [out[0], out[1].view(shape), out[2], out[3]]
         a.workspace_ints = _capi.plan_workspace(d.ctx, n, k, n_experts)
         workspace = d.empty((a.workspace_ints,), i32) if a.workspace_ints else None
         a.workspace = A.ptr(workspace)
