@@ -517,7 +517,7 @@ static int route_grad_launch(hipStream_t stream, const oak_route_args* a) {
 // ---------------------------------------------------------------------------------------------------------------------
 // plan: stable counting sort of the n k slots by expert
 // ---------------------------------------------------------------------------------------------------------------------
-// Every wave owns one consecutive piece of the slots, so that the order inside an expert is the slots' own without any atomic
+// Bound by latency, three short launches (524288 slots, 24 experts: 3 + 4 + 7 us for 6 MB): every wave owns one consecutive piece of the slots, so that the order inside an expert is the slots' own without any atomic
 // whose order could show: pieces are counted, the counts are summed in piece order, and each wave then places its slots 64 at a
 // time -- a slot's rank among the 64 is the number of lower lanes with the same expert (one ballot per bit of the expert's number).
 constexpr int64_t PLAN_SMALL_SLOTS = 16384;
@@ -715,7 +715,8 @@ static int plan_launch(hipStream_t stream, const oak_plan_args* a) {
 // ---------------------------------------------------------------------------------------------------------------------
 // All of them walk rows: a row is read or written once where the slots' order would touch it k times.  tpr threads share a row; a unit is
 // 16 bytes, the row's last elements that do not fill one are units of their own.  A thread asks for the places, then for the answers of up
-// to 4 slots before it adds the first.  Bound by memory: 32768 rows, k = 6, 2048 bf16 columns at MIX_RATES.
+// to 8 slots before it adds the first (k = 6: 198 us, 4 at a time 210).  Bound by memory: 32768 rows, k = 6, 2048 bf16 columns, of 0.94 GB
+// each: dispatch 158 us (5.9 TB/s), combine 198 (4.7), and of 1.74 GB combine_grad 353 (4.9), where a large copy reaches 5.06 TB/s.
 struct MixDev {
     int64_t row0, n, slots, ld_rows, ld_slots, ld_grad;
     int64_t units;              // 16-byte units of a row, then its last elements
@@ -806,8 +807,8 @@ template <typename T, int CHUNK> __global__ void __launch_bounds__(256) combine_
     }
 }
 
-// dF[place] = w dy, dw = <dy, F[place]>: slot by slot, the row of dy stays in the nearest cache.  TPR <= 64: the dot product is
-// finished inside a wave.
+// dF[place] = w dy, dw = <dy, F[place]>: slot by slot, the row of dy stays in the nearest cache, 4 units of both asked for together.  At
+// most 64 threads a row: the dot product is finished inside a wave.
 template <typename T> __global__ void __launch_bounds__(256) combine_grad_kernel(MixDev a) {
     using acc = typename Num<T>::acc;
     const int64_t n = a.row0 + (int64_t)blockIdx.x * a.rows_per_wg + (threadIdx.x >> a.tpr_log2);
@@ -823,19 +824,29 @@ template <typename T> __global__ void __launch_bounds__(256) combine_grad_kernel
         acc d = 0;
         if (p >= 0) {
             const acc wj = w[n * a.k + j];
-            for (int64_t u = t; u < a.units; u += tpr) {
-                if (u < a.nvec) {
-                    const auto f = Vec<T>::load(F + p * a.ld_slots + u * Vec<T>::N), v = Vec<T>::load(dy + u * Vec<T>::N);
+            const T* fr = F + p * a.ld_slots;
+            T* gr = dF + p * (int64_t)a.C;
+            constexpr int U = 4;                       // units asked for together
+            for (int64_t u0 = t; u0 < a.nvec; u0 += U * tpr) {
+                typename Vec<T>::raw f[U], v[U];
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    const int64_t u = u0 + i * tpr < a.nvec ? u0 + i * tpr : u0;
+                    f[i] = Vec<T>::load(fr + u * Vec<T>::N);
+                    v[i] = Vec<T>::load(dy + u * Vec<T>::N);
+                }
+#pragma unroll
+                for (int i = 0; i < U; ++i) if (u0 + i * tpr < a.nvec) {
                     typename Vec<T>::raw o;
 #pragma unroll
-                    for (int i = 0; i < Vec<T>::N; ++i) { d += (acc)f[i] * (acc)v[i]; o[i] = (T)(wj * (acc)v[i]); }
-                    Vec<T>::store(dF + p * (int64_t)a.C + u * Vec<T>::N, o);
-                } else {
-                    const int64_t c = a.nvec * (int64_t)Vec<T>::N + (u - a.nvec);
-                    const acc v = (acc)dy[c];
-                    d += (acc)F[p * a.ld_slots + c] * v;
-                    dF[p * (int64_t)a.C + c] = (T)(wj * v);
+                    for (int e = 0; e < Vec<T>::N; ++e) { d += (acc)f[i][e] * (acc)v[i][e]; o[e] = (T)(wj * (acc)v[i][e]); }
+                    Vec<T>::store_stream(gr + (u0 + i * tpr) * Vec<T>::N, o);
                 }
+            }
+            for (int64_t c = (int64_t)a.nvec * Vec<T>::N + t; c < a.C; c += tpr) {
+                const acc v = (acc)dy[c];
+                d += (acc)fr[c] * v;
+                gr[c] = (T)(wj * v);
             }
         }
         for (int m = 1; m < tpr; m <<= 1) d += __shfl_xor(d, m, 64);
@@ -871,7 +882,7 @@ static int mix_launch(hipStream_t stream, const oak_mix_args* a, int what /* 0 d
     d.inv_tpr = (65536 + d.tpr - 1) / d.tpr;           // t / tpr = t inv_tpr >> 16 for t < 256
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        auto kernel = what == 0 ? dispatch_kernel<T> : what == 2 ? combine_grad_kernel<T> : d.k <= 2 ? combine_kernel<T, 2> : combine_kernel<T, 4>;
+        auto kernel = what == 0 ? dispatch_kernel<T> : what == 2 ? combine_grad_kernel<T> : d.k <= 2 ? combine_kernel<T, 2> : d.k <= 4 ? combine_kernel<T, 4> : combine_kernel<T, 8>;
         return launch_rows(kernel, d.rows_per_wg, 0, stream, d);
     });
 }
