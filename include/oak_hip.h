@@ -529,7 +529,10 @@ typedef struct oak_distill_args {
     const void* row_weight;    /* [n_rows] weight_dtype, or NULL: all 1     */
     void* loss;                /* [n_rows] wide, out                        */
     void* dlogits;             /* [n_rows, n_classes] dtype, out, or NULL   */
+    double* workspace;         /* oak_distill_device: scratch of its own     */
+    int64_t workspace_doubles; /* at least oak_distill_workspace(...): a few rows of many classes need some, 0 otherwise */
 } oak_distill_args;
+int64_t oak_distill_workspace(oak_ctx* ctx, int64_t n_rows, int32_t n_classes, int32_t dtype);   /* 0 for ctx NULL */
 int oak_distill(oak_ctx* ctx, const oak_distill_args* args);
 int oak_distill_device(oak_ctx* ctx, void* stream, const oak_distill_args* args);
 

@@ -26,6 +26,8 @@ struct DistillDev {
     float c_hi, c_lo;           // log2(e) / tau in two floats, c_hi rounded towards zero
     const void* logits; const void* top; const void* index; const void* lse; const void* weight;
     void* loss; void* dlogits;
+    double* part;               // split rows: maximum and sum of every slice [n][slices][2]
+    int slices, slice;          // and the units of a slice
 };
 
 // exp(t / tau) for t <= 0.  float: 2^(t c) with c in two parts, since a c off by half a unit would put a common relative error of |t| c 2^-25
@@ -46,12 +48,83 @@ __host__ __device__ inline size_t distill_lds(int V, int K, int NT) {
 // what the team does with its row's gradient
 enum { ROW_COMPUTE = 0, ROW_ZERO = 1, ROW_NAN = 2 };
 
-template <typename T, int NT, int NV, bool LONG>
-__global__ void __launch_bounds__(NT < 256 ? 256 : NT, LONG ? 4 : 1) distill_kernel(DistillDev a) {
+// where a team's row is: in its registers; there and, what does not fit, read twice; cut into slices, a workgroup each, whose sums
+// distill_slice_kernel has made
+enum { HELD = 0, LONG = 1, SPLIT = 2 };
+
+__device__ __forceinline__ float lowest(float) { return -3.402823466e38f; }
+__device__ __forceinline__ double lowest(double) { return -1.7976931348623157e308; }
+
+// one more unit into a running maximum m and sum z
+template <int VN, typename A, typename R> __device__ __forceinline__ void take_unit(const DistillDev& a, const R& r, A& m, A& z) {
+    A top = m;
+#pragma unroll
+    for (int j = 0; j < VN; ++j) top = OpMax()(top, (A)r[j]);
+    z *= exp_scaled(a, m - top);
+    m = top;
+#pragma unroll
+    for (int j = 0; j < VN; ++j) z += exp_scaled(a, (A)r[j] - m);
+}
+
+// Few rows: maximum and sum of the rest over one slice of one row.
+template <typename T, int NT> __global__ void __launch_bounds__(NT) distill_slice_kernel(DistillDev a) {
+    using acc = typename Num<T>::acc;
+    constexpr int VN = Vec<T>::N, U = 4;
+    extern __shared__ __align__(16) unsigned char lds_all[];
+    __shared__ double share[NT / 64][2];
+    unsigned* bits = reinterpret_cast<unsigned*>(lds_all);
+    const int tid = threadIdx.x, nvec = a.V / VN, u_begin = blockIdx.x * a.slice, u_end = u_begin + a.slice < nvec ? u_begin + a.slice : nvec;
+    const bool last_slice = blockIdx.x + 1 == gridDim.x;
+    const int64_t row = blockIdx.y;
+    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+    if (a.weight && load_any(a.weight, a.weight_dtype, row) == 0.0) return;
+    const int64_t v_begin = (int64_t)u_begin * VN, v_end = last_slice ? a.V : (int64_t)u_end * VN;
+    for (int i = tid; i < (int)((v_end - v_begin + 31) / 32); i += NT) bits[i] = 0;
+    __syncthreads();
+    if (a.lse != nullptr)
+        for (int k = tid; k < a.K; k += NT) {
+            const int64_t c = a.index_64 ? static_cast<const int64_t*>(a.index)[row * a.ld_index + k] : static_cast<const int32_t*>(a.index)[row * a.ld_index + k];
+            if (c >= v_begin && c < v_end && !(load_any(a.top, a.top_dtype, row * a.ld_top + k) == -INFINITY))
+                atomicOr(&bits[(c - v_begin) >> 5], 1u << ((c - v_begin) & 31));
+        }
+    __syncthreads();
+    acc m = lowest(acc()), z = 0;
+    for (int u0 = u_begin + tid; u0 < u_end; u0 += U * NT) {
+        typename Vec<T>::raw r[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) { const int u = u0 + i * NT; r[i] = Vec<T>::load(x + (size_t)(u < u_end ? u : u_end - 1) * VN); }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int u = u0 + i * NT;
+            if (u >= u_end) break;
+            const int v = (u - u_begin) * VN;
+            const unsigned b = bits[v >> 5] >> (v & 31);
+#pragma unroll
+            for (int j = 0; j < VN; ++j) r[i][j] = b >> j & 1 ? (T)-INFINITY : r[i][j];
+            take_unit<VN>(a, r[i], m, z);
+        }
+    }
+    const int64_t extra = (int64_t)nvec * VN + tid;                                // elements that do not fill a unit
+    if (last_slice && extra < a.V && !(bits[(extra - v_begin) >> 5] >> ((extra - v_begin) & 31) & 1)) {
+        const acc one[1] = {(acc)x[extra]};
+        take_unit<1>(a, one, m, z);
+    }
+    const acc mw = lanes_reduce<64>(m, OpMax());
+    const acc zw = lanes_reduce<64>(z * exp_scaled(a, m - mw), OpSum());
+    if ((tid & 63) == 0) { share[tid >> 6][0] = (double)mw; share[tid >> 6][1] = (double)zw; }
+    __syncthreads();
+    if (tid < NT / 64) {
+        const double mine = share[tid][0], all = lanes_reduce<NT / 64>(mine, OpMax());
+        const double sum = lanes_reduce<NT / 64>(share[tid][1] * exp_of((mine - all) * a.inv_tau), OpSum());
+        if (tid == 0) { double* p = a.part + (row * a.slices + blockIdx.x) * 2; p[0] = all; p[1] = sum; }
+    }
+}
+
+template <typename T, int NT, int NV, int MODE>
+__global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) distill_kernel(DistillDev a) {
     using acc = typename Num<T>::acc;
     using raw = typename Vec<T>::raw;
     constexpr int VN = Vec<T>::N, ROWS = NT < 256 ? 256 / NT : 1, LEAD = NT < 64 ? NT : 64, WAVES = NT / 64;
-    constexpr acc LOWEST = sizeof(acc) == 8 ? (acc)-1.7976931348623157e308 : (acc)-3.402823466e38f;
     extern __shared__ __align__(16) unsigned char lds_all[];
     const int tid = threadIdx.x & (NT - 1);
     unsigned char* lds = lds_all + (NT < 256 ? threadIdx.x / NT : 0) * distill_lds(a.V, a.K, NT);
@@ -62,14 +135,18 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, LONG ? 4 : 1) distill_ker
     double* ek = pk + a.K;
     double* share = ek + a.K;
     int* cls = reinterpret_cast<int*>(share + (NT > 64 ? WAVES * 2 + 4 : 0));
-    const int nvec = a.V / VN, tail = a.V - nvec * VN;
+    const int nvec = a.V / VN;
+    // the units read from memory (not held), and the elements that do not fill one
+    const int u_begin = MODE == SPLIT ? blockIdx.x * a.slice : NV * NT, u_end = MODE == SPLIT && u_begin + a.slice < nvec ? u_begin + a.slice : nvec;
+    const int tail = MODE == SPLIT && blockIdx.x + 1 != gridDim.x ? 0 : a.V - nvec * VN;
     const bool lead = tid < LEAD;
     auto team_sync = [] { if constexpr (NT <= 64) wave_sync(); else __syncthreads(); };
 
     for (int i = tid; i < words; i += NT) bits[i] = 0;
     team_sync();
 
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + (NT < 256 ? threadIdx.x / NT : 0); row < a.n; row += (int64_t)gridDim.x * ROWS) {
+    const int64_t stride = MODE == SPLIT ? a.n : (int64_t)gridDim.x * ROWS;
+    for (int64_t row = MODE == SPLIT ? (int64_t)blockIdx.y : (int64_t)blockIdx.x * ROWS + (NT < 256 ? threadIdx.x / NT : 0); row < a.n; row += stride) {
         const T* x = static_cast<const T*>(a.logits) + row * a.ld;
         T* g = a.dlogits ? static_cast<T*>(a.dlogits) + row * a.ld_out : nullptr;
         const double w = a.weight ? load_any(a.weight, a.weight_dtype, row) : 1.0;
@@ -85,7 +162,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, LONG ? 4 : 1) distill_ker
         words4 data[NV];
         acc last = -INFINITY;                          // one of the elements that do not fill a unit
         if (todo == ROW_COMPUTE) {
-            if (nvec > 0) {
+            if (MODE != SPLIT && nvec > 0) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     const int u = i * NT + at;
@@ -161,8 +238,8 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, LONG ? 4 : 1) distill_ker
             todo = (int)share[WAVES * 2];
         }
 
-        acc m = LOWEST, z = 0;                         // a finite start: -inf - m stays -inf
-        if (todo == ROW_COMPUTE) {
+        acc m = lowest(acc()), z = 0;                  // a finite start: -inf - m stays -inf
+        if (MODE != SPLIT && todo == ROW_COMPUTE) {
             auto forget = [&] {                         // the units, not their 32-bit forms, live from one walk to the next
 #pragma unroll
                 for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(data[i]));
@@ -206,25 +283,16 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, LONG ? 4 : 1) distill_ker
                 z += exp_scaled(a, last - m);
                 forget();
             }
-            if constexpr (LONG) {
-                auto take = [&](raw r) {
-                    acc top = m;
-#pragma unroll
-                    for (int j = 0; j < VN; ++j) top = OpMax()(top, (acc)r[j]);
-                    z *= exp_scaled(a, m - top);
-                    m = top;
-#pragma unroll
-                    for (int j = 0; j < VN; ++j) z += exp_scaled(a, (acc)r[j] - m);
-                };
+            if constexpr (MODE == LONG) {
                 constexpr int U = 4;
-                for (int u0 = NV * NT + tid; u0 < nvec; u0 += U * NT) {
+                for (int u0 = u_begin + tid; u0 < nvec; u0 += U * NT) {
                     raw r[U];
 #pragma unroll
                     for (int i = 0; i < U; ++i) { const int u = u0 + i * NT; r[i] = Vec<T>::load(x + (size_t)(u < nvec ? u : nvec - 1) * VN); }
 #pragma unroll
                     for (int i = 0; i < U; ++i) {
                         const int u = u0 + i * NT;
-                        if (u < nvec) { if (leave_out) hide(r[i], u); take(r[i]); }
+                        if (u < nvec) { if (leave_out) hide(r[i], u); take_unit<VN>(a, r[i], m, z); }
                     }
                 }
             }
@@ -233,7 +301,14 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, LONG ? 4 : 1) distill_ker
         acc mr = lanes_reduce<LEAD>(m, OpMax());
         z = lanes_reduce<LEAD>(z * exp_scaled(a, m - mr), OpSum());
         double zr = (double)z;
-        if constexpr (NT > 64) {
+        if constexpr (MODE == SPLIT) {
+            if (lead && todo == ROW_COMPUTE) {
+                const double* p = a.part + row * a.slices * 2;
+                const double mw = tid < a.slices ? p[tid * 2] : (double)lowest(acc()), all = lanes_reduce<64>(mw, OpMax());
+                zr = lanes_reduce<64>(tid < a.slices ? p[tid * 2 + 1] * exp_of((mw - all) * a.inv_tau) : 0.0, OpSum());
+                mr = (acc)all;
+            }
+        } else if constexpr (NT > 64) {
             if ((tid & 63) == 0) { share[tid >> 6] = (double)mr; share[WAVES + (tid >> 6)] = zr; }
             __syncthreads();
             if (lead) {
@@ -274,7 +349,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, LONG ? 4 : 1) distill_ker
             }
             coef *= a.tau * w;
         }
-        if (tid == 0) static_cast<acc*>(a.loss)[row] = todo == ROW_COMPUTE ? (acc)(a.tau * a.tau * w * kl) : todo == ROW_ZERO ? (acc)0 : (acc)NAN;
+        if (tid == 0 && (MODE != SPLIT || blockIdx.x == 0)) static_cast<acc*>(a.loss)[row] = todo == ROW_COMPUTE ? (acc)(a.tau * a.tau * w * kl) : todo == ROW_ZERO ? (acc)0 : (acc)NAN;
         if (g != nullptr) {
             if constexpr (NT > 64) {
                 if (tid == 0) { share[WAVES * 2 + 1] = coef; share[WAVES * 2 + 2] = (double)mr; }
@@ -289,9 +364,9 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, LONG ? 4 : 1) distill_ker
                 for (int j = 0; j < VN; ++j) o[j] = (T)(todo == ROW_COMPUTE ? cf * exp_gradient<T>(a, (acc)r[j] - mr) : fill);
                 // a long row's gradient passes the caches by (16384 x 8192 bf16: 140 us, otherwise 158); short rows end inside a cache line, which
                 // the next row fills there (262144 x 1000 float32: 430 us, otherwise 510)
-                if constexpr (LONG || NT * NV >= 1024) Vec<T>::store_stream(g + (size_t)u * VN, o); else Vec<T>::store(g + (size_t)u * VN, o);
+                if constexpr (MODE != HELD || NT * NV >= 1024) Vec<T>::store_stream(g + (size_t)u * VN, o); else Vec<T>::store(g + (size_t)u * VN, o);
             };
-            {
+            if constexpr (MODE != SPLIT) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     const int u = i * NT + at;
@@ -299,16 +374,16 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, LONG ? 4 : 1) distill_ker
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if constexpr (LONG) {
+            if constexpr (MODE != HELD) {
                 constexpr int U = 4;
-                for (int u0 = NV * NT + tid; u0 < nvec; u0 += U * NT) {
+                for (int u0 = u_begin + tid; u0 < u_end; u0 += U * NT) {
                     raw r[U] = {};
                     if (todo == ROW_COMPUTE) {
 #pragma unroll
-                        for (int i = 0; i < U; ++i) { const int u = u0 + i * NT; r[i] = Vec<T>::load(x + (size_t)(u < nvec ? u : nvec - 1) * VN); }
+                        for (int i = 0; i < U; ++i) { const int u = u0 + i * NT; r[i] = Vec<T>::load(x + (size_t)(u < u_end ? u : u_end - 1) * VN); }
                     }
 #pragma unroll
-                    for (int i = 0; i < U; ++i) { const int u = u0 + i * NT; if (u < nvec) put(r[i], u); }
+                    for (int i = 0; i < U; ++i) { const int u = u0 + i * NT; if (u < u_end) put(r[i], u); }
                 }
             }
             if (tid < tail) g[nvec * VN + tid] = (T)(todo == ROW_COMPUTE ? cf * exp_gradient<T>(a, last - mr) : fill);
@@ -316,6 +391,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, LONG ? 4 : 1) distill_ker
             if (lead && todo == ROW_COMPUTE) {
                 const double scale = exp_of(-log_z), ip = 1.0 / psum;
                 for (int k = tid; k < a.K; k += LEAD) if (cls[k] >= 0) {
+                    if (MODE == SPLIT && !(cls[k] / VN >= u_begin && cls[k] / VN < u_end) && !(tail > 0 && cls[k] >= nvec * VN)) continue;   // another slice's
                     const double q = ek[k] * scale;
                     const double d = a.reverse ? (q != 0.0 ? q * (log_of(ek[k]) - log_z - tk[k] - kl) : 0.0) : q - pk[k] * ip;
                     g[cls[k]] = (T)(acc)(a.tau * w * d);
@@ -323,7 +399,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, LONG ? 4 : 1) distill_ker
             }
         }
         // the bits back to 0 for the next row (a padded or wrong index has set none)
-        if (lead && row + (int64_t)gridDim.x * ROWS < a.n && w != 0.0) {
+        if (lead && row + stride < a.n && w != 0.0) {
             wave_sync();
             for (int k = tid; k < a.K; k += LEAD) {
                 const int64_t c = a.index_64 ? static_cast<const int64_t*>(a.index)[row * a.ld_index + k] : static_cast<const int32_t*>(a.index)[row * a.ld_index + k];
@@ -352,14 +428,32 @@ static int distill_check(const oak_distill_args* a) {
     return OAK_OK;
 }
 
-template <typename T, int NT, int NV, bool LONG = false> static int distill_run(hipStream_t stream, const DistillDev& d) {
+template <typename T, int NT, int NV, int MODE = HELD> static int distill_run(hipStream_t stream, const DistillDev& d) {
     constexpr int ROWS = NT < 256 ? 256 / NT : 1;
     const size_t lds = distill_lds(d.V, d.K, NT) * ROWS;
-    auto kernel = distill_kernel<T, NT, NV, LONG>;
+    auto kernel = distill_kernel<T, NT, NV, MODE>;
     if (lds > 64 * 1024) OAK_CHECK(ensure_dynamic_lds((const void*)kernel, 160 * 1024));
+    if constexpr (MODE == SPLIT) {
+        const size_t bits = ((size_t)d.slice * Vec<T>::N + Vec<T>::N + 31) / 32 * 4;
+        OAK_CHECK(launch(distill_slice_kernel<T, NT>, dim3((unsigned)d.slices, (unsigned)d.n), dim3(NT), bits, stream, d));
+        return launch(kernel, dim3(d.dlogits ? (unsigned)d.slices : 1u, (unsigned)d.n), dim3(NT), lds, stream, d);
+    }
     // a launch has fewer than 2^32 threads; the kernel walks on from row to row
     const int64_t wgs = (d.n + ROWS - 1) / ROWS, most = (int64_t)1 << 22;
     return launch(kernel, dim3((unsigned)(wgs < most ? wgs : most)), dim3(NT < 256 ? 256 : NT), lds, stream, d);
+}
+
+// Rows so long and so few that compute units would idle are cut into slices: at most 64 (a wave joins them), of at least 512 units,
+// together at most two workgroups a compute unit.  With the gradient, one launch against two: 2 x 131072 bf16 24.8 -> 9.9 us, 64 x 131072
+// 25.9 -> 15.0, 8 x 32768 11.3 -> 9.9, but 64 x 32768 11.7 -> 11.6, 8 x 16384 9.3 -> 9.8 and, in two slices, 200 x 131072 34.4 -> 38.6; the value
+// alone is half of that work, and the second launch costs the host 3 us: from 8192 units on, for both, so that they agree to the last bit.
+static int distill_slices(int64_t n, int V, int dtype) {
+    const int64_t units = V / (16 / (int64_t)dtype_size(dtype));
+    if (n <= 0 || n > 128 || units < 8192) return 1;
+    int64_t s = 512 / n;
+    if (s > 64) s = 64;
+    if (s > units / 512) s = units / 512;
+    return (int)s;
 }
 
 static int distill_launch(hipStream_t stream, const oak_distill_args* a) {
@@ -379,7 +473,15 @@ static int distill_launch(hipStream_t stream, const oak_distill_args* a) {
         const int units = (d.V + Vec<T>::N - 1) / Vec<T>::N;
         // the smallest team whose registers hold the row; few rows, with compute units to spare, are faster with many threads each
         // (8 rows of 32768 bf16: 11.2 us with 512 threads, 13.1 with 256)
-        if (d.n <= 256 && units > 64) return distill_run<T, 512, 8, true>(stream, d);
+        d.slices = distill_slices(d.n, d.V, a->dtype);
+        const int whole = d.V / Vec<T>::N;
+        if (d.slices > 1) {
+            d.slice = (whole + d.slices - 1) / d.slices;
+            d.slices = (whole + d.slice - 1) / d.slice;
+            d.part = (double*)a->workspace;
+            return distill_run<T, 512, 1, SPLIT>(stream, d);
+        }
+        if (d.n <= 256 && units > 64) return distill_run<T, 512, 8, LONG>(stream, d);
         if (units <= 16 && d.K <= 16) return distill_run<T, 4, 4>(stream, d);
         if (units <= 64 && d.K <= 64) return distill_run<T, 16, 4>(stream, d);
         if (units <= 128 && d.K <= 64) return distill_run<T, 16, 8>(stream, d);
@@ -392,7 +494,7 @@ static int distill_launch(hipStream_t stream, const oak_distill_args* a) {
         // Longer rows: what 512 threads can hold with two workgroups a compute unit, the rest is read twice, the second time out of the last cache
         // (2 x 256 rows in flight fit it up to 2^18 bf16 classes, and the gradient passes it by).  2048 x 131072 bf16: 265 us; all of it
         // read twice 279; the whole row in the registers of 1024 threads, one workgroup a unit, 330.
-        return distill_run<T, 512, 8, true>(stream, d);
+        return distill_run<T, 512, 8, LONG>(stream, d);
     });
 }
 
@@ -418,9 +520,18 @@ int oak_device_pointer_check(oak_ctx* ctx, const void* p) {
     });
 }
 
+int64_t oak_distill_workspace(oak_ctx* ctx, int64_t n_rows, int32_t n_classes, int32_t dtype) {
+    if (!ctx || n_rows <= 0 || n_classes <= 0 || dtype < OAK_F64 || dtype > OAK_F16) return 0;
+    const int slices = distill_slices(n_rows, n_classes, dtype);
+    return slices > 1 ? n_rows * slices * 2 : 0;
+}
+
 int oak_distill_device(oak_ctx* ctx, void* stream, const oak_distill_args* a) {
     return c_entry([&] {
         OAK_CHECK(distill_check(a));
+        const int64_t doubles = oak_distill_workspace(ctx, a->n_rows, a->n_classes, a->dtype);
+        OAK_REQUIRE(doubles == 0 || (a->workspace && a->workspace_doubles >= doubles), "distill: the workspace holds %lld of the %lld doubles asked for by "
+                    "oak_distill_workspace", (long long)a->workspace_doubles, (long long)doubles);
         DeviceGuard g;
         OAK_CHECK(g.enter(ctx));
         return distill_launch((hipStream_t)stream, a);
@@ -448,6 +559,10 @@ int oak_distill(oak_ctx* ctx, const oak_distill_args* args) {
         OAK_CHECK(st.in("kd_weight", a.row_weight, n * 8));
         OAK_CHECK(st.out("kd_loss", a.loss, n * 8));
         OAK_CHECK(st.out("kd_dlogits", a.dlogits, cells * 8));
+        a.workspace_doubles = oak_distill_workspace(ctx, a.n_rows, a.n_classes, a.dtype);
+        void* ws = nullptr;
+        OAK_CHECK(get_buf(ctx, "kd_ws", (size_t)a.workspace_doubles * 8, &ws));
+        a.workspace = (double*)ws;
         OAK_CHECK(distill_launch(ctx->stream, &a));
         t.stop();
         return st.finish();

@@ -75,7 +75,8 @@ class DistillArgs(C.Structure):
     _fields_ = ([(n, C.c_int64) for n in ("n_rows", "ld_logits", "ld_top", "ld_index", "ld_dlogits")]
                 + [(n, C.c_int32) for n in ("n_classes", "top_k", "dtype", "top_dtype", "lse_dtype", "weight_dtype", "index_64", "direction")]
                 + [("temperature", C.c_double)]
-                + [(n, C.c_void_p) for n in ("logits", "top", "index", "top_lse", "row_weight", "loss", "dlogits")])
+                + [(n, C.c_void_p) for n in ("logits", "top", "index", "top_lse", "row_weight", "loss", "dlogits", "workspace")]
+                + [("workspace_doubles", C.c_int64)])
 
 
 _D = C.POINTER(C.c_double)
@@ -173,6 +174,7 @@ for _name, _args in (("route", RouteArgs), ("route_grad", RouteArgs), ("plan", P
     SIGNATURES[f"oak_{_name}"] = (C.c_int, [_CTX, C.POINTER(_args)])
     SIGNATURES[f"oak_{_name}_device"] = (C.c_int, [_CTX, C.c_void_p, C.POINTER(_args)])
 SIGNATURES["oak_plan_workspace"] = (C.c_int64, [_CTX, C.c_int64, C.c_int32, C.c_int32])
+SIGNATURES["oak_distill_workspace"] = (C.c_int64, [_CTX, C.c_int64, C.c_int32, C.c_int32])
 SIGNATURES["oak_device_pointer_check"] = (C.c_int, [_CTX, C.c_void_p])
 
 _lib = None
@@ -1001,6 +1003,10 @@ def call_device(name: str, ctx: Optional[HipContext], stream: int, args):
 
 def plan_workspace(ctx: Optional[HipContext], n_rows: int, top_k: int, n_experts: int) -> int:
     return load_library().oak_plan_workspace(ctx and ctx._h, n_rows, top_k, n_experts)
+
+
+def distill_workspace(ctx: Optional[HipContext], n_rows: int, n_classes: int, dtype: int) -> int:
+    return load_library().oak_distill_workspace(ctx and ctx._h, n_rows, n_classes, dtype)
 
 
 def hip_runtimes() -> set:

@@ -92,6 +92,10 @@ def _distill(logits, top, index, top_lse, temperature, direction, row_weight, gr
     a.logits, a.top, a.index, a.top_lse, a.row_weight = A.ptr(logits), A.ptr(top), A.ptr(index), A.ptr(top_lse), A.ptr(row_weight)
     a.loss, a.dlogits = A.ptr(loss), A.ptr(dlogits)
     if device:
+        if n <= 128:                                                     # few rows may be cut into slices, whose sums are kept meanwhile
+            a.workspace_doubles = _capi.distill_workspace(d.ctx, n, v, a.dtype)
+            workspace = d.empty((a.workspace_doubles,), d.torch.float64) if a.workspace_doubles else None
+            a.workspace = A.ptr(workspace)
         _capi.call_device("distill", d.ctx, d.stream, a)
     else:
         _capi.default_context().call("distill", a)

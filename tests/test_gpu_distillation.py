@@ -258,3 +258,51 @@ def test_refusals_on_the_device():
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"case {i} was not refused")
+
+
+@pytest.mark.parametrize("n,v,k,dtype,tail,direction,pad", [
+    (1, 131072, 128, "bf16", True, "forward", 0), (2, 131075, 64, "bf16", True, "reverse", 5), (3, 70001, 1, "f16", False, "forward", 1),
+    (128, 66003, 20, "bf16", True, "forward", 0), (129, 66003, 20, "bf16", True, "forward", 0), (17, 32773, 300, "f32", True, "forward", 3),
+    (5, 16384, 7, "f64", True, "reverse", 0), (5, 16383, 7, "f64", False, "forward", 1), (8, 65535, 9, "bf16", True, "forward", 0), (1, 262147, 3, "f32", True, "forward", 0),
+])
+def test_few_rows_cut_into_slices(n, v, k, dtype, tail, direction, pad):
+    """Sizes around the rule that cuts a row into slices, entries on both sides of the cuts."""
+    s, top, idx, lse = problem(n, v, k, dtype, tail, 1.0, 1, pad)
+    idx = idx.clone()
+    if v > 40000 and k > 3:
+        idx[0, :4] = torch.tensor([0, v - 1, v // 2, v // 2 - 1], device="cuda")   # ends, and the middle cut of an even number of slices
+    w = torch.rand(n, device="cuda", dtype=top.dtype) + 0.5
+    if n > 2:
+        w[1] = 0
+        s[1] = float("nan")
+    compare(s, top, idx, lse, 1.0, direction, w, dtype)
+
+
+def test_slices_merge_entries_of_one_class():
+    s, top, idx, lse = problem(3, 90000, 12, "bf16", True, seed=8)
+    idx = idx.clone()
+    idx[0, 5] = idx[0, 2]
+    idx[1, :] = idx[1, 0]
+    idx[2, 3] = 90000
+    lse = torch.logsumexp(top, 1) + 0.3
+    for direction in ("forward", "reverse"):
+        compare(s, top, idx, lse, 1.0, direction, None, "bf16")
+
+
+def test_two_graphs_of_split_rows_do_not_share_scratch():
+    a, b = problem(2, 100000, 9, "bf16", True, seed=1), problem(4, 90000, 9, "bf16", True, seed=2)
+    ref = [od.distill_grad(p[0], p[1], p[2], top_lse=p[3]) for p in (a, b)]
+    graphs, held = [], []
+    for p in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(od.distill_grad(p[0], p[1], p[2], top_lse=p[3]))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(10):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for h, r in zip(held, ref):
+            assert torch.equal(h[0], r[0]) and torch.equal(h[1], r[1])

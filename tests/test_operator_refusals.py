@@ -98,7 +98,7 @@ def test_null_arguments_and_contexts():
         assert getattr(lib, f"oak_{name}_device")(None, None, None) == _capi.OAK_E_ARG
     with pytest.raises(ValueError):
         _capi.check_device_pointer(None, ctypes.addressof(FAKE))
-    assert _capi.plan_workspace(None, 1 << 20, 2, 24) == 0
+    assert _capi.plan_workspace(None, 1 << 20, 2, 24) == 0 and _capi.distill_workspace(None, 1, 1 << 17, 2) == 0
     for name, args in (("route", route_args()), ("plan", plan_args()), ("combine", mix_args()), ("distill", distill_args())):
         refused(name, args, "ctx is NULL")
 
