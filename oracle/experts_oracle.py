@@ -16,13 +16,13 @@ def route(x, k, score="softmax", bias=None, n_groups=1, top_groups=None, group_s
             weights[i] = np.nan
             continue
         p = probabilities(x[i], open_, score)
-        adds = bias is not None or (n_groups > 1 and group_score == "top2")
-        key = {c: (p[c] + (0.0 if bias is None else float(bias[c]))) if adds else x[i, c] for c in open_}
+        key = {c: p[c] + float(bias[c]) if bias is not None else x[i, c] for c in open_}
         if n_groups > 1:
             size = e // n_groups
             gs = []
+            rank = key if bias is not None or group_score == "max" else {c: p[c] for c in open_}       # sums are sums of probabilities
             for g in range(n_groups):
-                mine = sorted((key[c] for c in open_ if c // size == g), reverse=True)
+                mine = sorted((rank[c] for c in open_ if c // size == g), reverse=True)
                 gs.append(-np.inf if not mine else sum(mine[:2]) if group_score == "top2" else mine[0])
             keep = set(sorted(range(n_groups), key=lambda g: (-gs[g], g))[:top_groups])
             key = {c: v for c, v in key.items() if c // size in keep}

@@ -8,7 +8,7 @@
 // so the gradient is one coefficient times q_v on the rest and k values of their own on the top.
 //
 // q_r is summed over the rest itself (the teacher's entries left out, found by a bit per class in LDS): taken as 1 - sum q_k it would lose
-// every digit where the student is sure of itself.  The sums over the classes run in 32 bits (64 for double), everything per entry
+// every digit where the student is sure of itself, and so would log z next to one sure class.  The sums over the classes run in 32 bits (64 for double), everything per entry
 // and per row in 64.
 //
 // A row stays in the registers of its team of NT threads, NV units of 16 bytes each, so that it is read once: the sum and the gradient
@@ -81,12 +81,11 @@ template <typename T, int NT> __global__ void __launch_bounds__(NT) distill_slic
     const int64_t v_begin = (int64_t)u_begin * VN, v_end = last_slice ? a.V : (int64_t)u_end * VN;
     for (int i = tid; i < (int)((v_end - v_begin + 31) / 32); i += NT) bits[i] = 0;
     __syncthreads();
-    if (a.lse != nullptr)
-        for (int k = tid; k < a.K; k += NT) {
-            const int64_t c = a.index_64 ? static_cast<const int64_t*>(a.index)[row * a.ld_index + k] : static_cast<const int32_t*>(a.index)[row * a.ld_index + k];
-            if (c >= v_begin && c < v_end && !(load_any(a.top, a.top_dtype, row * a.ld_top + k) == -INFINITY))
-                atomicOr(&bits[(c - v_begin) >> 5], 1u << ((c - v_begin) & 31));
-        }
+    for (int k = tid; k < a.K; k += NT) {
+        const int64_t c = a.index_64 ? static_cast<const int64_t*>(a.index)[row * a.ld_index + k] : static_cast<const int32_t*>(a.index)[row * a.ld_index + k];
+        if (c >= v_begin && c < v_end && !(load_any(a.top, a.top_dtype, row * a.ld_top + k) == -INFINITY))
+            atomicOr(&bits[(c - v_begin) >> 5], 1u << ((c - v_begin) & 31));
+    }
     __syncthreads();
     acc m = lowest(acc()), z = 0;
     for (int u0 = u_begin + tid; u0 < u_end; u0 += U * NT) {
@@ -125,6 +124,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
     using acc = typename Num<T>::acc;
     using raw = typename Vec<T>::raw;
     constexpr int VN = Vec<T>::N, ROWS = NT < 256 ? 256 / NT : 1, LEAD = NT < 64 ? NT : 64, WAVES = NT / 64;
+    static_assert(NT >= VN, "a thread for every element that does not fill a unit");
     extern __shared__ __align__(16) unsigned char lds_all[];
     const int tid = threadIdx.x & (NT - 1);
     unsigned char* lds = lds_all + (NT < 256 ? threadIdx.x / NT : 0) * distill_lds(a.V, a.K, NT);
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
             ref = a.lse ? load_any(a.lse, a.lse_dtype, row) : lanes_reduce<LEAD>(tmax, OpMax());
             xref = __builtin_fmax(lanes_reduce<LEAD>(xref, OpMax()), -1e300);
             for (int k = tid; k < a.K; k += LEAD) if (cls[k] >= 0) {
-                const double dt = tk[k] - ref, dx = ek[k] - xref, e = exp_of(dt), f = exp_of(dx * a.inv_tau);
+                const double dt = tk[k] - ref, dx = ek[k] - xref, e = exp_of(dt > 1000.0 ? 1000.0 : dt), f = exp_of(dx * a.inv_tau);   // a top_lse below its entries: infinite
                 tk[k] = dt; pk[k] = e; ek[k] = f;
                 sums[0] += e;
                 if (e != 0.0) { sums[1] += e * dt; sums[2] += e * dx; }
@@ -245,8 +245,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
                 for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(data[i]));
                 forget_place();
             };
-            // ---- maximum and sum of the rest (without a rest outcome: of all classes) ----------------------------------------
-            const bool leave_out = a.lse != nullptr;
+            // ---- maximum and sum of the rest -----------------------------------------------------------------------------------
             auto hide = [&](raw& r, int u) {            // the entries' classes become -inf; their gradients are written over at the end
                 const int v = u * VN;
                 const unsigned b = bits[v >> 5] >> (v & 31) & ((1u << VN) - 1);
@@ -255,7 +254,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
                     for (int i = 0; i < VN; ++i) r[i] = b >> i & 1 ? (T)-INFINITY : r[i];
                 }
             };
-            if (leave_out && tid < tail && (bits[(nvec * VN + tid) >> 5] >> ((nvec * VN + tid) & 31) & 1)) last = -INFINITY;
+            if (tid < tail && (bits[(nvec * VN + tid) >> 5] >> ((nvec * VN + tid) & 31) & 1)) last = -INFINITY;
             {
                 forget_place();
 #pragma unroll
@@ -263,7 +262,8 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
                     const int u = i * NT + at;
                     if (u < nvec) {
                         raw r = __builtin_bit_cast(raw, data[i]);
-                        if (leave_out) { hide(r, u); data[i] = __builtin_bit_cast(words4, r); }
+                        hide(r, u);
+                        data[i] = __builtin_bit_cast(words4, r);
 #pragma unroll
                         for (int j = 0; j < VN; ++j) m = OpMax()(m, (acc)r[j]);
                     }
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
 #pragma unroll
                     for (int i = 0; i < U; ++i) {
                         const int u = u0 + i * NT;
-                        if (u < nvec) { if (leave_out) hide(r[i], u); take_unit<VN>(a, r[i], m, z); }
+                        if (u < nvec) { hide(r[i], u); take_unit<VN>(a, r[i], m, z); }
                     }
                 }
             }
@@ -324,29 +324,30 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
         if (lead && todo == ROW_COMPUTE) {
             const double far = ((double)mr - xref) * a.inv_tau, log_zr = log_of(zr);
             const bool rest = a.lse != nullptr && some_rest;
+            // z over all classes: the rest in 32 bits, the entries in 64.  Next to a sure student's entry (z = 1 + little) the little keeps its digits
+            log_z = far > 0.0 ? far + log_of(zr + sums[3] * exp_of(-far)) : log_of(zr * exp_of(far) + sums[3]);
+            const double lqr = far + log_zr - log_z, qr = some_rest ? exp_of(lqr) : 0.0;
+            double pr = 0.0, mass = qr;
             if (a.lse == nullptr) {
-                log_z = far + log_zr;
                 psum = sums[0];
-                kl = sums[1] / psum - log_of(psum) - sums[2] * a.inv_tau / psum + log_z;
-                coef = 1.0 / zr;
+                kl = (sums[1] - sums[2] * a.inv_tau) / psum - log_of(psum) + log_z;
             } else {
-                log_z = far > 0.0 ? far + log_of(zr + sums[3] * exp_of(-far)) : log_of(zr * exp_of(far) + sums[3]);
-                const double lqr = far + log_zr - log_z, qr = some_rest ? exp_of(lqr) : 0.0;
-                double pr = rest ? 1.0 - sums[0] : 0.0, mass = qr;
+                pr = rest ? 1.0 - sums[0] : 0.0;
                 pr = pr < 0.0 ? 0.0 : pr;
-                if (a.reverse) {
-                    const double scale = exp_of(-log_z), lr = rest ? lqr - log_of(pr > a.floor_rest ? pr : a.floor_rest) : 0.0;
-                    kl = scale != 0.0 ? scale * (sums[4] * a.inv_tau - sums[5] - sums[3] * log_z) : 0.0;
-                    if (qr != 0.0) kl += qr * lr;
-                    mass = qr != 0.0 ? qr * (lr - kl) : 0.0;
-                } else {
-                    kl = sums[1] - sums[2] * a.inv_tau + sums[0] * log_z;
-                    if (pr > 0.0) { kl += pr * (log_of(pr) - lqr); mass = qr - pr; }
-                }
-                // mass e_v / sum e on the rest, e_v = exp((s_v - m_r) / tau): q_v (1 - p_r / q_r) would be 0 times infinity where the student is
-                // sure of itself
-                coef = zr == 0.0 ? 0.0 : mass / zr;
+                kl = sums[1] - sums[2] * a.inv_tau + sums[0] * log_z;
             }
+            if (a.reverse) {
+                const double scale = exp_of(-log_z), lr = rest ? lqr - log_of(pr > a.floor_rest ? pr : a.floor_rest) : 0.0;
+                kl = scale != 0.0 ? scale * (sums[4] * a.inv_tau - sums[5] - sums[3] * log_z) : 0.0;
+                if (qr != 0.0) kl += qr * lr;
+                mass = qr != 0.0 ? qr * (lr - kl) : 0.0;
+            } else if (pr > 0.0) {
+                kl += pr * (log_of(pr) - lqr);
+                mass = qr - pr;
+            }
+            // mass e_v / sum e on the rest, e_v = exp((s_v - m_r) / tau): q_v (1 - p_r / q_r) would be 0 times infinity where the student is
+            // sure of itself
+            coef = zr == 0.0 ? 0.0 : mass / zr;
             coef *= a.tau * w;
         }
         if (tid == 0 && (MODE != SPLIT || blockIdx.x == 0)) static_cast<acc*>(a.loss)[row] = todo == ROW_COMPUTE ? (acc)(a.tau * a.tau * w * kl) : todo == ROW_ZERO ? (acc)0 : (acc)NAN;
@@ -482,7 +483,8 @@ static int distill_launch(hipStream_t stream, const oak_distill_args* a) {
             return distill_run<T, 512, 1, SPLIT>(stream, d);
         }
         if (d.n <= 256 && units > 64) return distill_run<T, 512, 8, LONG>(stream, d);
-        if (units <= 16 && d.K <= 16) return distill_run<T, 4, 4>(stream, d);
+        constexpr int FEWEST = Vec<T>::N > 4 ? 8 : 4;              // as many threads as elements may be left over behind the units
+        if (units <= 16 && d.K <= 16) return distill_run<T, FEWEST, 16 / FEWEST>(stream, d);
         if (units <= 64 && d.K <= 64) return distill_run<T, 16, 4>(stream, d);
         if (units <= 128 && d.K <= 64) return distill_run<T, 16, 8>(stream, d);
         if (units <= 256 && d.K <= 32) return distill_run<T, 16, 16>(stream, d);       // 65536 x 1000 float32: k = 10 120 us, with 64 threads 138;

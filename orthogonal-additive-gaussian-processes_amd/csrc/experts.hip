@@ -10,6 +10,8 @@
 
 namespace oak {
 
+constexpr int64_t MOST_SLOTS = ((int64_t)1 << 31) - 1;      // places and slots are 32-bit numbers
+
 // ---------------------------------------------------------------------------------------------------------------------
 // route
 // ---------------------------------------------------------------------------------------------------------------------
@@ -178,12 +180,14 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
             for (int s = 0; s < VPL; ++s) v[s] += b[s];
         }
     }
-    if constexpr (KIND != KEY_16) {
+    // a closed key: -inf, but for tags the lowest double (-inf with a tag would be NaN); scores of 64 bits reach that one themselves
+    constexpr clean CLOSED = KIND == KEY_TAG ? (clean)-1.7976931348623157e308 : (clean)-INFINITY;
+    auto is_open = [](clean t) { return t > (KIND == KEY_TAG ? (clean)CLOSED_BELOW : (clean)-INFINITY); };
 #pragma unroll
-        for (int s = 0; s < VPL; ++s) v[s] = with_hi(v[s], x[s] == -INFINITY ? CLOSED_HI : hi_of(v[s]));
+    for (int s = 0; s < VPL; ++s) {
+        if constexpr (KIND == KEY_TAG) v[s] = with_hi(v[s], x[s] == -INFINITY ? CLOSED_HI : hi_of(v[s]));
+        else if constexpr (KIND == KEY_F64) v[s] = x[s] == -INFINITY ? CLOSED : v[s];
     }
-    constexpr clean CLOSED = KIND == KEY_16 ? (clean)-INFINITY : (clean)-1.7976931348623157e308;
-    auto is_open = [](clean t) { return KIND == KEY_16 ? t > (clean)-INFINITY : t > (clean)CLOSED_BELOW; };
 
     if (a.groups > 1) {
         clean* gs = reinterpret_cast<clean*>(lds) + (size_t)(wave * TEAMS + team) * (a.lanes_per_group ? a.groups : a.E + a.groups);
@@ -250,6 +254,12 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
         }
     }
 
+    if constexpr (KIND != KEY_16) if (!plain_keys && a.bias == nullptr) {
+        // probabilities were for the groups; the experts are chosen by the scores, which do not saturate
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) v[s] = is_open(v[s]) ? (clean)x[s] : CLOSED;
+    }
+
     // the k best; lane j of the team keeps the j-th and, where the key is the score, that
     int mine = -1;
     double xe = 0.0;
@@ -300,7 +310,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
 
     // weights: one slot a lane, in 64 bits except for the plain softmax (a sigmoid's sum may be far below 1)
     const bool chosen = mine >= 0;
-    if (chosen && (KIND == KEY_F64 || !plain_keys)) xe = (double)score_at<acc>(a, at, mine);
+    if (chosen && (KIND == KEY_F64 || a.bias != nullptr)) xe = (double)score_at<acc>(a, at, mine);
     acc w = 0;
     if (a.renorm) {
         const double top = lanes_reduce<L>(chosen ? xe : -INFINITY, OpMax());
@@ -308,7 +318,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
         double p = 0.0;
         if (chosen) p = a.sigmoid && top > -40.0 ? sigmoid_of(xe) : exp_of(xe - top);
         const double sum = lanes_reduce<L>(p, OpSum());
-        if (chosen) w = (acc)(a.scale * p * inverse(sum));
+        if (chosen) w = (acc)(a.scale * (p / sum));               // a division: one expert's weight is 1 and not next to it
     } else if (chosen) {
         w = a.sigmoid ? (acc)(a.scale * (xe < -700.0 ? exp_of(xe) : sigmoid_of(xe))) : (acc)a.scale * (exp_of((acc)xe - xmax) / z);
     }
@@ -379,10 +389,10 @@ __global__ void __launch_bounds__(256) route_grad_kernel(RouteDev a) {
     wave_sync();
 
     acc r = 0;
-    const acc p = inverse((acc)1 + exp_of(-xe)), not_p = inverse((acc)1 + exp_of(xe));     // sigmoid and 1 - sigmoid, each to its own size
+    const acc p = (acc)1 / ((acc)1 + exp(-xe)), not_p = (acc)1 / ((acc)1 + exp(xe));     // sigmoid and 1 - sigmoid, each to its own size
     if (chosen) r = a.sigmoid && (!a.renorm || xmax > (acc)-40) ? p : exp_of(xe - xmax);
     if (dense) r *= inv;
-    else if (a.renorm) r *= inverse(lanes_reduce<L>(r, OpSum()));
+    else if (a.renorm) r /= lanes_reduce<L>(r, OpSum());       // one expert's r is 1, its gradient 0
     const acc dot = lanes_reduce<L>(r * g, OpSum());
     const bool some = lanes_reduce<L>(chosen ? 1u : 0u, OpMax()) != 0;
     if (chosen) {
@@ -454,7 +464,7 @@ static int route_check(const oak_route_args* a) {
     OAK_REQUIRE(a->scale - a->scale == 0.0, "route: scale is not finite");
     OAK_REQUIRE(a->n_rows <= 1 || a->ld_scores >= 0, "route: negative row stride");
     OAK_REQUIRE(a->n_rows == 0 || (a->scores && a->experts), "route: scores or experts are NULL");
-    OAK_REQUIRE(a->n_rows * (int64_t)a->top_k < ((int64_t)1 << 31), "route: %lld rows x %d experts pass 2^31 slots", (long long)a->n_rows, a->top_k);
+    OAK_REQUIRE(a->n_rows <= MOST_SLOTS / a->top_k, "route: %lld rows x %d experts pass 2^31 slots", (long long)a->n_rows, a->top_k);
     return OAK_OK;
 }
 
@@ -517,8 +527,8 @@ static int route_grad_launch(hipStream_t stream, const oak_route_args* a) {
 // ---------------------------------------------------------------------------------------------------------------------
 // plan: stable counting sort of the n k slots by expert
 // ---------------------------------------------------------------------------------------------------------------------
-// Bound by latency, three short launches (524288 slots, 24 experts: 3 + 4 + 7 us for 6 MB): every wave owns one consecutive piece of the slots, so that the order inside an expert is the slots' own without any atomic
-// whose order could show: pieces are counted, the counts are summed in piece order, and each wave then places its slots 64 at a
+// Bound by latency, three short launches (524288 slots, 24 experts: 4 + 4 + 7 us for 6 MB).  Every wave owns one consecutive piece of the
+// slots, so that the order inside an expert is the slots' own without any atomic whose order could show: pieces are counted, the counts are summed in piece order, and each wave then places its slots 64 at a
 // time -- a slot's rank among the 64 is the number of lower lanes with the same expert (one ballot per bit of the expert's number).
 constexpr int64_t PLAN_SMALL_SLOTS = 16384;
 constexpr int PLAN_MAX_PIECES = 2048;
@@ -672,7 +682,7 @@ static void plan_pieces(int64_t slots, int E, int64_t* piece, int* npieces, bool
 }
 
 static int64_t plan_workspace(int64_t n_rows, int32_t top_k, int32_t n_experts) {
-    if (n_rows <= 0 || top_k <= 0 || n_experts <= 0) return 0;
+    if (n_rows <= 0 || top_k <= 0 || n_experts <= 0 || n_experts > OAK_MAX_PLAN_EXPERTS || n_rows > MOST_SLOTS / top_k) return 0;
     int64_t piece; int np; bool small;
     plan_pieces(n_rows * top_k, n_experts, &piece, &np, &small);
     return small ? 0 : (int64_t)np * n_experts;
@@ -682,7 +692,7 @@ static int plan_check(const oak_plan_args* a) {
     OAK_REQUIRE(a != nullptr, "plan: arguments are NULL");
     OAK_REQUIRE(a->n_rows >= 0 && a->top_k >= 1 && a->top_k <= OAK_MAX_TOP_K, "plan: %lld rows of %d experts", (long long)a->n_rows, a->top_k);
     OAK_REQUIRE(a->n_experts >= 1 && a->n_experts <= OAK_MAX_PLAN_EXPERTS, "plan: n_experts = %d is not in 1 .. %d", a->n_experts, OAK_MAX_PLAN_EXPERTS);
-    OAK_REQUIRE(a->n_rows * (int64_t)a->top_k < ((int64_t)1 << 31), "plan: %lld rows x %d experts pass 2^31 slots", (long long)a->n_rows, a->top_k);
+    OAK_REQUIRE(a->n_rows <= MOST_SLOTS / a->top_k, "plan: %lld rows x %d experts pass 2^31 slots", (long long)a->n_rows, a->top_k);
     OAK_REQUIRE(a->counts && a->offsets && (a->n_rows == 0 || (a->experts && a->rows && a->positions)), "plan: an array is NULL");
     return OAK_OK;
 }
@@ -861,7 +871,7 @@ static int mix_check(const char* what, const oak_mix_args* a) {
     OAK_REQUIRE(a->n_experts >= 1 && a->n_experts <= OAK_MAX_PLAN_EXPERTS, "%s: n_experts = %d", what, a->n_experts);
     OAK_REQUIRE(a->n_cols >= 1 && a->n_cols <= (1 << 30), "%s: n_cols = %d", what, a->n_cols);
     OAK_REQUIRE(a->dtype >= OAK_F64 && a->dtype <= OAK_F16, "%s: unknown element type %d", what, a->dtype);
-    OAK_REQUIRE(a->n_rows * (int64_t)a->top_k < ((int64_t)1 << 31), "%s: %lld rows x %d experts pass 2^31 slots", what, (long long)a->n_rows, a->top_k);
+    OAK_REQUIRE(a->n_rows <= MOST_SLOTS / a->top_k, "%s: %lld rows x %d experts pass 2^31 slots", what, (long long)a->n_rows, a->top_k);
     OAK_REQUIRE(a->ld_rows >= 0 && a->ld_slots >= 0 && a->ld_grad >= 0, "%s: negative row stride", what);
     OAK_REQUIRE(a->n_rows == 0 || (a->positions && a->offsets), "%s: positions or offsets are NULL", what);
     return OAK_OK;

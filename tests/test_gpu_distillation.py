@@ -3,7 +3,9 @@
 Tolerances, u = 2^-24 (2^-53 for float64).  log z carries d = (far / tau + V / 64 + 16) u: the argument's rounding is u of the
 distance ``far`` of the logits, the exponential's two, and a sum of V terms by at least 64 threads takes at most V / 64 + 12 roundings.  A
 divergence adds d (and a few u of its terms, ``size`` of the oracle) to its value; a gradient entry carries 2 d of both of its parts and
-one rounding to its type, half a step.
+one rounding to its type, half a step.  Teacher probabilities are formed in 64 bits everywhere, so they only count for float64: the rounding
+of t / tau - lse, (|t| / tau + |lse|) 2^-53, and as much again in the oracle, which works in the same 64 bits.  The reverse direction
+holds log p_rest, p_rest = 1 - sum p: that error and the k roundings of the sum over p_rest.
 """
 import numpy as np
 import pytest
@@ -52,6 +54,14 @@ def compare(s, top, idx, lse, tau, direction, weight, dtype):
     far = np.array([np.ptp(r[np.isfinite(r)]) if np.isfinite(r).any() else 0.0 for r in finite])
     far = np.minimum(far, 110.0 * tau)                                   # further down an exponential is 0 in 32 bits
     d = (far / tau + v / 64 + 16) * u
+    if dtype == "f64":
+        t = np.where((back(idx) >= 0) & np.isfinite(back(top)), np.abs(back(top)), 0.0).max(1)
+        t = t / tau + (0.0 if lse is None else np.abs(back(lse)))
+        d = d + 2 * t * u
+        if direction == "reverse":
+            there = (back(idx) >= 0) & np.isfinite(back(top))
+            p = np.where(there, np.exp(np.where(there, back(top), 0.0) / tau - back(lse)[:, None]), 0.0)
+            d = d + 2 * (t + top.shape[1]) * u / np.maximum(1.0 - p.sum(1), 2.0 ** -53)
     assert np.array_equal(np.isnan(back(loss)), np.isnan(ref)) and np.array_equal(np.isinf(back(loss)), np.isinf(ref))
     ok = np.isfinite(ref)
     err, tol = np.abs(back(loss) - np.where(ok, ref, 0)), (2 * d + 4 * u) * (size + np.abs(np.where(ok, ref, 0)))
@@ -306,3 +316,25 @@ def test_two_graphs_of_split_rows_do_not_share_scratch():
         torch.cuda.synchronize()
         for h, r in zip(held, ref):
             assert torch.equal(h[0], r[0]) and torch.equal(h[1], r[1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32", "f64"])
+@pytest.mark.parametrize("direction", ["forward", "reverse"])
+def test_every_small_number_of_classes(dtype, direction):
+    """1 .. 70 classes: every count of elements left over behind the 16-byte units, many rows, some of them left out."""
+    for v in range(1, 71):
+        k = 1 + v % min(v, 17)
+        s, top, idx, lse = problem(300, v, k, dtype, True, 1.0, v, pad=v % 3)
+        w = torch.rand(300, device="cuda", dtype=top.dtype) + 0.5
+        w[::7] = 0
+        compare(s, top, idx, lse, 1.0, direction, w, dtype)
+
+
+@pytest.mark.parametrize("units", [16, 64, 128, 256, 512, 1024, 2048, 4096])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_around_the_sizes_where_the_team_changes(units, dtype):
+    per = 8 if dtype == "bf16" else 4
+    for v in (units * per - 1, units * per, units * per + 1, units * per + per - 1):
+        for k, n in ((9, 270), (33, 260)):
+            s, top, idx, lse = problem(n, v, min(k, v), dtype, True, 1.0, v + k)
+            compare(s, top, idx, lse, 1.0, "forward", None, dtype)

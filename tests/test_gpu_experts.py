@@ -438,3 +438,32 @@ def test_two_threads_at_once():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not wrong
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalise", [True, False])
+def test_float64_at_the_ends_of_its_range(score, renormalise):
+    """Finite scores stay open, the lowest double among them; sigmoids far out on both sides; saturated probabilities do not tie."""
+    low, high = float(np.finfo(np.float64).min), 1e300
+    x = np.array([[low, low, -np.inf, low], [low, 1.0, low, 2.0], [800.0, -800.0, 750.0, -750.0], [-800.0, -900.0, -1e5, -1e6],
+                  [50.0, 60.0, 55.0, 40.0], [high, 0.0, -high, 1.0], [0.0, -0.0, 0.0, -0.0]])
+    dw = np.arange(1.0, 1.0 + x.shape[0] * 3).reshape(-1, 3)
+    ex, w = ox.route(x, 3, score=score, renormalise=renormalise)
+    er, wr = eo.route(x, 3, score=score, renormalise=renormalise)
+    np.testing.assert_array_equal(ex, er)
+    np.testing.assert_allclose(w, wr, rtol=1e-13, atol=1e-300)
+    dx, ref = ox.route_grad(x, ex, dw, score=score, renormalise=renormalise), eo.route_grad(x, er, dw, score=score, renormalise=renormalise)
+    np.testing.assert_allclose(dx, ref, rtol=1e-12, atol=1e-13)
+    grouped = dict(score=score, renormalise=renormalise, n_groups=2, top_groups=1, group_score="top2")
+    ex, w = ox.route(x[1:], 2, **grouped)
+    np.testing.assert_array_equal(ex, eo.route(x[1:], 2, **grouped)[0])
+
+
+def test_saturated_probabilities_do_not_tie_without_a_bias():
+    """Scores whose sigmoids agree in every bit that 64 bits hold are still told apart: the choice goes by the scores."""
+    x = torch.tensor([[40.0, 41.0, 39.0, 42.0, 45.0, 44.0, 43.0, 46.0]], device="cuda")
+    for dtype in ("f32", "bf16", "f64"):
+        ex, _ = ox.route(x.to(DT[dtype]), 3, score="sigmoid", n_groups=2, top_groups=2, group_score="top2")
+        np.testing.assert_array_equal(back(ex), [[7, 4, 5]])
+        ex, _ = ox.route(x.to(DT[dtype]), 3, score="sigmoid")
+        np.testing.assert_array_equal(back(ex), [[7, 4, 5]])

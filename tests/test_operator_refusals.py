@@ -27,7 +27,7 @@ def route_args(**kw):
     (dict(n_experts=0), "n_experts"), (dict(n_experts=1025), "n_experts"), (dict(top_k=0), "top_k"), (dict(top_k=5), "top_k"),
     (dict(n_groups=3), "n_groups"), (dict(n_groups=0), "n_groups"), (dict(n_groups=2, top_groups=3), "top_groups"),
     (dict(n_groups=4, top_groups=1, top_k=2), "top_k"), (dict(dtype=9), "type"), (dict(score=2), "score"), (dict(group_score=-1), "group score"),
-    (dict(scale=float("inf")), "scale"), (dict(n_rows=-1), "n_rows"), (dict(n_rows=1 << 31), "slots"), (dict(scores=None), "NULL"),
+    (dict(scale=float("inf")), "scale"), (dict(n_rows=-1), "n_rows"), (dict(n_rows=1 << 31), "slots"), (dict(n_rows=1 << 62, top_k=4), "slots"), (dict(scores=None), "NULL"),
     (dict(weights=None), "NULL"), (dict(ld_scores=-4), "stride"),
 ])
 def test_route_refuses(kw, match):
@@ -49,7 +49,7 @@ def plan_args(**kw):
 
 @pytest.mark.parametrize("kw,match", [
     (dict(n_experts=0), "n_experts"), (dict(n_experts=4097), "n_experts"), (dict(top_k=0), "experts"), (dict(top_k=65), "experts"),
-    (dict(n_rows=1 << 30), "slots"), (dict(rows=None), "NULL"), (dict(n_rows=1 << 20), "workspace"),
+    (dict(n_rows=1 << 30), "slots"), (dict(n_rows=1 << 62, top_k=4), "slots"), (dict(rows=None), "NULL"), (dict(n_rows=1 << 20), "workspace"),
 ])
 def test_plan_refuses(kw, match):
     refused("plan", plan_args(**kw), match)
