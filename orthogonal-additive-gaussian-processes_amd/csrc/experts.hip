@@ -740,6 +740,12 @@ template <typename T> __device__ __forceinline__ void zero_unit(const MixDev& a,
     else row[a.nvec * (int64_t)Vec<T>::N + (u - a.nvec)] = (T)0;
 }
 
+// slots of 1 KiB and more are written past the caches (32768 x 2048 bf16, k = 6: all five calls of a training step 922 -> 899 us; 262144 x 17
+// float64, whose rows end inside cache lines, 88 -> 90)
+template <typename T, bool WIDE> __device__ __forceinline__ void store_slot(T* p, typename Vec<T>::raw v) {
+    if constexpr (WIDE) Vec<T>::store_stream(p, v); else Vec<T>::store(p, v);
+}
+
 // a place outside [0, slots) is no place
 __device__ __forceinline__ int64_t place_of(const MixDev& a, int64_t n, int j) {
     const int p = a.positions[n * a.k + j];
@@ -754,7 +760,7 @@ __device__ __forceinline__ int64_t mix_row(const MixDev& a, int* unit) {
     return r < a.rows_per_wg && n < a.n ? n : -1;
 }
 
-template <typename T> __global__ void __launch_bounds__(256) dispatch_kernel(MixDev a) {
+template <typename T, bool WIDE> __global__ void __launch_bounds__(256) dispatch_kernel(MixDev a) {
     int t;
     const int64_t n = mix_row(a, &t);
     if (n < 0) return;
@@ -764,7 +770,7 @@ template <typename T> __global__ void __launch_bounds__(256) dispatch_kernel(Mix
     for (int64_t u = t; u < a.units; u += a.tpr) {
         if (u < a.nvec) {
             const auto v = Vec<T>::load(src + u * Vec<T>::N);
-            for (int j = 0; j < a.k; ++j) { const int64_t p = place_of(a, n, j); if (p >= 0) Vec<T>::store(dst + p * a.ld_slots + u * Vec<T>::N, v); }
+            for (int j = 0; j < a.k; ++j) { const int64_t p = place_of(a, n, j); if (p >= 0) store_slot<T, WIDE>(dst + p * a.ld_slots + u * Vec<T>::N, v); }
         } else {
             const int64_t c = a.nvec * (int64_t)Vec<T>::N + (u - a.nvec);
             const T v = src[c];
@@ -819,7 +825,7 @@ template <typename T, int CHUNK> __global__ void __launch_bounds__(256) combine_
 
 // dF[place] = w dy, dw = <dy, F[place]>: slot by slot, the row of dy stays in the nearest cache, 4 units of both asked for together.  At
 // most 64 threads a row: the dot product is finished inside a wave.
-template <typename T> __global__ void __launch_bounds__(256) combine_grad_kernel(MixDev a) {
+template <typename T, bool WIDE> __global__ void __launch_bounds__(256) combine_grad_kernel(MixDev a) {
     using acc = typename Num<T>::acc;
     const int64_t n = a.row0 + (int64_t)blockIdx.x * a.rows_per_wg + (threadIdx.x >> a.tpr_log2);
     const int tpr = 1 << a.tpr_log2, t = (int)(threadIdx.x & (tpr - 1));
@@ -850,7 +856,7 @@ template <typename T> __global__ void __launch_bounds__(256) combine_grad_kernel
                     typename Vec<T>::raw o;
 #pragma unroll
                     for (int e = 0; e < Vec<T>::N; ++e) { d += (acc)f[i][e] * (acc)v[i][e]; o[e] = (T)(wj * (acc)v[i][e]); }
-                    Vec<T>::store_stream(gr + (u0 + i * tpr) * Vec<T>::N, o);
+                    store_slot<T, WIDE>(gr + (u0 + i * tpr) * Vec<T>::N, o);
                 }
             }
             for (int64_t c = (int64_t)a.nvec * Vec<T>::N + t; c < a.C; c += tpr) {
@@ -892,7 +898,10 @@ static int mix_launch(hipStream_t stream, const oak_mix_args* a, int what /* 0 d
     d.inv_tpr = (65536 + d.tpr - 1) / d.tpr;           // t / tpr = t inv_tpr >> 16 for t < 256
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        auto kernel = what == 0 ? dispatch_kernel<T> : what == 2 ? combine_grad_kernel<T> : d.k <= 2 ? combine_kernel<T, 2> : d.k <= 4 ? combine_kernel<T, 4> : combine_kernel<T, 8>;
+        const bool wide = (int64_t)d.C * (int64_t)sizeof(T) >= 1024;
+        auto kernel = what == 0 ? (wide ? dispatch_kernel<T, true> : dispatch_kernel<T, false>)
+                      : what == 2 ? (wide ? combine_grad_kernel<T, true> : combine_grad_kernel<T, false>)
+                      : d.k <= 2 ? combine_kernel<T, 2> : d.k <= 4 ? combine_kernel<T, 4> : combine_kernel<T, 8>;
         return launch_rows(kernel, d.rows_per_wg, 0, stream, d);
     });
 }
