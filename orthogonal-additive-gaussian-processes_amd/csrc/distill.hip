@@ -55,6 +55,26 @@ enum { HELD = 0, LONG = 1, SPLIT = 2 };
 __device__ __forceinline__ float lowest(float) { return -3.402823466e38f; }
 __device__ __forceinline__ double lowest(double) { return -1.7976931348623157e308; }
 
+// a unit with the elements of the bits set in b replaced by -inf; two 16-bit elements at a time
+template <typename T> __device__ __forceinline__ typename Vec<T>::raw hidden(typename Vec<T>::raw r, unsigned b) {
+    if constexpr (sizeof(T) == 2) {
+        typedef unsigned words4 __attribute__((ext_vector_type(4)));
+        words4 w = __builtin_bit_cast(words4, r);
+        const unsigned inf = (unsigned)__builtin_bit_cast(unsigned short, (T)-INFINITY) * 0x10001u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned low = (unsigned)((int)(b << (31 - 2 * i)) >> 31), high = (unsigned)((int)(b << (30 - 2 * i)) >> 31);
+            const unsigned mask = (low & 0xffffu) | (high & 0xffff0000u);
+            w[i] = (inf & mask) | (w[i] & ~mask);
+        }
+        return __builtin_bit_cast(typename Vec<T>::raw, w);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Vec<T>::N; ++i) r[i] = b >> i & 1 ? (T)-INFINITY : r[i];
+        return r;
+    }
+}
+
 // one more unit into a running maximum m and sum z
 template <int VN, typename A, typename R> __device__ __forceinline__ void take_unit(const DistillDev& a, const R& r, A& m, A& z) {
     A top = m;
@@ -98,8 +118,7 @@ template <typename T, int NT> __global__ void __launch_bounds__(NT) distill_slic
             if (u >= u_end) break;
             const int v = (u - u_begin) * VN;
             const unsigned b = bits[v >> 5] >> (v & 31);
-#pragma unroll
-            for (int j = 0; j < VN; ++j) r[i][j] = b >> j & 1 ? (T)-INFINITY : r[i][j];
+            r[i] = hidden<T>(r[i], b);
             take_unit<VN>(a, r[i], m, z);
         }
     }
@@ -249,10 +268,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
             auto hide = [&](raw& r, int u) {            // the entries' classes become -inf; their gradients are written over at the end
                 const int v = u * VN;
                 const unsigned b = bits[v >> 5] >> (v & 31) & ((1u << VN) - 1);
-                if (__any(b != 0)) {
-#pragma unroll
-                    for (int i = 0; i < VN; ++i) r[i] = b >> i & 1 ? (T)-INFINITY : r[i];
-                }
+                if (__any(b != 0)) r = hidden<T>(r, b);
             };
             if (tid < tail && (bits[(nvec * VN + tid) >> 5] >> ((nvec * VN + tid) & 31) & 1)) last = -INFINITY;
             {
