@@ -164,10 +164,12 @@ def _device_experts(d, experts, shape, n_experts):
     experts = d.tensor(experts, "experts")
     if experts.dtype == d.torch.int32:
         return d.dense(experts, "experts", shape)
-    if experts.dtype.is_floating_point or experts.dtype.is_complex or experts.dtype == d.torch.bool:
-        raise ValueError(f"experts must be integers, not {experts.dtype}")
-    return d.dense(experts.clamp(-1, n_experts), "experts", shape, d.torch.int32) if experts.dtype == d.torch.int64 else d.dense(
-        experts, "experts", shape, d.torch.int32)
+    t = d.torch
+    if experts.dtype == t.int64:                                        # what 32 bits cannot hold stays no expert's number
+        return d.dense(experts.clamp(-1, n_experts), "experts", shape, t.int32)
+    if experts.dtype not in (t.int16, t.int8, t.uint8):
+        raise ValueError(f"experts is of type {experts.dtype}; int8, int16, int32, int64 and uint8 are supported")
+    return d.dense(experts, "experts", shape, t.int32)
 
 
 class Plan(NamedTuple):

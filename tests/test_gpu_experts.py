@@ -467,3 +467,15 @@ def test_saturated_probabilities_do_not_tie_without_a_bias():
         np.testing.assert_array_equal(back(ex), [[7, 4, 5]])
         ex, _ = ox.route(x.to(DT[dtype]), 3, score="sigmoid")
         np.testing.assert_array_equal(back(ex), [[7, 4, 5]])
+
+
+def test_types_of_experts():
+    """The smaller integers count like int32; unsigned ones whose numbers 32 bits would wrap are refused."""
+    ex = torch.tensor([[0, 2], [1, 3], [3, 0]], dtype=torch.int32, device="cuda")
+    p = ox.plan(ex, 4)
+    for dtype in (torch.int8, torch.uint8, torch.int16, torch.int64):
+        for got, ref in zip(ox.plan(ex.to(dtype), 4)[:4], p[:4]):
+            np.testing.assert_array_equal(back(got), back(ref))
+    for dtype in (torch.uint32, torch.uint64, torch.bool, torch.float32):
+        with pytest.raises(ValueError):
+            ox.plan(torch.zeros(3, 2, dtype=dtype, device="cuda"), 4)
