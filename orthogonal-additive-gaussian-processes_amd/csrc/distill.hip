@@ -8,8 +8,8 @@
 // so the gradient is one coefficient times q_v on the rest and k values of their own on the top.
 //
 // q_r is summed over the rest itself (the teacher's entries left out, found by a bit per class in LDS): taken as 1 - sum q_k it would lose
-// every digit where the student is sure of itself, and so would log z next to one sure class.  The sums over the classes run in 32 bits (64 for double), everything per entry
-// and per row in 64.
+// every digit where the student is sure of itself, and so would log z next to one sure class.  The sums over the classes run in 32 bits
+// (64 for double), everything per entry and per row in 64.
 //
 // A row stays in the registers of its team of NT threads, NV units of 16 bytes each, so that it is read once: the sum and the gradient
 // each walk the registers (LONG: what does not fit is read twice).  The team's first wave (all of a smaller team) does what concerns the entries.
@@ -508,10 +508,10 @@ static int distill_launch(hipStream_t stream, const oak_distill_args* a) {
         if (units <= 512) return distill_run<T, 64, 8>(stream, d);
         if (units <= 1024) return distill_run<T, 64, 16>(stream, d);
         if (units <= 2048) return distill_run<T, 256, 8>(stream, d);
-        if (units <= 4096) return distill_run<T, 256, 16>(stream, d);                  // 4096 x 32768 bf16: 119 us, read twice 146
+        if (units <= 4096) return distill_run<T, 256, 16>(stream, d);                  // 4096 x 32768 bf16: 119 us (4.5 TB/s), read twice 146
         // Longer rows: what 512 threads can hold with two workgroups a compute unit, the rest is read twice, the second time out of the last cache
-        // (2 x 256 rows in flight fit it up to 2^18 bf16 classes, and the gradient passes it by).  2048 x 131072 bf16: 265 us; all of it
-        // read twice 279; the whole row in the registers of 1024 threads, one workgroup a unit, 330.
+        // (2 x 256 rows in flight fit it up to 2^18 bf16 classes, and the gradient passes it by).  2048 x 131072 bf16: 250 us (265 when this was
+        // chosen; all of it read twice 279; the whole row in the registers of 1024 threads, one workgroup a unit, 330).
         return distill_run<T, 512, 8, LONG>(stream, d);
     });
 }

@@ -528,8 +528,9 @@ static int route_grad_launch(hipStream_t stream, const oak_route_args* a) {
 // plan: stable counting sort of the n k slots by expert
 // ---------------------------------------------------------------------------------------------------------------------
 // Bound by latency, three short launches (524288 slots, 24 experts: 4 + 4 + 7 us for 6 MB).  Every wave owns one consecutive piece of the
-// slots, so that the order inside an expert is the slots' own without any atomic whose order could show: pieces are counted, the counts are summed in piece order, and each wave then places its slots 64 at a
-// time -- a slot's rank among the 64 is the number of lower lanes with the same expert (one ballot per bit of the expert's number).
+// slots, so that the order inside an expert is the slots' own without any atomic whose order could show: pieces are counted, the counts
+// are summed in piece order, and each wave then places its slots 64 at a time -- a slot's rank among the 64 is the number of lower lanes
+// with the same expert (one ballot per bit of the expert's number).
 constexpr int64_t PLAN_SMALL_SLOTS = 16384;
 constexpr int PLAN_MAX_PIECES = 2048;
 
@@ -725,8 +726,8 @@ static int plan_launch(hipStream_t stream, const oak_plan_args* a) {
 // ---------------------------------------------------------------------------------------------------------------------
 // All of them walk rows: a row is read or written once where the slots' order would touch it k times.  tpr threads share a row; a unit is
 // 16 bytes, the row's last elements that do not fill one are units of their own.  A thread asks for the places, then for the answers of up
-// to 8 slots before it adds the first (k = 6: 198 us, 4 at a time 210).  Bound by memory: 32768 rows, k = 6, 2048 bf16 columns, of 0.94 GB
-// each: dispatch 158 us (5.9 TB/s), combine 198 (4.7), and of 1.74 GB combine_grad 353 (4.9), where a large copy reaches 5.06 TB/s.
+// to 8 slots before it adds the first (k = 6: combine 198 us, 4 at a time 210).  Bound by memory: 32768 rows, k = 6, 2048 bf16 columns, of 0.94 GB
+// each: dispatch 177 us (5.3 TB/s), combine 178 (5.3), and of 1.74 GB combine_grad 352 (4.9), where a large copy reaches 5.06 TB/s.
 struct MixDev {
     int64_t row0, n, slots, ld_rows, ld_slots, ld_grad;
     int64_t units;              // 16-byte units of a row, then its last elements
@@ -740,7 +741,8 @@ template <typename T> __device__ __forceinline__ void zero_unit(const MixDev& a,
     else row[a.nvec * (int64_t)Vec<T>::N + (u - a.nvec)] = (T)0;
 }
 
-// slots of 1 KiB and more are written past the caches (32768 x 2048 bf16, k = 6: all five calls of a training step 922 -> 899 us; 262144 x 17
+// slots of 1 KiB and more are written past the caches (32768 x 2048 bf16, k = 6: all five calls of a training step 922 -> 899 us: dispatch
+// 158 -> 177, but the combine that reads other slots meanwhile 198 -> 178; 262144 x 17
 // float64, whose rows end inside cache lines, 88 -> 90)
 template <typename T, bool WIDE> __device__ __forceinline__ void store_slot(T* p, typename Vec<T>::raw v) {
     if constexpr (WIDE) Vec<T>::store_stream(p, v); else Vec<T>::store(p, v);
