@@ -418,6 +418,7 @@ int oak_kmeans_plusplus(oak_ctx* ctx, const double* X, int64_t N, int32_t D, int
    the default stream) and returns.  It takes nothing but the device from ctx, so that any number of threads may share one for these calls; it
    allocates nothing, keeps nothing, waits for nothing, leaves the thread's current device as it was and may be captured into a graph.  The
    arrays must belong to the HIP runtime this library is linked against (oak_device_pointer_check).
+   No output may overlap another array of the call.
    Sums, weights, losses and softmax statistics are float64 for float64 arrays and float32 otherwise: "wide" below. */
 #define OAK_F64   0
 #define OAK_F32   1

@@ -81,7 +81,7 @@ class Device:
             raise ValueError(f"{what} must be on {self.like.device} like the first array of the call")
         if a.requires_grad and self.torch.is_grad_enabled():
             raise ValueError(f"{what} requires grad: the operators record no graph, their gradients are calls of their own; pass {what}.detach()")
-        return a
+        return a.resolve_neg() if a.is_neg() else a          # a view that negates when it is read
 
     def matrix(self, a, what: str, shape=None):
         """A 2-D tensor whose columns are consecutive (copied if they are not)."""

@@ -928,8 +928,9 @@ class HipContext:
 
     # -- operators on host or device arrays (oak.experts, oak.distillation) -----------------------
     def call(self, name: str, args):
-        """One operator of the ``oak_X(ctx, args)`` form on contiguous float64 host arrays."""
-        _check(getattr(self._lib, f"oak_{name}")(self._h, C.byref(args)))
+        """One operator of the ``oak_X(ctx, args)`` form on contiguous float64 host arrays; calls of several threads wait for each other."""
+        with _call_lock:
+            _check(getattr(self._lib, f"oak_{name}")(self._h, C.byref(args)))
 
     # -- benchmarking -------------------------------------------------------------------------
     def bench_gram_resident(self, desc: KernelDesc) -> float:
@@ -978,6 +979,7 @@ def default_context() -> HipContext:
     return _default_ctx
 
 
+_call_lock = threading.Lock()               # a context's buffers and stream serve one call at a time
 _device_ctx = {}
 _device_ctx_lock = threading.Lock()
 

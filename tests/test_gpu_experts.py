@@ -479,3 +479,31 @@ def test_types_of_experts():
     for dtype in (torch.uint32, torch.uint64, torch.bool, torch.float32):
         with pytest.raises(ValueError):
             ox.plan(torch.zeros(3, 2, dtype=dtype, device="cuda"), 4)
+
+
+def test_two_threads_with_numpy_arrays():
+    """Host calls share the process's context and wait for each other."""
+    import threading
+    rng = np.random.default_rng(1)
+    xs = [rng.standard_normal((n, 24)) for n in (3000, 500)]
+    ref = [ox.route(x, 3) for x in xs]
+    wrong = []
+
+    def work(i):
+        for _ in range(20):
+            ex, w = ox.route(xs[i], 3)
+            if not (np.array_equal(ex, ref[i][0]) and np.array_equal(w, ref[i][1])):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
+
+
+def test_views_that_negate_when_they_are_read():
+    z = torch.randn(7, 1, dtype=torch.complex64, device="cuda")
+    x = z.conj().imag
+    assert x.is_neg()
+    p = ox.plan(torch.zeros(7, 1, dtype=torch.int32, device="cuda"), 1)
+    np.testing.assert_array_equal(back(ox.dispatch(x, p)), -back(z.imag.contiguous()))
