@@ -1,7 +1,7 @@
 // Mixtures of models: rows routed to their experts, laid out by expert, and the experts' answers summed with the router's weights.
 //
 //   route      x[n, e] -> the k experts of each row and their weights            (route_kernel), and the gradient (route_grad_kernel)
-//   plan       experts[n, k] -> a stable order of the slots by expert             (plan_small_kernel | plan_count / _scan / _place)
+//   plan       experts[n, k] -> a stable order of the slots by expert             (plan_small_kernel | plan_count_piece / _join | plan_count / _scan / _place)
 //   dispatch   X[n] copied to the places of its slots                              (dispatch_kernel)
 //   combine    y[n] = sum_j w[n, j] F[place(n, j)], and its gradients              (combine_kernel, combine_grad_kernel)
 //
@@ -527,12 +527,17 @@ static int route_grad_launch(hipStream_t stream, const oak_route_args* a) {
 // ---------------------------------------------------------------------------------------------------------------------
 // plan: stable counting sort of the n k slots by expert
 // ---------------------------------------------------------------------------------------------------------------------
-// Bound by latency, three short launches (524288 slots, 24 experts: 4 + 4 + 7 us for 6 MB).  Every wave owns one consecutive piece of the
+// Bound by latency, two or three short launches (524288 slots, 24 experts: 12 us for 6 MB).  Every wave owns one consecutive piece of the
 // slots, so that the order inside an expert is the slots' own without any atomic whose order could show: pieces are counted, the counts
 // are summed in piece order, and each wave then places its slots 64 at a time -- a slot's rank among the 64 is the number of lower lanes
-// with the same expert (one ballot per bit of the expert's number).
+// with the same expert (one ballot per bit of the expert's number).  The experts of 4 such steps are asked for together (8000000 slots of 16
+// experts: 58.6 us, one at a time 81.4).
 constexpr int64_t PLAN_SMALL_SLOTS = 16384;
 constexpr int PLAN_MAX_PIECES = 2048;
+// two launches instead of three up to here: 524288 slots of 24 experts 11.9 us (three: 12.6), 20000 of 8 7.2 (9.7), and 2.5 us less of the host;
+// 196608 slots of 64 experts 13.5 (11.5), 8000000 of 16 65.8 (58.6)
+constexpr int PLAN_JOIN_EXPERTS = 32, PLAN_JOIN_PIECES = 512;
+constexpr int64_t PLAN_JOIN_SLOTS = 1 << 20;
 
 struct PlanDev {
     int64_t slots, piece;
@@ -541,32 +546,53 @@ struct PlanDev {
     int* ws;                    // [E][npieces]
 };
 
-__device__ __forceinline__ int slot_expert(const PlanDev& a, int64_t s, int64_t end) {
-    const int e = s < end ? a.experts[s] : -1;
-    return (unsigned)e < (unsigned)a.E ? e : -1;      // whatever is not an expert's number belongs to no expert
+// the experts of the slots s, s + STEP, ... below end (s may be behind it, end > 0), asked for together
+template <int U, int STEP> __device__ __forceinline__ void slot_experts(const PlanDev& a, int64_t s, int64_t end, int (&e)[U]) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) e[i] = a.experts[s + i * STEP < end ? s + i * STEP : end - 1];
+#pragma unroll
+    for (int i = 0; i < U; ++i) e[i] = s + i * STEP < end && (unsigned)e[i] < (unsigned)a.E ? e[i] : -1;      // whatever is not an expert's number belongs to no expert
+}
+
+// adds the slots [s0, s1) to cnt[e] (LDS), STEP threads of which this is number t
+template <int STEP> __device__ __forceinline__ void plan_count_slots(const PlanDev& a, int* cnt, int64_t s0, int64_t s1, int t) {
+    constexpr int U = 4;
+    for (int64_t s = s0; s < s1; s += U * STEP) {
+        int e[U];
+        slot_experts<U, STEP>(a, s + t, s1, e);
+#pragma unroll
+        for (int i = 0; i < U; ++i) if (e[i] >= 0) atomicAdd(&cnt[e[i]], 1);
+    }
 }
 
 // places the slots [s0, s1) of one wave; next[e] (LDS, this wave's own): where the expert's next slot goes
 __device__ __forceinline__ void plan_place_piece(const PlanDev& a, int* next, int64_t s0, int64_t s1) {
     const int lane = threadIdx.x & 63;
-    for (int64_t t = s0; t < s1; t += 64) {
-        const int64_t s = t + lane;
-        const int e = slot_expert(a, s, s1);
-        unsigned long long same = __ballot(e >= 0);
-        for (int b = 0; b < a.bits; ++b) {
-            const unsigned long long ones = __ballot(e >> b & 1);
-            same &= (e >> b & 1) ? ones : ~ones;
+    constexpr int U = 4;
+    for (int64_t t = s0; t < s1; t += U * 64) {
+        int es[U];
+        slot_experts<U, 64>(a, t + lane, s1, es);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int64_t s = t + i * 64 + lane;
+            if (t + i * 64 >= s1) break;
+            const int e = es[i];
+            unsigned long long same = __ballot(e >= 0);
+            for (int b = 0; b < a.bits; ++b) {
+                const unsigned long long ones = __ballot(e >> b & 1);
+                same &= (e >> b & 1) ? ones : ~ones;
+            }
+            int pos = -1;
+            if (e >= 0) {
+                const int rank = __popcll(same & (((unsigned long long)1 << lane) - 1));
+                pos = next[e] + rank;
+            }
+            wave_sync();
+            if (e >= 0 && (same >> lane) == 1ull) next[e] = pos + 1;      // the last of them
+            wave_sync();
+            if (s < s1) a.positions[s] = pos;
+            if (pos >= 0) a.rows[pos] = (int)((unsigned)s / (unsigned)a.k);
         }
-        int pos = -1;
-        if (e >= 0) {
-            const int rank = __popcll(same & (((unsigned long long)1 << lane) - 1));
-            pos = next[e] + rank;
-        }
-        wave_sync();
-        if (e >= 0 && (same >> lane) == 1ull) next[e] = pos + 1;      // the last of them
-        wave_sync();
-        if (s < s1) a.positions[s] = pos;
-        if (pos >= 0) a.rows[pos] = (int)(s / a.k);
     }
 }
 
@@ -579,10 +605,7 @@ __global__ void __launch_bounds__(1024) plan_small_kernel(PlanDev a) {
     for (int i = tid; i < 16 * a.E; i += 1024) cnt[i] = 0;
     __syncthreads();
     const int64_t s0 = wave * a.piece < a.slots ? wave * a.piece : a.slots, s1 = s0 + a.piece < a.slots ? s0 + a.piece : a.slots;
-    for (int64_t s = s0 + lane; s < s1; s += 64) {
-        const int e = slot_expert(a, s, s1);
-        if (e >= 0) atomicAdd(&cnt[wave * a.E + e], 1);
-    }
+    plan_count_slots<64>(a, cnt + wave * a.E, s0, s1, lane);
     __syncthreads();
     int total = 0;                                    // E <= 1024: one expert per thread
     if (tid < a.E) for (int w = 0; w < 16; ++w) total += cnt[w * a.E + tid];
@@ -611,10 +634,7 @@ __global__ void __launch_bounds__(256) plan_count_kernel(PlanDev a) {
     for (int e = lane; e < a.E; e += 64) mine[e] = 0;
     wave_sync();
     const int64_t s0 = piece * a.piece, s1 = s0 + a.piece < a.slots ? s0 + a.piece : a.slots;
-    for (int64_t s = s0 + lane; s < s1; s += 64) {
-        const int e = slot_expert(a, s, s1);
-        if (e >= 0) atomicAdd(&mine[e], 1);
-    }
+    plan_count_slots<64>(a, mine, s0, s1, lane);
     wave_sync();
     if (piece < a.npieces) for (int e = lane; e < a.E; e += 64) a.ws[(int64_t)e * a.npieces + piece] = mine[e];
 }
@@ -671,22 +691,82 @@ __global__ void __launch_bounds__(256) plan_place_kernel(PlanDev a) {
     }
 }
 
-static void plan_pieces(int64_t slots, int E, int64_t* piece, int* npieces, bool* small) {
-    *small = slots <= PLAN_SMALL_SLOTS && E <= 1024;
-    // 8 waves a compute unit; with many experts fewer, so that the table of counts stays within 2^20 integers
-    const int want = *small ? 16 : E <= 512 ? PLAN_MAX_PIECES : (1 << 20) / E;
+// Few experts: the counts of 512 pieces, a workgroup each, ...
+__global__ void __launch_bounds__(256) plan_count_piece_kernel(PlanDev a) {
+    __shared__ int cnt[PLAN_JOIN_EXPERTS];
+    const int tid = threadIdx.x;
+    if (tid < a.E) cnt[tid] = 0;
+    __syncthreads();
+    const int64_t s0 = blockIdx.x * a.piece, s1 = s0 + a.piece < a.slots ? s0 + a.piece : a.slots;
+    plan_count_slots<256>(a, cnt, s0, s1, tid);
+    __syncthreads();
+    if (tid < a.E) a.ws[(int64_t)tid * a.npieces + blockIdx.x] = cnt[tid];
+}
+
+// ... which every workgroup sums itself (wave w the experts w, w + 4, ...) before each of its waves places a quarter of its piece
+__global__ void __launch_bounds__(256) plan_join_kernel(PlanDev a) {
+    __shared__ int cnt[4][64], next[4][PLAN_JOIN_EXPERTS], before[PLAN_JOIN_EXPERTS], total[PLAN_JOIN_EXPERTS];
+    static_assert(PLAN_JOIN_EXPERTS <= 64, "a lane an expert");
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, piece = (int)blockIdx.x;
+    const int64_t end = (piece + 1) * a.piece < a.slots ? (piece + 1) * a.piece : a.slots, quarter = a.piece / 4;
+    const int64_t q0 = piece * a.piece + wave * quarter, s0 = q0 < end ? q0 : end, s1 = s0 + quarter < end ? s0 + quarter : end;
+    cnt[wave][lane] = 0;
+    wave_sync();
+    plan_count_slots<64>(a, cnt[wave], s0, s1, lane);
+    constexpr int U = 4;                              // columns asked for together
+    for (int e0 = wave; e0 < a.E; e0 += 4 * U) {
+        int c[U][PLAN_JOIN_PIECES / 64];
+#pragma unroll
+        for (int q = 0; q < U; ++q) {
+            const int* col = a.ws + (int64_t)(e0 + 4 * q < a.E ? e0 + 4 * q : e0) * a.npieces;
+#pragma unroll
+            for (int i = 0; i < PLAN_JOIN_PIECES / 64; ++i) c[q][i] = i * 64 + lane < a.npieces ? col[i * 64 + lane] : 0;
+        }
+#pragma unroll
+        for (int q = 0; q < U; ++q) {
+            int mine = 0, all = 0;
+#pragma unroll
+            for (int i = 0; i < PLAN_JOIN_PIECES / 64; ++i) { all += c[q][i]; mine += i * 64 + lane < piece ? c[q][i] : 0; }
+            mine = lanes_reduce<64>(mine, OpSum());
+            all = lanes_reduce<64>(all, OpSum());
+            if (lane == 0 && e0 + 4 * q < a.E) { before[e0 + 4 * q] = mine; total[e0 + 4 * q] = all; }
+        }
+    }
+    __syncthreads();
+    const int mine = lane < a.E ? total[lane] : 0;
+    int incl = mine;
+    for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(incl, d, 64); if (lane >= d) incl += o; }
+    const int off = incl - mine, all = __shfl(incl, 63, 64);
+    if (lane < a.E) {
+        int at = off + before[lane];
+        for (int w = 0; w < wave; ++w) at += cnt[w][lane];
+        next[wave][lane] = at;
+        if (piece == 0 && wave == 0) { a.counts[lane] = mine; a.offsets[lane] = off; }
+    }
+    if (piece == 0 && threadIdx.x == 0) a.offsets[a.E] = all;
+    wave_sync();
+    plan_place_piece(a, next[wave], s0, s1);
+    for (int64_t s = s0 + lane; s < s1; s += 64) if (s >= all) a.rows[s] = -1;
+}
+
+enum { PLAN_SMALL = 0, PLAN_JOIN = 1, PLAN_SCAN = 2 };
+
+static int plan_pieces(int64_t slots, int E, int64_t* piece, int* npieces) {
+    const int kind = slots <= PLAN_SMALL_SLOTS && E <= 1024 ? PLAN_SMALL : E <= PLAN_JOIN_EXPERTS && slots <= PLAN_JOIN_SLOTS ? PLAN_JOIN : PLAN_SCAN;
+    // PLAN_SCAN: 8 waves a compute unit; with many experts fewer, so that the table of counts stays within 2^20 integers
+    const int want = kind == PLAN_SMALL ? 16 : kind == PLAN_JOIN ? PLAN_JOIN_PIECES : E <= 512 ? PLAN_MAX_PIECES : (1 << 20) / E;
+    const int64_t step = kind == PLAN_JOIN ? 256 : 64, least = kind == PLAN_SMALL ? 64 : 256;
     int64_t p = (slots + want - 1) / want;
-    const int64_t least = *small ? 64 : 256;
-    p = p < least ? least : (p + 63) / 64 * 64;
+    p = p < least ? least : (p + step - 1) / step * step;
     *piece = p;
     *npieces = (int)((slots + p - 1) / p);
+    return kind;
 }
 
 static int64_t plan_workspace(int64_t n_rows, int32_t top_k, int32_t n_experts) {
     if (n_rows <= 0 || top_k <= 0 || n_experts <= 0 || n_experts > OAK_MAX_PLAN_EXPERTS || n_rows > MOST_SLOTS / top_k) return 0;
-    int64_t piece; int np; bool small;
-    plan_pieces(n_rows * top_k, n_experts, &piece, &np, &small);
-    return small ? 0 : (int64_t)np * n_experts;
+    int64_t piece; int np;
+    return plan_pieces(n_rows * top_k, n_experts, &piece, &np) == PLAN_SMALL ? 0 : (int64_t)np * n_experts;
 }
 
 static int plan_check(const oak_plan_args* a) {
@@ -700,15 +780,18 @@ static int plan_check(const oak_plan_args* a) {
 
 static int plan_launch(hipStream_t stream, const oak_plan_args* a) {
     PlanDev d{};
-    bool small;
     d.slots = a->n_rows * a->top_k; d.k = a->top_k; d.E = a->n_experts;
-    plan_pieces(d.slots, d.E, &d.piece, &d.npieces, &small);
+    const int kind = plan_pieces(d.slots, d.E, &d.piece, &d.npieces);
     d.experts = a->experts; d.rows = a->rows; d.positions = a->positions; d.counts = a->counts; d.offsets = a->offsets; d.ws = a->workspace;
     while ((1 << d.bits) < d.E) ++d.bits;
-    if (small) {
+    if (kind == PLAN_SMALL) {
         const size_t lds = (size_t)16 * d.E * sizeof(int);
         if (lds > 32 * 1024) OAK_CHECK(ensure_dynamic_lds((const void*)plan_small_kernel, 16 * 1024 * sizeof(int)));
         return launch(plan_small_kernel, dim3(1), dim3(1024), lds, stream, d);
+    }
+    if (kind == PLAN_JOIN) {
+        OAK_CHECK(launch(plan_count_piece_kernel, dim3((unsigned)d.npieces), dim3(256), 0, stream, d));
+        return launch(plan_join_kernel, dim3((unsigned)d.npieces), dim3(256), 0, stream, d);
     }
     const unsigned wgs = (unsigned)((d.npieces + 3) / 4);
     const size_t lds = (size_t)(5 * d.E + 1) * sizeof(int);

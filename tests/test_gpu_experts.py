@@ -168,7 +168,8 @@ def test_route_strides_offsets_and_empty():
 
 
 PLANS = [(0, 2, 5), (1, 1, 1), (3, 2, 16), (64, 1, 7), (1000, 6, 160), (4096, 4, 1024), (4097, 4, 24), (5000, 4, 1025), (40000, 2, 3),
-         (70001, 8, 333), (6000, 3, 4096)]
+         (70001, 8, 333), (6000, 3, 4096), (16385, 1, 1), (100003, 3, 24), (30000, 6, 32),
+         (30000, 6, 33), (1 << 20, 1, 2), (349526, 3, 32)]
 
 
 @pytest.mark.parametrize("n,k,e", PLANS)
