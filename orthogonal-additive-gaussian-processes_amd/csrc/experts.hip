@@ -128,6 +128,14 @@ __device__ __forceinline__ unsigned tag_of(double v) {
     return ((unsigned)b ^ (unsigned)((int)(unsigned)(b >> 32) >> 31)) & TAG_BITS;
 }
 
+// Maximum and minimum of a lane's own keys.  fmax() first quietens operands that may be signalling NaN (v_max_f64 of a register with itself),
+// half of a selection's instructions where keys are put together from bits.  The results go to data-parallel moves first, never straight to
+// a row swap, whose wait after an instruction of inline assembly is not the compiler's concern.
+__device__ __forceinline__ double key_max(double a, double b) { double r; asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; }
+__device__ __forceinline__ double key_min(double a, double b) { double r; asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; }
+__device__ __forceinline__ float key_max(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ float key_min(float a, float b) { return __builtin_fminf(a, b); }
+
 template <int KIND, int L, int VPL>
 __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
     using acc = std::conditional_t<KIND == KEY_F64, double, float>;
@@ -196,8 +204,8 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
             clean m1 = CLOSED, m2 = CLOSED;
 #pragma unroll
             for (int s = 0; s < VPL; ++s) {
-                m2 = OpMax()(m2, OpMin()(v[s], m1));
-                m1 = OpMax()(m1, v[s]);
+                m2 = key_max(m2, key_min(v[s], m1));
+                m1 = key_max(m1, v[s]);
             }
             auto join = [&](auto mc) {
                 constexpr int M = decltype(mc)::value;
@@ -231,8 +239,8 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
                 clean m1 = CLOSED, m2 = CLOSED;
                 for (int i = 0; i < a.group_size; ++i) {
                     const clean t = keys[g * a.group_size + i];
-                    m2 = OpMax()(m2, OpMin()(t, m1));
-                    m1 = OpMax()(m1, t);
+                    m2 = key_max(m2, key_min(t, m1));
+                    m1 = key_max(m1, t);
                 }
                 gs[g] = a.top2 && is_open(m2) ? m1 + m2 : m1;
             }
@@ -298,7 +306,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
         for (int j = 0; j < a.k; ++j) {
             double m = v[0];
 #pragma unroll
-            for (int s = 1; s < VPL; ++s) m = OpMax()(m, v[s]);
+            for (int s = 1; s < VPL; ++s) m = key_max(m, v[s]);
             m = lanes_reduce<L>(m, OpMax());
 #pragma unroll
             for (int s = 0; s < VPL; ++s) v[s] = with_hi(v[s], v[s] == m ? CLOSED_HI : hi_of(v[s]));
@@ -389,8 +397,12 @@ __global__ void __launch_bounds__(256) route_grad_kernel(RouteDev a) {
     wave_sync();
 
     acc r = 0;
-    const acc p = (acc)1 / ((acc)1 + exp(-xe)), not_p = (acc)1 / ((acc)1 + exp(xe));     // sigmoid and 1 - sigmoid, each to its own size
-    if (chosen) r = a.sigmoid && (!a.renorm || xmax > (acc)-40) ? p : exp_of(xe - xmax);
+    acc not_p = 1;
+    if (a.sigmoid) {
+        const acc p = (acc)1 / ((acc)1 + exp(-xe));        // sigmoid and 1 - sigmoid, each to its own size
+        not_p = (acc)1 / ((acc)1 + exp(xe));
+        if (chosen) r = !a.renorm || xmax > (acc)-40 ? p : exp_of(xe - xmax);
+    } else if (chosen) r = exp_of(xe - xmax);
     if (dense) r *= inv;
     else if (a.renorm) r /= lanes_reduce<L>(r, OpSum());       // one expert's r is 1, its gradient 0
     const acc dot = lanes_reduce<L>(r * g, OpSum());
@@ -399,7 +411,7 @@ __global__ void __launch_bounds__(256) route_grad_kernel(RouteDev a) {
         acc d = g;
         if (!dense) {
             d = a.renorm ? r * (g - dot) : r * g;
-            if (a.sigmoid) d *= not_p;
+            d *= not_p;
         }
         atomicAdd(&buf[e], d);
     }
