@@ -370,57 +370,57 @@ __global__ void __launch_bounds__(256) route_grad_kernel(RouteDev a) {
     acc* buf = reinterpret_cast<acc*>(lds) + (size_t)(wave * TEAMS + team) * (L * VPL);
     const bool dense = !a.sigmoid && !a.renorm;
 
-    // this lane's slot (L >= k)
-    const int e = l < a.k ? a.experts[at * a.k + l] : -1;
-    const bool chosen = e >= 0 && e < a.E;
-    const acc xe = chosen ? score_at<acc>(a, at, e) : (acc)0;
-    const acc g = chosen ? (acc)a.scale * static_cast<const acc*>(a.dweights)[at * a.k + l] : (acc)0;
-
-    acc x[VPL], xmax, inv = 0;
+    // this lane's slot (L >= k); both loads on their way before either is looked at
+    const int64_t slot = at * a.k + (l < a.k ? l : 0);
+    const int e_read = a.experts[slot];
+    const acc dw = static_cast<const acc*>(a.dweights)[slot];
+    acc x[VPL], out[VPL];
     if (dense) {
         open_scores<L, VPL>(a, at, base, x);
-        xmax = x[0];
+    } else {
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) x[s] = 0;
+    }
+#pragma unroll
+    for (int s = 0; s < VPL; ++s) buf[base + s] = 0;
+    const int e = l < a.k ? e_read : -1;
+    const bool chosen = e >= 0 && e < a.E;
+    const acc g = chosen ? (acc)a.scale * dw : (acc)0;
+    const bool some = lanes_reduce<L>(chosen ? 1u : 0u, OpMax()) != 0;
+    wave_sync();
+    if (dense) {
+        // every element against its g, 0 for what was not chosen
+        if (chosen) atomicAdd(&buf[e], g);
+        acc xmax = x[0];
 #pragma unroll
         for (int s = 1; s < VPL; ++s) xmax = OpMax()(xmax, x[s]);
         xmax = lanes_reduce<L>(xmax, OpMax());
         acc z = 0;
 #pragma unroll
         for (int s = 0; s < VPL; ++s) { x[s] = exp_of(x[s] - xmax); z += x[s]; }
-        inv = inverse(lanes_reduce<L>(z, OpSum()));
+        wave_sync();
+        acc dot = 0;
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) { out[s] = buf[base + s]; dot += x[s] * out[s]; }
+        const acc inv = inverse(lanes_reduce<L>(z, OpSum()));
+        dot = lanes_reduce<L>(dot, OpSum()) * inv;
+#pragma unroll
+        for (int s = 0; s < VPL; ++s) out[s] = some ? x[s] * inv * (out[s] - dot) : (acc)0;
     } else {
+        const acc xe = chosen ? score_at<acc>(a, at, e) : (acc)0;
+        const acc xmax = lanes_reduce<L>(chosen ? xe : (acc)-INFINITY, OpMax());
+        acc r = 0, not_p = 1;
+        if (a.sigmoid) {
+            const acc p = (acc)1 / ((acc)1 + exp(-xe));        // sigmoid and 1 - sigmoid, each to its own size
+            not_p = (acc)1 / ((acc)1 + exp(xe));
+            if (chosen) r = !a.renorm || xmax > (acc)-40 ? p : exp_of(xe - xmax);
+        } else if (chosen) r = exp_of(xe - xmax);
+        if (a.renorm) r /= lanes_reduce<L>(r, OpSum());        // one expert's r is 1, its gradient 0
+        const acc dot = lanes_reduce<L>(r * g, OpSum());
+        if (chosen) atomicAdd(&buf[e], (a.renorm ? r * (g - dot) : r * g) * not_p);
+        wave_sync();
 #pragma unroll
-        for (int s = 0; s < VPL; ++s) x[s] = 0;
-        xmax = lanes_reduce<L>(chosen ? xe : (acc)-INFINITY, OpMax());
-    }
-#pragma unroll
-    for (int s = 0; s < VPL; ++s) buf[base + s] = 0;
-    wave_sync();
-
-    acc r = 0;
-    acc not_p = 1;
-    if (a.sigmoid) {
-        const acc p = (acc)1 / ((acc)1 + exp(-xe));        // sigmoid and 1 - sigmoid, each to its own size
-        not_p = (acc)1 / ((acc)1 + exp(xe));
-        if (chosen) r = !a.renorm || xmax > (acc)-40 ? p : exp_of(xe - xmax);
-    } else if (chosen) r = exp_of(xe - xmax);
-    if (dense) r *= inv;
-    else if (a.renorm) r /= lanes_reduce<L>(r, OpSum());       // one expert's r is 1, its gradient 0
-    const acc dot = lanes_reduce<L>(r * g, OpSum());
-    const bool some = lanes_reduce<L>(chosen ? 1u : 0u, OpMax()) != 0;
-    if (chosen) {
-        acc d = g;
-        if (!dense) {
-            d = a.renorm ? r * (g - dot) : r * g;
-            d *= not_p;
-        }
-        atomicAdd(&buf[e], d);
-    }
-    wave_sync();
-    acc out[VPL];
-#pragma unroll
-    for (int s = 0; s < VPL; ++s) {
-        const acc d = buf[base + s];
-        out[s] = dense ? (some ? x[s] * inv * (d - dot) : (acc)0) : d;
+        for (int s = 0; s < VPL; ++s) out[s] = buf[base + s];
     }
     if (!live) return;
     if constexpr (sizeof(acc) == 8) store_pieces<acc, VPL>(static_cast<double*>(a.dscores) + row * a.ld_out, base, a.E, out);
