@@ -438,11 +438,12 @@ int oak_kmeans_plusplus(oak_ctx* ctx, const double* X, int64_t N, int32_t D, int
 int oak_device_pointer_check(oak_ctx* ctx, const void* p);
 
 /* Each row's experts.  p = softmax over the row's open scores, or sigmoid; a score is open unless its mask is 0 or it is -inf.
-   key = p + bias where there is a bias (it moves the choice, not the weights; |bias| < 1e300), else the score itself.  With n_groups > 1 only the
+   key = p + bias where there is a bias (it moves the choice, not the weights; |bias| < 1e300, or -inf, which closes the expert to the choice), else
+   the score itself.  With n_groups > 1 only the
    top_groups groups of consecutive experts with the highest group scores stay open (OAK_GROUP_MAX: the highest key, OAK_GROUP_TOP2: the
    sum of the two highest p + bias; ties by lower index).  The top_k highest keys are chosen, highest first, ties by lower index (p + bias is
    formed in 64 bits; unless the scores are float64, sums closer than 2^-41 of their size count as ties); slots left over get expert -1 and weight 0.  weight = scale p, or scale p / sum of the chosen p.
-   A row with a NaN or +inf among its open scores gets experts -1 and weights NaN.
+   A row with a NaN or +inf among its open scores, or their bias, gets experts -1 and weights NaN.
    oak_route_grad: dscores from dweights for the experts chosen, recomputing p; the choice itself is not differentiated, slots whose expert is
    not in [0, n_experts) count for nothing and a row without experts has gradient 0. */
 typedef struct oak_route_args {

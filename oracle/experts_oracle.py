@@ -15,14 +15,17 @@ def route(x, k, score="softmax", bias=None, n_groups=1, top_groups=None, group_s
         if any(not x[i, c] < np.inf for c in open_):
             weights[i] = np.nan
             continue
+        if bias is not None and any(not bias[c] < np.inf for c in open_):
+            weights[i] = np.nan
+            continue
         p = probabilities(x[i], open_, score)
-        key = {c: p[c] + float(bias[c]) if bias is not None else x[i, c] for c in open_}
+        key = {c: p[c] + float(bias[c]) if bias is not None else x[i, c] for c in open_ if bias is None or bias[c] != -np.inf}
         if n_groups > 1:
             size = e // n_groups
             gs = []
             rank = key if bias is not None or group_score == "max" else {c: p[c] for c in open_}       # sums are sums of probabilities
             for g in range(n_groups):
-                mine = sorted((rank[c] for c in open_ if c // size == g), reverse=True)
+                mine = sorted((rank[c] for c in key if c // size == g), reverse=True)
                 gs.append(-np.inf if not mine else sum(mine[:2]) if group_score == "top2" else mine[0])
             keep = set(sorted(range(n_groups), key=lambda g: (-gs[g], g))[:top_groups])
             key = {c: v for c, v in key.items() if c // size in keep}

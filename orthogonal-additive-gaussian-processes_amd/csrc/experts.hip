@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
     const int base = l * VPL;
 
     acc x[VPL];
-    const bool bad = open_scores<L, VPL>(a, at, base, x);
+    bool bad = open_scores<L, VPL>(a, at, base, x);
 
     // the softmax's maximum and sum, where something asks for them
     const bool plain_keys = KIND == KEY_16 || (a.bias == nullptr && !(a.groups > 1 && a.top2));
@@ -184,8 +184,20 @@ __global__ void __launch_bounds__(256) route_kernel(RouteDev a) {
             double b[VPL];
             if (a.bias_f64) load_pieces<double, VPL>(static_cast<const double*>(a.bias), base, a.E, b, 0.0);
             else load_pieces<float, VPL>(static_cast<const float*>(a.bias), base, a.E, b, 0.0);
+            double odd = 0.0;                             // NaN if an entry is infinite or NaN: one instruction a score finds out
 #pragma unroll
-            for (int s = 0; s < VPL; ++s) v[s] += b[s];
+            for (int s = 0; s < VPL; ++s) { v[s] += b[s]; odd = __builtin_fma(b[s], 0.0, odd); }
+            if (__any(odd != odd)) {
+                // -inf closes its expert, NaN and +inf are like such a score (a tag would turn an infinite key into NaN)
+                bool wrong = false;
+#pragma unroll
+                for (int s = 0; s < VPL; ++s) {
+                    const double t = base + s >= a.E ? 0.0 : load_any(a.bias, a.bias_f64 ? OAK_F64 : OAK_F32, base + s);
+                    wrong |= x[s] > (acc)-INFINITY && !(t < INFINITY);
+                    if (t == -INFINITY) x[s] = -INFINITY;
+                }
+                bad |= lanes_reduce<L>(wrong ? 1u : 0u, OpOr()) != 0;
+            }
         }
     }
     // a closed key: -inf, but for tags the lowest double (-inf with a tag would be NaN); scores of 64 bits reach that one themselves

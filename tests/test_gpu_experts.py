@@ -508,3 +508,42 @@ def test_views_that_negate_when_they_are_read():
     assert x.is_neg()
     p = ox.plan(torch.zeros(7, 1, dtype=torch.int32, device="cuda"), 1)
     np.testing.assert_array_equal(back(ox.dispatch(x, p)), -back(z.imag.contiguous()))
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32", "bf16", "f16"])
+@pytest.mark.parametrize("opt", [{}, dict(renormalise=False), dict(score="sigmoid"), dict(n_groups=4, top_groups=2, group_score="top2"),
+                                 dict(score="sigmoid", n_groups=4, top_groups=3, renormalise=False), dict(n_groups=20, top_groups=5)])
+def test_bias_closes_experts_and_what_is_no_number_shows(dtype, opt):
+    """-inf in the bias closes its expert for every row; rows for which an expert of bias NaN or +inf is open hold -1 and NaN."""
+    rng = np.random.default_rng(17)
+    n, e, k = 90, 60, 5
+    x, xr = scores_of(rng, n, e, dtype)
+    mask = rng.random((n, e)) < 0.9
+    mask[:40, [7, 33]] = False
+    bias = rng.standard_normal(e) * 0.05
+    for odd in ((-np.inf, -np.inf), (np.nan, -np.inf), (-np.inf, np.inf), (np.nan, np.inf)):
+        bias[[7, 33]] = odd
+        bias[[0, 12, 50, 59]] = -np.inf
+        b32 = bias.astype(np.float32)
+        for b in (torch.as_tensor(b32, device="cuda"), torch.as_tensor(b32.astype(np.float64), device="cuda")):
+            ex, w = ox.route(x, k, bias=b, mask=torch.as_tensor(mask, device="cuda"), **opt)
+            er, wr = eo.route(xr, k, bias=b32, mask=mask, **opt)
+            np.testing.assert_array_equal(back(ex), er)
+            check_weights(back(w), wr, xr, er, dtype, opt)
+            assert not np.isin(back(ex), [0, 12, 50, 59]).any() and (back(ex)[:40] >= 0).all()
+            assert (back(ex)[40:][mask[40:, 7] & ~np.isneginf(odd[0])] == -1).all()
+    bias[:] = -np.inf
+    ex, w = ox.route(x, k, bias=torch.as_tensor(bias, device="cuda"), **opt)
+    assert (ex == -1).all() and (w == 0).all()
+
+
+def test_bias_of_numpy_arrays_may_close_experts():
+    rng = np.random.default_rng(18)
+    x, bias = rng.standard_normal((50, 12)), rng.standard_normal(12) * 0.05
+    bias[[0, 5]] = -np.inf
+    for kw in (dict(), dict(score="sigmoid", n_groups=3, top_groups=2, group_score="top2"), dict(renormalise=False)):
+        ex, w = ox.route(x, 3, bias=bias, **kw)
+        er, wr = eo.route(x, 3, bias=bias, **kw)
+        np.testing.assert_array_equal(ex, er)
+        np.testing.assert_allclose(w, wr, rtol=1e-13, atol=1e-300)
+        assert not np.isin(ex, [0, 5]).any()
