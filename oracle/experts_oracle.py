@@ -166,8 +166,9 @@ def distill(logits, top, index, top_lse=None, temperature=1.0, direction="forwar
                 terms = np.where(p > 0, p * (lp - lqt), 0.0)
                 kl = terms.sum() + (pr * (np.log(pr) - lqr) if pr > 0 else 0.0)
                 ratio = np.exp(np.log(pr) - lqr) if pr > 0 else 0.0
-                grad[i] = np.exp(lq) * (1.0 - ratio)
-                grad[i, classes] = np.exp(lqt) - p
+                total = p.sum() + pr                             # 1 unless top_lse leaves no room for it
+                grad[i] = np.exp(lq) * (total - ratio)
+                grad[i, classes] = np.exp(lqt) * total - p
                 size[i] = factor * (np.abs(p * lp).sum() + np.abs(p * lqt).sum() + abs(pr * lqr) + 1.0 + ratio)
             else:
                 q, qr = np.exp(lqt), np.exp(lqr) if rest else 0.0

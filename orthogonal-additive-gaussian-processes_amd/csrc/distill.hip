@@ -2,7 +2,8 @@
 //
 // With z = log sum_v exp(s_v / tau), q_v = exp(s_v / tau - z), "top" the teacher's entries and "rest" every other class:
 //   forward  L = tau^2 w [ sum p_k (log p_k - log q_k) + p_r (log p_r - log q_r) ]
-//            dL/ds_v = tau w (q_v - p_v) on the top,  tau w q_v (1 - p_r / q_r) on the rest   (p_r = 0 without a rest outcome)
+//            dL/ds_v = tau w (S q_v - p_v) on the top,  tau w q_v (S - p_r / q_r) on the rest   (p_r = 0 without a rest outcome; S = sum p_k + p_r,
+//            which is 1 unless a rounded top_lse puts the entries' own sum above 1, or the entries are all the classes)
 //   reverse  L = tau^2 w [ sum q_k (log q_k - log p_k) + q_r (log q_r - log p_r) ]
 //            dL/ds_v = tau w q_v (log q_b - log p_b - L / (tau^2 w)),  b the outcome v belongs to
 // so the gradient is one coefficient times q_v on the rest and k values of their own on the top.
@@ -336,20 +337,21 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
         }
 
         // ---- the row's numbers -----------------------------------------------------------------------------------------
-        double log_z = 0.0, kl = 0.0, coef = 0.0, psum = 1.0;        // log_z on xref
+        double log_z = 0.0, kl = 0.0, coef = 0.0, psum = 1.0, total = 1.0;        // log_z on xref, total the teacher's mass
         if (lead && todo == ROW_COMPUTE) {
             const double far = ((double)mr - xref) * a.inv_tau, log_zr = log_of(zr);
             const bool rest = a.lse != nullptr && some_rest;
             // z over all classes: the rest in 32 bits, the entries in 64.  Next to a sure student's entry (z = 1 + little) the little keeps its digits
             log_z = far > 0.0 ? far + log_of(zr + sums[3] * exp_of(-far)) : log_of(zr * exp_of(far) + sums[3]);
             const double lqr = far + log_zr - log_z, qr = some_rest ? exp_of(lqr) : 0.0;
-            double pr = 0.0, mass = qr;
+            double pr = 0.0, mass;
             if (a.lse == nullptr) {
                 psum = sums[0];
                 kl = (sums[1] - sums[2] * a.inv_tau) / psum - log_of(psum) + log_z;
             } else {
                 pr = rest ? 1.0 - sums[0] : 0.0;
                 pr = pr < 0.0 ? 0.0 : pr;
+                total = pr > 0.0 ? 1.0 : sums[0];
                 kl = sums[1] - sums[2] * a.inv_tau + sums[0] * log_z;
             }
             if (a.reverse) {
@@ -357,11 +359,11 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
                 kl = scale != 0.0 ? scale * (sums[4] * a.inv_tau - sums[5] - sums[3] * log_z) : 0.0;
                 if (qr != 0.0) kl += qr * lr;
                 mass = qr != 0.0 ? qr * (lr - kl) : 0.0;
-            } else if (pr > 0.0) {
-                kl += pr * (log_of(pr) - lqr);
-                mass = qr - pr;
+            } else {
+                if (pr > 0.0) kl += pr * (log_of(pr) - lqr);
+                mass = total * qr - pr;
             }
-            // mass e_v / sum e on the rest, e_v = exp((s_v - m_r) / tau): q_v (1 - p_r / q_r) would be 0 times infinity where the student is
+            // mass e_v / sum e on the rest, e_v = exp((s_v - m_r) / tau): q_v (S - p_r / q_r) would be 0 times infinity where the student is
             // sure of itself
             coef = zr == 0.0 ? 0.0 : mass / zr;
             coef *= a.tau * w;
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
                 for (int k = tid; k < a.K; k += LEAD) if (cls[k] >= 0) {
                     if (MODE == SPLIT && !(cls[k] / VN >= u_begin && cls[k] / VN < u_end) && !(tail > 0 && cls[k] >= nvec * VN)) continue;   // another slice's
                     const double q = ek[k] * scale;
-                    const double d = a.reverse ? (q != 0.0 ? q * (log_of(ek[k]) - log_z - tk[k] - kl) : 0.0) : q - pk[k] * ip;
+                    const double d = a.reverse ? (q != 0.0 ? q * (log_of(ek[k]) - log_z - tk[k] - kl) : 0.0) : total * q - pk[k] * ip;
                     g[cls[k]] = (T)(acc)(a.tau * w * d);
                 }
             }

@@ -338,3 +338,34 @@ def test_around_the_sizes_where_the_team_changes(units, dtype):
         for k, n in ((9, 270), (33, 260)):
             s, top, idx, lse = problem(n, v, min(k, v), dtype, True, 1.0, v + k)
             compare(s, top, idx, lse, 1.0, "forward", None, dtype)
+
+
+@pytest.mark.parametrize("k,shift", [(11, 0.4), (11, -0.7), (4, -0.7), (4, 0.4)])
+def test_gradient_where_the_kept_mass_is_not_what_top_lse_leaves(k, shift):
+    """A rounded top_lse (or one entry that is kept twice): the entries' mass passes 1, or they are all the classes and stay below it.  The
+    loss as it stands is differentiated: against differences, and a shift of all logits changes nothing."""
+    rng = np.random.default_rng(21)
+    n, v, tau = 5, 11, 1.3
+    s, top = rng.standard_normal((n, v)), rng.standard_normal((n, k)) * 2
+    idx = np.argsort(rng.random((n, v)), 1)[:, :k].copy()
+    lse = np.log(np.exp(top / tau).sum(1)) + shift                       # the entries' mass is exp(-shift)
+    kw = dict(top_lse=lse, temperature=tau)
+    loss, grad = od.distill_grad(s, top, idx, **kw)
+    ref, gref, _ = eo.distill(s, top, idx, lse, tau)
+    np.testing.assert_allclose(loss, ref, rtol=1e-12, atol=1e-13)
+    np.testing.assert_allclose(grad, gref, rtol=1e-11, atol=1e-13)
+    np.testing.assert_allclose(grad.sum(1), 0, atol=1e-12)
+    for i, j in ((0, idx[0, 0]), (2, 7), (3, idx[3, 2]), (4, 10)):
+        up, down = s.copy(), s.copy()
+        up[i, j] += 1e-5
+        down[i, j] -= 1e-5
+        fd = (od.distill(up, top, idx, **kw).sum() - od.distill(down, top, idx, **kw).sum()) / 2e-5
+        assert abs(fd - grad[i, j]) <= 1e-8
+
+
+@pytest.mark.parametrize("v", [40, 5000, 140001])
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "f64"])
+def test_top_lse_of_16_bits(v, dtype):
+    s, top, idx, lse = problem(6, v, 9, dtype, True, spread=6.0, seed=2)  # nearly all of the teacher's mass is kept
+    for low in (lse.to(torch.bfloat16), (lse - 0.02).to(torch.float16)):
+        compare(s, top, idx, low, 1.0, "forward", None, dtype)
