@@ -200,8 +200,9 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
             double tmax = -INFINITY;
             for (int k = tid; k < a.K; k += LEAD) {
                 const int64_t c = a.index_64 ? static_cast<const int64_t*>(a.index)[row * a.ld_index + k] : static_cast<const int32_t*>(a.index)[row * a.ld_index + k];
-                const double t = load_any(a.top, a.top_dtype, row * a.ld_top + k) * a.inv_tau;
-                const bool in = c >= 0 && c < a.V, there = in && !(t == -INFINITY);
+                const double kept = load_any(a.top, a.top_dtype, row * a.ld_top + k), scaled = kept * a.inv_tau;
+                const double t = scaled < lowest(double()) ? lowest(double()) : scaled;      // a value that is not -inf is an entry at any temperature
+                const bool in = c >= 0 && c < a.V, there = in && !(kept == -INFINITY);
                 wrong |= !in && c != -1 ? 1u : 0u;
                 cls[k] = there ? (int)c : -1;
                 if (there) {

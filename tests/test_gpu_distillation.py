@@ -369,3 +369,21 @@ def test_top_lse_of_16_bits(v, dtype):
     s, top, idx, lse = problem(6, v, 9, dtype, True, spread=6.0, seed=2)  # nearly all of the teacher's mass is kept
     for low in (lse.to(torch.bfloat16), (lse - 0.02).to(torch.float16)):
         compare(s, top, idx, low, 1.0, "forward", None, dtype)
+
+
+@pytest.mark.parametrize("v", [70, 5000, 70001])
+def test_lowest_values_are_entries_of_no_mass_and_not_padding(v):
+    """-inf is padding, the type's lowest value is not, whatever the temperature makes of it: its class stays out of the rest."""
+    s, top, idx, lse = problem(3, v, 6, "f64", True, 0.5)
+    low, far = top.clone(), top.clone()
+    for t, value in ((low, torch.finfo(torch.float64).min), (far, -1e5)):
+        t[0, 3:] = value
+        t[1] = value
+    for given in (lse, None):
+        for a, b in zip(od.distill_grad(s, low, idx, top_lse=given, temperature=0.5), od.distill_grad(s, far, idx, top_lse=given, temperature=0.5)):
+            assert torch.equal(a, b)
+        assert torch.equal(od.distill(s, low, idx, top_lse=given, temperature=0.5), od.distill(s, far, idx, top_lse=given, temperature=0.5))
+    ref, gref, _ = eo.distill(back(s), back(far), back(idx), back(lse), 0.5)
+    loss, grad = od.distill_grad(s, low, idx, top_lse=lse, temperature=0.5)
+    np.testing.assert_allclose(back(loss), ref, rtol=1e-11)
+    np.testing.assert_allclose(back(grad), gref, rtol=1e-10, atol=1e-14)
