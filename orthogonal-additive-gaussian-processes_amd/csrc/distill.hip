@@ -9,8 +9,9 @@
 // so the gradient is one coefficient times q_v on the rest and k values of their own on the top.
 //
 // q_r is summed over the rest itself (the teacher's entries left out, found by a bit per class in LDS): taken as 1 - sum q_k it would lose
-// every digit where the student is sure of itself, and so would log z next to one sure class.  The sums over the classes run in 32 bits
-// (64 for double), everything per entry and per row in 64.
+// every digit where the student is sure of itself, and so would log z next to one sure class.  Exponentials and the sum over the 4 or 8 classes
+// of a 16-byte unit are 32 bits (64 for double), everything across units, per entry and per row is 64: a lane takes up to 2048 classes, and a flat
+// row rounds alike at every step of a running sum in 32 bits (1e-5 of the sum at 2^20 classes).
 //
 // A row stays in the registers of its team of NT threads, NV units of 16 bytes each, so that it is read once: the sum and the gradient
 // each walk the registers (LONG: what does not fit is read twice).  The team's first wave (all of a smaller team) does what concerns the entries.
@@ -76,15 +77,20 @@ template <typename T> __device__ __forceinline__ typename Vec<T>::raw hidden(typ
     }
 }
 
+// sum over one unit, on m
+template <int VN, typename A, typename R> __device__ __forceinline__ A sum_unit(const DistillDev& a, const R& r, A m) {
+    A sum = exp_scaled(a, (A)r[0] - m);
+#pragma unroll
+    for (int j = 1; j < VN; ++j) sum += exp_scaled(a, (A)r[j] - m);
+    return sum;
+}
 // one more unit into a running maximum m and sum z
-template <int VN, typename A, typename R> __device__ __forceinline__ void take_unit(const DistillDev& a, const R& r, A& m, A& z) {
+template <int VN, typename A, typename R> __device__ __forceinline__ void take_unit(const DistillDev& a, const R& r, A& m, double& z) {
     A top = m;
 #pragma unroll
     for (int j = 0; j < VN; ++j) top = OpMax()(top, (A)r[j]);
-    z *= exp_scaled(a, m - top);
+    z = z * (double)exp_scaled(a, m - top) + (double)sum_unit<VN>(a, r, top);
     m = top;
-#pragma unroll
-    for (int j = 0; j < VN; ++j) z += exp_scaled(a, (A)r[j] - m);
 }
 
 // Few rows: maximum and sum of the rest over one slice of one row.
@@ -108,7 +114,8 @@ template <typename T, int NT> __global__ void __launch_bounds__(NT) distill_slic
             atomicOr(&bits[(c - v_begin) >> 5], 1u << ((c - v_begin) & 31));
     }
     __syncthreads();
-    acc m = lowest(acc()), z = 0;
+    acc m = lowest(acc());
+    double z = 0.0;
     for (int u0 = u_begin + tid; u0 < u_end; u0 += U * NT) {
         typename Vec<T>::raw r[U];
 #pragma unroll
@@ -129,8 +136,8 @@ template <typename T, int NT> __global__ void __launch_bounds__(NT) distill_slic
         take_unit<1>(a, one, m, z);
     }
     const acc mw = lanes_reduce<64>(m, OpMax());
-    const acc zw = lanes_reduce<64>(z * exp_scaled(a, m - mw), OpSum());
-    if ((tid & 63) == 0) { share[tid >> 6][0] = (double)mw; share[tid >> 6][1] = (double)zw; }
+    const double zw = lanes_reduce<64>(z * (double)exp_scaled(a, m - mw), OpSum());
+    if ((tid & 63) == 0) { share[tid >> 6][0] = (double)mw; share[tid >> 6][1] = zw; }
     __syncthreads();
     if (tid < NT / 64) {
         const double mine = share[tid][0], all = lanes_reduce<NT / 64>(mine, OpMax());
@@ -259,7 +266,8 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
             todo = (int)share[WAVES * 2];
         }
 
-        acc m = lowest(acc()), z = 0;                  // a finite start: -inf - m stays -inf
+        acc m = lowest(acc());                         // a finite start: -inf - m stays -inf
+        double z = 0.0;
         if (MODE != SPLIT && todo == ROW_COMPUTE) {
             auto forget = [&] {                         // the units, not their 32-bit forms, live from one walk to the next
 #pragma unroll
@@ -292,13 +300,11 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     if (i * NT + at < nvec) {
-                        const raw r = __builtin_bit_cast(raw, data[i]);
-#pragma unroll
-                        for (int j = 0; j < VN; ++j) z += exp_scaled(a, (acc)r[j] - m);
+                        z += (double)sum_unit<VN>(a, __builtin_bit_cast(raw, data[i]), m);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                z += exp_scaled(a, last - m);
+                z += (double)exp_scaled(a, last - m);
                 forget();
             }
             if constexpr (MODE == LONG) {
@@ -317,8 +323,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
         }
         // ---- across the team -------------------------------------------------------------------------------------------
         acc mr = lanes_reduce<LEAD>(m, OpMax());
-        z = lanes_reduce<LEAD>(z * exp_scaled(a, m - mr), OpSum());
-        double zr = (double)z;
+        double zr = lanes_reduce<LEAD>(z * (double)exp_scaled(a, m - mr), OpSum());
         if constexpr (MODE == SPLIT) {
             if (lead && todo == ROW_COMPUTE) {
                 const double* p = a.part + row * a.slices * 2;
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
         if (lead && todo == ROW_COMPUTE) {
             const double far = ((double)mr - xref) * a.inv_tau, log_zr = log_of(zr);
             const bool rest = a.lse != nullptr && some_rest;
-            // z over all classes: the rest in 32 bits, the entries in 64.  Next to a sure student's entry (z = 1 + little) the little keeps its digits
+            // z over all classes: the rest of 32-bit exponentials, the entries of 64-bit ones.  Next to a sure student's entry (z = 1 + little) the little keeps its digits
             log_z = far > 0.0 ? far + log_of(zr + sums[3] * exp_of(-far)) : log_of(zr * exp_of(far) + sums[3]);
             const double lqr = far + log_zr - log_z, qr = some_rest ? exp_of(lqr) : 0.0;
             double pr = 0.0, mass;

@@ -387,3 +387,26 @@ def test_lowest_values_are_entries_of_no_mass_and_not_padding(v):
     loss, grad = od.distill_grad(s, low, idx, top_lse=lse, temperature=0.5)
     np.testing.assert_allclose(back(loss), ref, rtol=1e-11)
     np.testing.assert_allclose(back(grad), gref, rtol=1e-10, atol=1e-14)
+
+
+@pytest.mark.parametrize("n,v", [(300, 4096), (300, 32768), (300, 131072), (2, 131072), (128, 1 << 20), (130, 1 << 20)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("t", [-1.25, -0.3125])
+def test_flat_rows_keep_the_digits_of_their_sum(n, v, dtype, t):
+    """Every 16-byte unit holds one 0 and otherwise t, so that a running sum in 32 bits would round alike at every step of every lane (at 2^20
+    classes by 179 u and more of the sum).  One sure class against the rest's sum S: L = log(1 + S e^-x).  A term carries |t| u of
+    its argument and 2 u of the exponential, a unit's sum at most as many additions as it has terms; everything else is 64 bits, the result one u."""
+    vn = 4 if dtype == "f32" else 8
+    row = torch.full((v,), t, dtype=torch.float64)
+    row[::vn] = 0.0
+    rest = float(row.exp().sum()) - 1.0                                  # without class 0, the teacher's
+    x = float(round(np.log(rest)))
+    row[0] = x
+    s = row.to("cuda").to(DT[dtype]).expand(n, v).contiguous()
+    ref = np.log1p(rest * np.exp(-x))
+    share = rest * np.exp(-x - ref)
+    top, idx = torch.zeros(n, 1, device="cuda"), torch.zeros(n, 1, dtype=torch.int64, device="cuda")
+    u = 2.0 ** -24
+    tol = share * (abs(t) + 2 + vn) * u + u * ref
+    loss = back(od.distill(s, top, idx))
+    assert (np.abs(loss - ref) <= tol).all(), (np.abs(loss - ref).max() / u, tol / u)
