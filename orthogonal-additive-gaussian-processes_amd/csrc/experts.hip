@@ -934,7 +934,8 @@ template <typename T, int CHUNK> __global__ void __launch_bounds__(256) combine_
 }
 
 // dF[place] = w dy, dw = <dy, F[place]>: slot by slot, the row of dy stays in the nearest cache, 4 units of both asked for together.  At
-// most 64 threads a row: the dot product is finished inside a wave.
+// most 64 threads a row: the dot product is finished inside a wave.  It is 32 bits within a unit and 64 across units: one lane adds up to a
+// 64th of a row, whose roundings all fall to one side where the row is flat (2^20 equal columns: 2e-4 of the sum in 32 bits).
 template <typename T, bool WIDE> __global__ void __launch_bounds__(256) combine_grad_kernel(MixDev a) {
     using acc = typename Num<T>::acc;
     const int64_t n = a.row0 + (int64_t)blockIdx.x * a.rows_per_wg + (threadIdx.x >> a.tpr_log2);
@@ -947,7 +948,7 @@ template <typename T, bool WIDE> __global__ void __launch_bounds__(256) combine_
     const int used = a.offsets[a.E];
     for (int j = 0; j < a.k; ++j) {
         const int64_t p = live ? place_of(a, n, j) : -1;
-        acc d = 0;
+        double d = 0.0;
         if (p >= 0) {
             const acc wj = w[n * a.k + j];
             const T* fr = F + p * a.ld_slots;
@@ -964,19 +965,21 @@ template <typename T, bool WIDE> __global__ void __launch_bounds__(256) combine_
 #pragma unroll
                 for (int i = 0; i < U; ++i) if (u0 + i * tpr < a.nvec) {
                     typename Vec<T>::raw o;
+                    acc unit = 0;
 #pragma unroll
-                    for (int e = 0; e < Vec<T>::N; ++e) { d += (acc)f[i][e] * (acc)v[i][e]; o[e] = (T)(wj * (acc)v[i][e]); }
+                    for (int e = 0; e < Vec<T>::N; ++e) { unit += (acc)f[i][e] * (acc)v[i][e]; o[e] = (T)(wj * (acc)v[i][e]); }
+                    d += (double)unit;
                     store_slot<T, WIDE>(gr + (u0 + i * tpr) * Vec<T>::N, o);
                 }
             }
             for (int64_t c = (int64_t)a.nvec * Vec<T>::N + t; c < a.C; c += tpr) {
                 const acc v = (acc)dy[c];
-                d += (acc)fr[c] * v;
+                d += (double)((acc)fr[c] * v);
                 gr[c] = (T)(wj * v);
             }
         }
         for (int m = 1; m < tpr; m <<= 1) d += __shfl_xor(d, m, 64);
-        if (live && t == 0) static_cast<acc*>(a.dweights)[n * a.k + j] = d;
+        if (live && t == 0) static_cast<acc*>(a.dweights)[n * a.k + j] = (acc)d;
         if (live && n * a.k + j >= used) for (int64_t u = t; u < a.units; u += tpr) zero_unit<T>(a, dF + (n * a.k + j) * (int64_t)a.C, u);
     }
 }

@@ -547,3 +547,19 @@ def test_bias_of_numpy_arrays_may_close_experts():
         np.testing.assert_array_equal(ex, er)
         np.testing.assert_allclose(w, wr, rtol=1e-13, atol=1e-300)
         assert not np.isin(ex, [0, 5]).any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("c", [65536, 1 << 20, (1 << 20) + 5])
+def test_weights_gradient_of_long_flat_rows(c, dtype):
+    """A long row of equal terms: one running sum in 32 bits would round the same way at every step.  Of the terms of a 16-byte unit each
+    carries a product's and at most 7 additions' roundings, the units are added in 64 bits, the result is rounded once: 9 u, and 2 u for the
+    elements left over, at most 7 of them a lane."""
+    p = ox.plan(torch.zeros(3, dtype=torch.int32, device="cuda"), 1)
+    F = torch.full((3, c), 1.0, device="cuda", dtype=DT[dtype])
+    dy = torch.full((3, c), 1.0, device="cuda", dtype=DT[dtype])
+    F[1], dy[1] = 0.2998046875, 0.2001953125
+    F[2], dy[2] = 1.0078125, 0.7109375
+    _, dw = ox.combine_grad(F, torch.ones(3, 1, device="cuda"), p, dy)
+    ref = (F.double() * dy.double()).sum(1).cpu().numpy()
+    assert (np.abs(back(dw)[:, 0] - ref) <= 11 * 2.0 ** -24 * ref).all(), (back(dw)[:, 0] / ref - 1) * 2.0 ** 24
