@@ -56,7 +56,7 @@ class Device:
             raise _capi.OakHipError("the first call on a device makes its context, which a stream cannot capture: make one call before the capture")
         with self.torch.cuda.device(self.index):            # making a context changes the current device
             ctx = _capi.device_context(self.index)
-        if t.numel() > 0:
+        if t.data_ptr() != 0:
             try:
                 _capi.check_device_pointer(ctx, t.data_ptr())
             except ValueError as e:
@@ -121,7 +121,10 @@ def ptr(a) -> int | None:
         return None
     if isinstance(a, np.ndarray):
         return a.ctypes.data if a.size else None
-    return a.data_ptr() or None
+    address = a.data_ptr()
+    if address == 0 and a.numel() > 0:                       # would be an array left out
+        raise ValueError("an array is zeros without storage; pass its clone()")
+    return address or None
 
 
 def host(a, what: str, shape=None) -> np.ndarray:

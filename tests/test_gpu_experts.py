@@ -563,3 +563,15 @@ def test_weights_gradient_of_long_flat_rows(c, dtype):
     _, dw = ox.combine_grad(F, torch.ones(3, 1, device="cuda"), p, dy)
     ref = (F.double() * dy.double()).sum(1).cpu().numpy()
     assert (np.abs(back(dw)[:, 0] - ref) <= 11 * 2.0 ** -24 * ref).all(), (back(dw)[:, 0] / ref - 1) * 2.0 ** 24
+
+
+def test_zeros_without_storage_are_refused():
+    """torch's zero tensors, which have no memory (tangents of what does not vary, for one), were taken for an array left out."""
+    z = torch._efficientzerotensor((2, 2), device="cuda")
+    p = ox.plan(torch.tensor([[0, 1], [1, 2]], dtype=torch.int32, device="cuda"), 3)
+    F, dy = torch.ones(4, 3, device="cuda"), torch.ones(2, 3, device="cuda")
+    for call in (lambda: ox.combine(F, z, p), lambda: ox.dispatch(z, p), lambda: ox.combine_grad(F, z, p, dy), lambda: ox.route(z, 1),
+                 lambda: ox.route(F, 1, bias=torch._efficientzerotensor((3,), device="cuda"))):
+        with pytest.raises(ValueError, match="without storage"):
+            call()
+    assert (ox.combine(F, z.clone(), p) == 0).all()

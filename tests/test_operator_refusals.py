@@ -159,3 +159,28 @@ def test_a_second_copy_of_the_hip_runtime_is_noticed(torch_first):
     out = subprocess.run([sys.executable, "-c", f"import sys; sys.path.insert(0, {str(_capi._PKG_ROOT)!r}); {code}"], capture_output=True, text=True)
     assert out.returncode == 0, out.stderr
     assert int(out.stdout) == (1 if torch_first else 2)
+
+
+def call_on_host_tensors():
+    """The checks a device call makes of every tensor, here on tensors of the host (which are on "device" -1)."""
+    import torch
+    from oak import _arrays
+    t = torch.zeros(1)
+    old, _arrays._contexts[-1] = _arrays._contexts.get(-1), type("Context", (), {"_h": 1})()
+    d = _arrays.Device(t)
+    if old is None:
+        del _arrays._contexts[-1]
+    return torch, d
+
+
+def test_zeros_without_storage_are_no_array_left_out():
+    torch, d = call_on_host_tensors()
+    from oak import _arrays
+    z = torch._efficientzerotensor((3, 2))
+    for a in (d.tensor(z, "a"), d.matrix(z, "a"), d.dense(z, "a", (3, 2)), d.matrix(z.t(), "a")):
+        assert a.data_ptr() == 0
+        with pytest.raises(ValueError, match="without storage"):
+            _arrays.ptr(a)
+    wide = d.dense(z, "a", (3, 2), torch.float64)            # the conversion made an array of it
+    assert _arrays.ptr(wide) is not None and (wide == 0).all()
+    assert _arrays.ptr(d.matrix(z.clone(), "a")) is not None and _arrays.ptr(d.matrix(torch.zeros(0, 2), "a")) is None
