@@ -38,10 +38,11 @@ def code_of(t, what: str) -> int:
 class Device:
     """The device and stream of one call, with its checks of every tensor."""
 
-    __slots__ = ("torch", "index", "ctx", "like")
+    __slots__ = ("torch", "index", "ctx", "like", "dual")
 
     def __init__(self, t):
         self.torch, self.like = _torch(), t
+        self.dual = getattr(self.torch.autograd.forward_ad, "_current_level", 0) >= 0        # a level of forward-mode differentiation is open
         self.index = t.get_device()
         self.ctx = _contexts.get(self.index)
         if self.ctx is None or self.ctx._h is None:
@@ -81,6 +82,8 @@ class Device:
             raise ValueError(f"{what} must be on {self.like.device} like the first array of the call")
         if a.requires_grad and self.torch.is_grad_enabled():
             raise ValueError(f"{what} requires grad: the operators record no graph, their gradients are calls of their own; pass {what}.detach()")
+        if self.dual and self.torch.autograd.forward_ad.unpack_dual(a).tangent is not None:
+            raise ValueError(f"{what} carries a forward-mode tangent, which the operators would drop; pass its primal")
         return a.resolve_neg() if a.is_neg() else a          # a view that negates when it is read
 
     def matrix(self, a, what: str, shape=None):

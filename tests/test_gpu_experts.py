@@ -575,3 +575,14 @@ def test_zeros_without_storage_are_refused():
         with pytest.raises(ValueError, match="without storage"):
             call()
     assert (ox.combine(F, z.clone(), p) == 0).all()
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    p = ox.plan(torch.tensor([[0, 1], [1, 2]], dtype=torch.int32, device="cuda"), 3)
+    F, w = torch.ones(4, 3, device="cuda"), torch.ones(2, 2, device="cuda")
+    with fwd.dual_level():
+        for call in (lambda: ox.combine(fwd.make_dual(F, F), w, p), lambda: ox.combine(F, fwd.make_dual(w, w), p), lambda: ox.route(fwd.make_dual(w, w), 1)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        assert (ox.combine(F, w, p) == 2).all()

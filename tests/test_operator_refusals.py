@@ -184,3 +184,22 @@ def test_zeros_without_storage_are_no_array_left_out():
     for a in (d.dense(z, "a", (3, 2), torch.float64), d.matrix(z.t(), "a")):           # the copy is an array of zeros
         assert _arrays.ptr(a) is not None and (a == 0).all()
     assert _arrays.ptr(d.matrix(z.clone(), "a")) is not None and _arrays.ptr(d.matrix(torch.zeros(0, 2), "a")) is None
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch
+    import torch.autograd.forward_ad as fwd
+    x = torch.ones(3, 2)
+    with fwd.dual_level():
+        _, d = call_on_host_tensors()
+        for make in (lambda t: fwd.make_dual(t, torch.ones_like(t)), lambda t: fwd.make_dual(t, torch.ones_like(t)).t()):
+            for call in (lambda t: d.tensor(t, "weights"), lambda t: d.matrix(t, "weights"), lambda t: d.dense(t, "weights", tuple(t.shape))):
+                with pytest.raises(ValueError, match="weights carries a forward-mode tangent"):
+                    call(make(x))
+        with torch.no_grad():
+            with pytest.raises(ValueError, match="tangent"):
+                d.tensor(fwd.make_dual(x, x), "weights")
+        assert d.tensor(x, "weights") is x                   # within a level, without a tangent
+        assert d.tensor(fwd.unpack_dual(fwd.make_dual(x, x)).primal, "weights").shape == x.shape
+    _, d = call_on_host_tensors()
+    assert d.tensor(x, "weights") is x
