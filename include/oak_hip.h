@@ -484,9 +484,11 @@ int oak_plan_device(oak_ctx* ctx, void* stream, const oak_plan_args* args);
 /* Row arrays have n_rows rows (ld_rows apart), slot arrays n_rows top_k rows (ld_slots apart) in the plan's order; places behind
    the last used one (offsets[n_experts]) are written as zeros where a slot array is an output.
    oak_dispatch:      dst slots[place] = src rows[row of the place]
-   oak_combine:       dst rows[n] = sum_j weights[n, j] src slots[positions[n, j]], slots without a place count as zeros;
+   oak_combine:       dst rows[n] = sum_j weights[n, j] src slots[positions[n, j]], a slot without a place has zeros for an answer, so that
+                      a NaN or infinite weight of such a slot makes its row NaN (oak_route's NaN weights show);
                       weights NULL: all 1 (the gradient of oak_dispatch)
-   oak_combine_grad:  src slots and dout rows (ld_grad apart) -> dslots [n_rows top_k, n_cols] contiguous, dweights [n_rows, top_k] */
+   oak_combine_grad:  src slots and dout rows (ld_grad apart) -> dslots [n_rows top_k, n_cols] contiguous, dweights [n_rows, top_k], 0 for slots
+                      without a place */
 typedef struct oak_mix_args {
     int64_t n_rows, ld_rows, ld_slots, ld_grad;
     int32_t top_k, n_experts, n_cols, dtype;

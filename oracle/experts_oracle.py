@@ -111,8 +111,8 @@ def combine(F, weights, positions):
     y = np.zeros((n, F.shape[1]))
     for i in range(n):
         for j in range(k):
-            if positions[i, j] >= 0:
-                y[i] += weights[i, j] * F[positions[i, j]]
+            with np.errstate(invalid="ignore"):              # no place: the weight times a row of zeros
+                y[i] += weights[i, j] * (F[positions[i, j]] if positions[i, j] >= 0 else 0.0)
     return y
 
 

@@ -307,13 +307,15 @@ def dispatch_grad(dlaid, plan: Plan):
 def combine(answers, weights, plan: Plan):
     """Sum over each row's experts of weight times answer, [N, C]; ``answers`` [N k, C] (or [N k]) in the plan's layout.
 
-    Slots without a place count as zeros.  What stands behind the last used place is not read.
+    The answer of a slot without a place is a row of zeros: its weight, if finite, leaves no trace, and one that is NaN or infinite makes the
+    row NaN, so that the NaN weights which :func:`route` gives a row it cannot route show in the sum.  What stands behind the last used
+    place is not read.
     """
     return _mix("combine", plan, answers, "answers", True, weights=_required(weights, "weights"))
 
 
 def combine_grad(answers, weights, plan: Plan, dout):
-    """Gradients of :func:`combine` from ``dout`` [N, C]: (danswers [N k, C], zeros behind the last used place; dweights [N, k])."""
+    """Gradients of :func:`combine` from ``dout`` [N, C]: (danswers [N k, C], zeros behind the last used place; dweights [N, k], 0 for slots without one)."""
     return _mix("combine_grad", plan, answers, "answers", True, weights=_required(weights, "weights"), dout=_required(dout, "dout"))
 
 

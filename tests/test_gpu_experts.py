@@ -586,3 +586,23 @@ def test_forward_mode_tangents_are_refused():
             with pytest.raises(ValueError, match="tangent"):
                 call()
         assert (ox.combine(F, w, p) == 2).all()
+
+
+@pytest.mark.parametrize("numpy", [False, True])
+def test_weights_of_slots_without_a_place(numpy):
+    """Their answer is a row of zeros: a finite weight leaves no trace, a NaN or infinite one shows, and the weight's gradient is 0."""
+    rng = np.random.default_rng(12)
+    ex = np.array([[0, -1], [-1, -1], [1, -1], [-1, 2], [2, 0], [-1, 1]], dtype=np.int32)
+    w = rng.standard_normal(ex.shape)
+    w[0, 1], w[1, 1], w[3, 0] = np.inf, np.nan, -np.inf
+    F, dy = rng.standard_normal((12, 5)), rng.standard_normal((6, 5))
+    put = (lambda a: a) if numpy else (lambda a: torch.as_tensor(a, device="cuda"))
+    get = (lambda a: a) if numpy else back
+    p = ox.plan(put(ex), 3)
+    y = get(ox.combine(put(F), put(w), p))
+    np.testing.assert_allclose(y, eo.combine(F, w, get(p.positions)), rtol=1e-13, atol=1e-13)
+    assert np.isnan(y[[0, 1, 3]]).all() and np.isfinite(y[[2, 4, 5]]).all()
+    dF, dw = map(get, ox.combine_grad(put(F), put(w), p, put(dy)))
+    for got, ref in zip((dF, dw), eo.combine_grad(F, w, get(p.positions), dy)):
+        np.testing.assert_allclose(got, ref, rtol=1e-13, atol=1e-13)
+    assert (dw[ex < 0] == 0).all() and np.isfinite(dF).all()
