@@ -410,3 +410,38 @@ def test_flat_rows_keep_the_digits_of_their_sum(n, v, dtype, t):
     tol = share * (abs(t) + 2 + vn) * u + u * ref
     loss = back(od.distill(s, top, idx))
     assert (np.abs(loss - ref) <= tol).all(), (np.abs(loss - ref).max() / u, tol / u)
+
+
+@pytest.mark.parametrize("teams,n,v,k,dtype,grad", [
+    (1 << 27, (1 << 27) + 100, 2, 1, "f16", True), (1 << 28, (1 << 28) + 100, 20, 2, "f64", False), (1 << 26, (1 << 26) + 100, 136, 2, "bf16", True),
+    (1 << 24, (1 << 24) + 100, 2100, 40, "bf16", False), (1 << 22, (1 << 22) + 100, 8200, 3, "bf16", True),
+    (1 << 22, (1 << 22) + 100, 33000, 70, "f16", False)])
+def test_a_teams_next_row_sees_nothing_of_its_last(teams, n, v, k, dtype, grad):
+    """A launch has teams for ``teams`` rows; the rows behind them are their second ones, whose teachers kept other classes (the student's row is
+    one row n times over).  A few rows in one launch are the reference, to the bit."""
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 2 * n * v * (2 if grad else 0) + (24 << 30):
+        pytest.skip("not enough free device memory")
+    rng = np.random.default_rng(v)
+    s = torch.as_tensor(rng.standard_normal((1, v)), device="cuda").to(DT[dtype])
+    top = torch.as_tensor(rng.standard_normal((1, k)), device="cuda", dtype=torch.float64 if dtype == "f64" else torch.float32)
+    lse = torch.logsumexp(top, 1) + 0.7
+    place = torch.arange(k, device="cuda", dtype=torch.int32) * max(1, v // (2 * k))
+
+    def run(rows, call):
+        r = torch.arange(rows, device="cuda", dtype=torch.int32)
+        first = (r + r // teams) % v                                     # classes of a team's second row: one further
+        out = call(s.expand(rows, v), top.expand(rows, k), (first[:, None] + place) % v, top_lse=lse.expand(rows))
+        return first, out
+
+    few = max(v, 257)                                                    # up to 256 rows another rule holds
+    _, (ref, gref) = run(few, od.distill_grad)
+    assert len(ref[:v].unique()) > 1
+    first, out = run(n, od.distill_grad if grad else od.distill)
+    loss = out[0] if grad else out
+    for a in range(0, n, 1 << 24):
+        assert torch.equal(loss[a:a + (1 << 24)], ref[first[a:a + (1 << 24)].long()]), a
+    if grad:
+        assert torch.equal(out[1][teams - 50:], gref[first[teams - 50:].long()])
+    del out, loss, gref, first
+    torch.cuda.empty_cache()
