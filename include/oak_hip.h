@@ -517,7 +517,8 @@ int oak_combine_grad_device(oak_ctx* ctx, void* stream, const oak_mix_args* args
      forward  L[n] = row_weight temperature^2 [ sum_k p_k log(p_k / q_k) + p_rest log(p_rest / q_rest) ]
      reverse  L[n] = row_weight temperature^2 [ sum_k q_k log(q_k / p_k) + q_rest log(q_rest / p_rest) ]   (needs top_lse; p_rest at
               least the resolution of top_lse, 2^-24 or for float64 2^-53)
-   dlogits (may be NULL) is the gradient of sum_n L[n].  A row of weight 0 is not read: its loss and gradient are 0.  A teacher that kept nothing
+   dlogits (may be NULL) is the gradient of sum_n L[n]; a teacher's mass sum p + p_rest within 2^-18 of 1 (top_lse of single precision) is
+   taken for 1 there.  A row of weight 0 is not read: its loss and gradient are 0.  A teacher that kept nothing
    has loss and gradient 0.  A row with an index outside [-1, n_classes) gets loss and gradient NaN. */
 #define OAK_KL_FORWARD 0
 #define OAK_KL_REVERSE 1

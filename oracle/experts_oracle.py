@@ -166,7 +166,8 @@ def distill(logits, top, index, top_lse=None, temperature=1.0, direction="forwar
                 terms = np.where(p > 0, p * (lp - lqt), 0.0)
                 kl = terms.sum() + (pr * (np.log(pr) - lqr) if pr > 0 else 0.0)
                 ratio = np.exp(np.log(pr) - lqr) if pr > 0 else 0.0
-                total = p.sum() + pr                             # 1 unless top_lse leaves no room for it
+                total = p.sum() + pr                             # the teacher's mass; 1 within what single precision leaves of top_lse
+                total = 1.0 if abs(total - 1.0) < 2.0 ** -18 else total
                 grad[i] = np.exp(lq) * (total - ratio)
                 grad[i, classes] = np.exp(lqt) * total - p
                 size[i] = factor * (np.abs(p * lp).sum() + np.abs(p * lqt).sum() + abs(pr * lqr) + 1.0 + ratio)

@@ -3,7 +3,8 @@
 // With z = log sum_v exp(s_v / tau), q_v = exp(s_v / tau - z), "top" the teacher's entries and "rest" every other class:
 //   forward  L = tau^2 w [ sum p_k (log p_k - log q_k) + p_r (log p_r - log q_r) ]
 //            dL/ds_v = tau w (S q_v - p_v) on the top,  tau w q_v (S - p_r / q_r) on the rest   (p_r = 0 without a rest outcome; S = sum p_k + p_r,
-//            which is 1 unless a rounded top_lse puts the entries' own sum above 1, or the entries are all the classes)
+//            1 unless the entries' own sum passes 1, as with a top_lse of 16 bits, or they are all the classes.  Off by less than 2^-18, as single
+//            precision leaves a top_lse of up to 32, it is taken for the 1 that it stands for)
 //   reverse  L = tau^2 w [ sum q_k (log q_k - log p_k) + q_r (log q_r - log p_r) ]
 //            dL/ds_v = tau w q_v (log q_b - log p_b - L / (tau^2 w)),  b the outcome v belongs to
 // so the gradient is one coefficient times q_v on the rest and k values of their own on the top.
@@ -357,7 +358,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
             } else {
                 pr = rest ? 1.0 - sums[0] : 0.0;
                 pr = pr < 0.0 ? 0.0 : pr;
-                total = pr > 0.0 ? 1.0 : sums[0];
+                total = pr > 0.0 || __builtin_fabs(sums[0] - 1.0) < 0x1p-18 ? 1.0 : sums[0];
                 kl = sums[1] - sums[2] * a.inv_tau + sums[0] * log_z;
             }
             if (a.reverse) {

@@ -42,7 +42,8 @@ def distill(logits, top, index, *, top_lse=None, temperature: float = 1.0, direc
 def distill_grad(logits, top, index, *, top_lse=None, temperature: float = 1.0, direction: str = "forward", row_weight=None):
     """(loss [N], gradient of their sum with respect to ``logits`` [N, V]) in one call; arguments as for :func:`distill`.
 
-    For the mean over rows, or any weighting of them, give ``row_weight``.
+    ``top_lse`` may be rounded: a kept mass above 1 stays what it is, in the loss and in its gradient (within 2^-18 of 1 it is taken for 1 in the
+    gradient).  For the mean over rows, or any weighting of them, give ``row_weight``.
     """
     return _distill(logits, top, index, top_lse, temperature, direction, row_weight, True)
 

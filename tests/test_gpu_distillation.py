@@ -445,3 +445,16 @@ def test_a_teams_next_row_sees_nothing_of_its_last(teams, n, v, k, dtype, grad):
         assert torch.equal(out[1][teams - 50:], gref[first[teams - 50:].long()])
     del out, loss, gref, first
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32"])
+def test_kept_mass_within_single_precision_of_1_is_1(dtype):
+    """All classes kept, top_lse rounded to float32: the gradient is q - p."""
+    s, top, idx, _ = problem(200, 20, 20, dtype, False)
+    low = torch.logsumexp(top.double(), 1).float()
+    loss, grad, _, _ = compare(s, top, idx, low.to(top.dtype), 1.0, "forward", None, dtype)
+    p = torch.exp(top.double() - low.double()[:, None])
+    want = torch.softmax(s.double(), 1).scatter_add_(1, idx, -p)
+    # beside the softmax's own error (see above; distances below 16 here) one rounding of the result
+    u = 2.0 ** -53 if dtype == "f64" else 2.0 ** -24
+    assert ((grad.double() - want).abs() <= 2 * (16 + 16) * u * (want.abs() + torch.softmax(s.double(), 1)) + (64 * u if dtype == "f64" else 0)).all()
