@@ -487,7 +487,7 @@ static int route_check(const oak_route_args* a) {
     OAK_REQUIRE(a->score == OAK_SCORE_SOFTMAX || a->score == OAK_SCORE_SIGMOID, "route: unknown score %d", a->score);
     OAK_REQUIRE(a->group_score == OAK_GROUP_MAX || a->group_score == OAK_GROUP_TOP2, "route: unknown group score %d", a->group_score);
     OAK_REQUIRE(a->scale - a->scale == 0.0, "route: scale is not finite");
-    OAK_REQUIRE(a->n_rows <= 1 || a->ld_scores >= 0, "route: negative row stride");
+    OAK_REQUIRE(a->n_rows <= 1 || (a->ld_scores >= 0 && (!a->mask || a->ld_mask >= 0)), "route: negative row stride");
     OAK_REQUIRE(a->n_rows == 0 || (a->scores && a->experts), "route: scores or experts are NULL");
     OAK_REQUIRE(a->n_rows <= MOST_SLOTS / a->top_k, "route: %lld rows x %d experts pass 2^31 slots", (long long)a->n_rows, a->top_k);
     return OAK_OK;

@@ -203,3 +203,11 @@ def test_forward_mode_tangents_are_refused():
         assert d.tensor(fwd.unpack_dual(fwd.make_dual(x, x)).primal, "weights").shape == x.shape
     _, d = call_on_host_tensors()
     assert d.tensor(x, "weights") is x
+
+
+@pytest.mark.parametrize("name", ["route", "route_grad"])
+def test_route_refuses_masks_that_run_backwards(name):
+    """Rows of a mask at a negative stride would be read from before its start, as those of scores would."""
+    refused(name, route_args(mask=ctypes.addressof(FAKE), ld_mask=-4), "stride")
+    for kw in (dict(mask=ctypes.addressof(FAKE), ld_mask=-4, n_rows=1), dict(mask=None, ld_mask=-4)):        # not used
+        refused(name, route_args(**kw), "ctx is NULL")
