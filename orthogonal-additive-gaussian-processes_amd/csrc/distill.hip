@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT, MODE == LONG ? 4 : 1) dis
             ref = a.lse ? load_any(a.lse, a.lse_dtype, row) : lanes_reduce<LEAD>(tmax, OpMax());
             xref = __builtin_fmax(lanes_reduce<LEAD>(xref, OpMax()), -1e300);
             for (int k = tid; k < a.K; k += LEAD) if (cls[k] >= 0) {
-                const double dt = tk[k] - ref, dx = ek[k] - xref, e = exp_of(dt > 1000.0 ? 1000.0 : dt), f = exp_of(dx * a.inv_tau);   // a top_lse below its entries: infinite
+                const double dt = tk[k] - ref, dx = ek[k] - xref, e = exp_of(dt > 1000.0 ? 1000.0 : dt), f = exp_of(dx * a.inv_tau);   // a top_lse far below its entries: no finite loss
                 tk[k] = dt; pk[k] = e; ek[k] = f;
                 sums[0] += e;
                 if (e != 0.0) { sums[1] += e * dt; sums[2] += e * dx; }
@@ -517,9 +517,9 @@ static int distill_launch(hipStream_t stream, const oak_distill_args* a) {
         if (units <= 512) return distill_run<T, 64, 8>(stream, d);
         if (units <= 1024) return distill_run<T, 64, 16>(stream, d);
         if (units <= 2048) return distill_run<T, 256, 8>(stream, d);
-        if (units <= 4096) return distill_run<T, 256, 16>(stream, d);                  // 4096 x 32768 bf16: 119 us (4.5 TB/s), read twice 146
+        if (units <= 4096) return distill_run<T, 256, 16>(stream, d);                  // 4096 x 32768 bf16: 117 us (4.6 TB/s), read twice 146
         // Longer rows: what 512 threads can hold with two workgroups a compute unit, the rest is read twice, the second time out of the last cache
-        // (2 x 256 rows in flight fit it up to 2^18 bf16 classes, and the gradient passes it by).  2048 x 131072 bf16: 250 us (265 when this was
+        // (2 x 256 rows in flight fit it up to 2^18 bf16 classes, and the gradient passes it by).  2048 x 131072 bf16: 241 us (265 when this was
         // chosen; all of it read twice 279; the whole row in the registers of 1024 threads, one workgroup a unit, 330).
         return distill_run<T, 512, 8, LONG>(stream, d);
     });

@@ -26,7 +26,7 @@ template <typename T> struct Vec {
 inline size_t dtype_size(int dtype) { return dtype == OAK_F64 ? 8 : dtype == OAK_F32 ? 4 : 2; }
 inline size_t dtype_acc_size(int dtype) { return dtype == OAK_F64 ? 8 : 4; }
 
-// calls fn.template operator()<T>() for the element type of a run-time code
+// calls fn(T value) for the element type T of a run-time code
 template <typename F> inline int with_dtype(int dtype, F&& fn) {
     switch (dtype) {
         case OAK_F64: return fn((double)0);
@@ -101,7 +101,7 @@ __device__ __forceinline__ double fma_const(double a, double b, double c) {
     return d;
 }
 // Cody-Waite reduction and the Taylor polynomial of degree 13 on |r| <= ln 2 / 2 (remainder 4e-18), without the special cases of exp();
-// for t < 709, NaN stays NaN
+// beyond t = 709.8 infinite (t of at most 1e9, so that n fits 32 bits), NaN stays NaN
 __device__ __forceinline__ double exp_of(double t) {
     t = t < -800.0 ? -800.0 : t;
     const double n = __builtin_rint(t * 1.4426950408889634074);

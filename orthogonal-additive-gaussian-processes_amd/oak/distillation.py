@@ -1,9 +1,11 @@
 """Training against another model's class probabilities of which only the highest logits are kept.
 
-A black-box teacher (any classifier, whatever its number of classes) is distilled into a student of this package: the
-teacher's ``k`` highest logits of every row are stored once, and :func:`distill_grad` gives the divergence of the student's
-distribution from the teacher's and its gradient with respect to the student's logits, to be chained into the student (through
-:func:`oak.experts.combine_grad` into a mixture's experts and router).
+A black-box teacher (any classifier, whatever its number of classes) is distilled into a student: the teacher's ``k`` highest
+logits of every row are stored once, and :func:`distill_grad` gives the divergence of the student's distribution from the teacher's
+and its gradient with respect to the student's logits.  The caller chains that gradient into what made the logits: the weights of
+features (a model's Gram matrix columns, say), or through :func:`oak.experts.combine_grad` and :func:`oak.experts.route_grad` a
+mixture's answers and router.  The models' own kernel parameters are not reached: their gradients in this package are those of the
+bound and of the log marginal likelihood.
 
 Arrays are NumPy arrays (float64; results are NumPy arrays) or torch tensors on a HIP device (logits of type float64, float32, bfloat16 or float16;
 results on the same device, computed on its current stream without waiting for them).  Losses are float64 for float64 logits
