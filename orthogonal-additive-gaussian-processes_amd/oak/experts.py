@@ -83,8 +83,9 @@ def route(scores, top_k: int, *, score: str = "softmax", bias=None, n_groups: in
     ``scores`` [N, E] become probabilities p by ``score`` = "softmax" (over the row's open experts) or "sigmoid".  An expert is
     open to a row unless ``mask`` [N, E] or [E] is False there or its score is -inf.  The choice goes by p + ``bias`` [E] (a balance
     correction of size below 1e300: it moves the choice, not the weights; -inf closes its expert to the choice), highest
-    first, ties to the lower index.  With ``n_groups`` > 1 the experts form groups of consecutive ones, of which the ``top_groups`` best stay open; ``group_score`` = "max" ranks them by their best expert,
-    "top2" by the sum of their two best.  weights = ``scale`` * p, divided by the chosen experts' sum if ``renormalise``.
+    first, ties to the lower index.  With ``n_groups`` > 1 the experts form groups of consecutive ones, of which the
+    ``top_groups`` best stay open; ``group_score`` = "max" ranks them by their best expert, "top2" by the sum of their two
+    best.  weights = ``scale`` * p, divided by the chosen experts' sum if ``renormalise``.
 
     Slots that no open expert is left for hold expert -1 and weight 0.  A row with a NaN or +inf among its open scores holds
     experts -1 and weights NaN.  A NaN or +inf in ``bias`` is refused in a NumPy array; on a device it counts like such a score of
